@@ -245,7 +245,7 @@ def _plain_distill(s):
         logq = log_softmax(torch.where(some[:, None], teacher, 0.0))
     q = torch.where(valid, logq.exp(), 0.0)
     soft = torch.where(q > 0, q * (logq - logp_t.gather(-1, ids)), 0.0).sum(-1)
-    ratio = torch.zeros_like(soft)
+    ratio, mass = torch.zeros_like(soft), q.sum(-1)
     if c["tail"]:
         # what the teacher and the student leave outside of the listed entries
         q_rest = (1.0 - q.double().sum(-1)).clamp(min=0).float()
@@ -254,6 +254,7 @@ def _plain_distill(s):
         rest = (q_rest > 0) & (p_rest > 0)
         soft = soft + torch.where(rest, q_rest * (q_rest.log() - p_rest.log()), 0.0)
         ratio = torch.where(rest, q_rest / p_rest, 0.0)
+        mass = mass + torch.where(rest, q_rest, 0.0)
     loss = torch.where(some, alpha * t * t * soft, 0.0)
     labelled = None
     if alpha < 1:
@@ -263,9 +264,9 @@ def _plain_distill(s):
         loss = loss + torch.where(labelled, -(1 - alpha) * logp.gather(-1, label)[:, 0], 0.0)
     if c["dir"] == "fwd":
         return loss
-    p = logp_t.exp()
+    p = logp_t.exp() * mass[:, None]           # the mass is 1 but for roundings of the teacher's logits
     if c["tail"]:
-        p = torch.where(inside, p, p * (1 - ratio[:, None]))
+        p = torch.where(inside, p, p - logp_t.exp() * ratio[:, None])
     dz = torch.where(some[:, None], alpha * t * p.scatter_add(-1, ids, -q), 0.0)
     if alpha < 1:
         d = logp.exp().scatter_add(-1, label, -torch.ones_like(logp[:, :1]))

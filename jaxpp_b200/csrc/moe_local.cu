@@ -239,6 +239,106 @@ __global__ void __launch_bounds__(1024) slots_kernel(const long long* __restrict
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------
+// Picks sorted by expert, those of an expert in their own order, nothing dropped.  The picks are cut into one run per CTA:
+// the first kernel counts the picks of every expert in every run (`hist` [runs][E]); in the second, each CTA adds up the
+// counts of all runs (the experts' totals, whose sums are the offsets) and of the runs before its own, and places its picks
+// 1024 at a time as slots_kernel does.  Picks that name no expert have no place, and the places behind the last one no pick.
+// ---------------------------------------------------------------------------------------------------------
+constexpr int ORDER_MAX_E = 256;
+__device__ __forceinline__ int order_pick(const long long* __restrict__ top_i, int i, int end, int E) {
+  if (i >= end) return -1;
+  const long long e = top_i[i];
+  return e >= 0 && e < E ? int(e) : -1;
+}
+__global__ void __launch_bounds__(1024) order_count_kernel(const long long* __restrict__ top_i, int* __restrict__ hist, int n, int E, int run) {
+  __shared__ int count[ORDER_MAX_E];
+  for (int e = threadIdx.x; e < E; e += 1024) count[e] = 0;
+  __syncthreads();
+  const int first = blockIdx.x * run, end = min(n, first + run);
+  for (int i = first + int(threadIdx.x); i < end; i += 1024) {
+    const int e = order_pick(top_i, i, end, E);
+    if (e >= 0) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += 1024) hist[size_t(blockIdx.x) * E + e] = count[e];
+}
+__global__ void __launch_bounds__(1024) order_place_kernel(const long long* __restrict__ top_i, const int* __restrict__ hist,
+                                                           long long* __restrict__ dest, int* __restrict__ inv, int* __restrict__ offsets,
+                                                           int n, int E, int run) {
+  __shared__ int warp_count[32][ORDER_MAX_E + 1];
+  __shared__ int total[ORDER_MAX_E], before[ORDER_MAX_E];   // picks of an expert, and those in the runs before this one
+  __shared__ int placed;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  for (int e = tid; e < E; e += 1024) total[e] = before[e] = 0;
+  __syncthreads();
+  for (int i = tid; i < int(gridDim.x) * E; i += 1024) {
+    const int c = hist[i], r = i / E, e = i - r * E;
+    if (c == 0) continue;
+    atomicAdd(&total[e], c);
+    if (r < int(blockIdx.x)) atomicAdd(&before[e], c);
+  }
+  __syncthreads();
+  if (warp == 0) {                                          // offsets: running sum of the totals
+    int base = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int c = e0 + lane < E ? total[e0 + lane] : 0;
+      int sum = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      if (e0 + lane < E) {
+        before[e0 + lane] += base + sum - c;
+        if (blockIdx.x == 0) offsets[e0 + lane] = base + sum - c;
+      }
+      base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) {
+      placed = base;
+      if (blockIdx.x == 0) offsets[E] = base;
+    }
+  }
+  __syncthreads();
+  const int first = blockIdx.x * run, end = min(n, first + run);
+  for (int at = first; at < end; at += 1024) {
+    for (int e = lane; e < E; e += 32) warp_count[warp][e] = 0;
+    __syncwarp();
+    const int i = at + tid;
+    const int e = order_pick(top_i, i, end, E);
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    if (e >= 0 && rank == 0) warp_count[warp][e] = __popc(same);
+    __syncthreads();
+    for (int x = warp; x < E; x += 32) {                    // counts of expert x in the 32 warps -> places
+      const int c = warp_count[lane][x];
+      int sum = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const int b = before[x];
+      __syncwarp();
+      warp_count[lane][x] = b + sum - c;
+      if (lane == 31) before[x] = b + sum;
+    }
+    __syncthreads();
+    if (i < end) {
+      const int place = e >= 0 ? warp_count[warp][e] + rank : n;
+      dest[i] = place;
+      if (e >= 0) inv[place] = i;
+    }
+    __syncthreads();
+  }
+  for (int i = placed + int(blockIdx.x) * 1024 + tid; i < n; i += int(gridDim.x) * 1024) inv[i] = -1;
+}
+static int order_run(int n) {   // picks of a CTA: whole steps of 1024, at most 128 CTAs
+  const long long steps = ((long long)n + 1023) / 1024;
+  return int((steps + 127) / 128) * 1024;
+}
+
 // out[slot] = x[inv[slot] / k], zeros where the slot is empty
 template <typename T>
 __global__ void dispatch_rows_kernel(const T* __restrict__ x, const int* __restrict__ inv, T* __restrict__ out, int slots, int d, int k) {
@@ -395,6 +495,25 @@ JPB_API int jpb_moe_slots(const long long* top_i, long long* dest, int* inv, int
   using namespace jpb;
   if (E < 1 || E > MOE_MAX_E || C < 0 || n < 0 || (long long)E * C > 0x7fffffffll) return -JPB_ERR_BAD_ARGUMENT;
   slots_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(top_i, dest, inv, counts, n, E, C);
+  return int(cudaGetLastError());
+}
+
+// int32 elements of scratch for jpb_expert_order.
+JPB_API long long jpb_expert_order_scratch_elems(int n, int E) {
+  if (n <= 0) return E;
+  const int run = jpb::order_run(n);
+  return ((long long)n + run - 1) / run * E;
+}
+// top_i [n] int64 -> dest [n] int64 (place of each pick, n where it names none of the E experts), inv [n] int32 (pick of each
+// place, or -1), offsets [E + 1] int32.  E <= 256.
+JPB_API int jpb_expert_order(const long long* top_i, long long* dest, int* inv, int* offsets, int* scratch, int n, int E, void* stream) {
+  using namespace jpb;
+  if (E < 1 || E > ORDER_MAX_E || n < 0 || n > 0x7fffffff - (1 << 24)) return -JPB_ERR_BAD_ARGUMENT;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n == 0) return int(cudaMemsetAsync(offsets, 0, sizeof(int) * (E + 1), s));
+  const int run = order_run(n), runs = int(((long long)n + run - 1) / run);
+  order_count_kernel<<<runs, 1024, 0, s>>>(top_i, scratch, n, E, run);
+  order_place_kernel<<<runs, 1024, 0, s>>>(top_i, scratch, dest, inv, offsets, n, E, run);
   return int(cudaGetLastError());
 }
 

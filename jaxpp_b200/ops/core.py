@@ -48,8 +48,9 @@ def _use_native(t: Tensor) -> bool:
     return t.is_cuda and config.use_native_kernels.value
 
 
-def _define(schema: str, ref_impl, fake_impl, native_name: str | None = None):
-    """Register ``b200::<schema>`` with reference, fake and (optional) native implementations."""
+def _define(schema: str, ref_impl, fake_impl, native_name: str | None = None, check=None):
+    """Register ``b200::<schema>`` with reference, fake and (optional) native implementations; ``check`` raises on arguments
+    that none of them takes."""
     name = schema.split("(")[0]
     _lib.define(schema)
     qual = f"b200::{name}"
@@ -57,14 +58,23 @@ def _define(schema: str, ref_impl, fake_impl, native_name: str | None = None):
     if native_name is None:
         impl = ref_impl
     else:
-        def impl(*args, __ref=ref_impl, __nn=native_name):
+        def impl(*args, __ref=ref_impl, __nn=native_name, __check=check):
+            if __check is not None:
+                __check(*args)
             first = next(a for a in args if isinstance(a, Tensor))
             if _use_native(first):
                 return getattr(_native(), __nn)(*args)
             return __ref(*args)
 
     _lib.impl(name, impl, "CompositeExplicitAutograd")
-    torch.library.register_fake(qual, fake_impl)
+    if check is None:
+        torch.library.register_fake(qual, fake_impl)
+    else:
+        def fake(*args, __fake=fake_impl, __check=check):
+            __check(*args)
+            return __fake(*args)
+
+        torch.library.register_fake(qual, fake)
     DIRECT[getattr(torch.ops.b200, name).default] = impl
     return getattr(torch.ops.b200, name)
 
@@ -216,6 +226,93 @@ _autograd("linear_batched", _linear_batched_bwd, _linear_batched_setup)
 
 
 # ======================================================================================
+# products grouped by ragged rows: rows offsets[e] .. offsets[e+1] of x belong to group (expert) e
+#   y[t] = x[t] @ w[e(t)]^T   x [T, K], w [E, N, K], offsets [E + 1] int32 -> [T, N]
+# Groups may have any length, none included.  Rows in front of offsets[0] and behind offsets[E] belong to no group: they
+# give zeros and add to no gradient, whatever they hold.  The offsets are read on the device (no synchronisation); values
+# that decrease or leave 0 .. T are taken as the nearest ones that do not.
+# ======================================================================================
+
+def _check_ragged(rows, w, offsets, width, what):
+    if rows.dim() != 2 or w.dim() != 3 or rows.shape[1] != w.shape[width]:
+        raise ValueError(f"{what}: rows {tuple(rows.shape)} and weights {tuple(w.shape)} do not go together "
+                         f"([T, {w.shape[width] if w.dim() == 3 else '?'}] and [E, N, K] are wanted)")
+    _check_offsets(rows, offsets, w.shape[0], what)
+
+
+def _check_offsets(rows, offsets, groups, what):
+    if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.shape[0] < 2 or (groups is not None and offsets.shape[0] != groups + 1):
+        raise ValueError(f"{what}: offsets are [groups + 1] int32, got {tuple(offsets.shape)} {offsets.dtype}")
+    if offsets.device != rows.device:
+        raise ValueError(f"{what}: offsets are on {offsets.device}, the rows on {rows.device}")
+
+
+def _ragged_bounds(offsets, rows: int) -> list:
+    o = offsets.clamp(0, rows).cummax(0).values.tolist()
+    return list(zip(o, o[1:]))
+
+
+def _linear_ragged_ref(x, w, offsets):
+    out = x.new_zeros(x.shape[0], w.shape[1])
+    for e, (a, b) in enumerate(_ragged_bounds(offsets, x.shape[0])):
+        out[a:b] = x[a:b] @ w[e].t()
+    return out
+
+
+def _linear_ragged_dgrad_ref(dy, w, offsets):
+    out = dy.new_zeros(dy.shape[0], w.shape[2])
+    for e, (a, b) in enumerate(_ragged_bounds(offsets, dy.shape[0])):
+        out[a:b] = dy[a:b] @ w[e]
+    return out
+
+
+def _check_ragged_wgrad(dy, x, offsets, out_dtype=None):
+    if dy.dim() != 2 or x.dim() != 2 or dy.shape[0] != x.shape[0]:
+        raise ValueError(f"linear_ragged_wgrad: dy {tuple(dy.shape)} and x {tuple(x.shape)} are [T, N] and [T, K]")
+    _check_offsets(x, offsets, None, "linear_ragged_wgrad")
+
+
+def _linear_ragged_wgrad_ref(dy, x, offsets, out_dtype=None):
+    parts = [_f32(dy[a:b]).t() @ _f32(x[a:b]) for a, b in _ragged_bounds(offsets, x.shape[0])]
+    return torch.stack(parts).to(_wg_dtype(dy, out_dtype))
+
+
+linear_ragged = _define(
+    "linear_ragged(Tensor x, Tensor w, Tensor offsets) -> Tensor",
+    _linear_ragged_ref,
+    lambda x, w, offsets: x.new_empty(x.shape[0], w.shape[1]),
+    "linear_ragged", lambda x, w, offsets: _check_ragged(x, w, offsets, 2, "linear_ragged"),
+)
+linear_ragged_dgrad = _define(
+    "linear_ragged_dgrad(Tensor dy, Tensor w, Tensor offsets) -> Tensor",
+    _linear_ragged_dgrad_ref,
+    lambda dy, w, offsets: dy.new_empty(dy.shape[0], w.shape[2]),
+    "linear_ragged_dgrad", lambda dy, w, offsets: _check_ragged(dy, w, offsets, 1, "linear_ragged_dgrad"),
+)
+linear_ragged_wgrad = _define(
+    "linear_ragged_wgrad(Tensor dy, Tensor x, Tensor offsets, ScalarType? out_dtype=None) -> Tensor",
+    _linear_ragged_wgrad_ref,
+    lambda dy, x, offsets, out_dtype=None: dy.new_empty(offsets.shape[0] - 1, dy.shape[1], x.shape[1], dtype=_wg_dtype(dy, out_dtype)),
+    "linear_ragged_wgrad", _check_ragged_wgrad,
+)
+
+
+def _linear_ragged_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _linear_ragged_bwd(ctx, dy):
+    x, w, offsets = ctx.saved_tensors
+    dy = dy.contiguous()
+    dx = linear_ragged_dgrad(dy, w, offsets) if ctx.needs_input_grad[0] else None
+    dw = linear_ragged_wgrad(dy, x, offsets, WGRAD_DTYPE[0]) if ctx.needs_input_grad[1] else None
+    return dx, dw, None
+
+
+_autograd("linear_ragged", _linear_ragged_bwd, _linear_ragged_setup)
+
+
+# ======================================================================================
 # RMSNorm / LayerNorm (statistics in fp32)
 # ======================================================================================
 
@@ -348,6 +445,139 @@ def _layernorm_autograd(ctx, dy, _dm, _dr):
 
 
 _autograd("layernorm", _layernorm_autograd, _layernorm_setup)
+
+
+# ======================================================================================
+# Residual connection of a block whose output is normalised as well as its input:
+#   r = scale * x + gate * n,   n = RMSNorm(y) * w_post   (w_post None: n = y;  gate None: 1)
+#   h = RMSNorm(r) * w_pre                                (w_pre None: no h, an empty tensor)
+# x is the residual stream, y the block's output, r the new stream and h the next block's input.  gate is one vector [d] or
+# [G, d]: one for each of G runs of rows / G consecutive rows (the sequences of a batch, or every row).  h is computed from r
+# before r is rounded to the stream's type, and the gradients are those of that function: they take x and y, not r.
+# ======================================================================================
+
+def _check_residual_norm(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
+    d = x.shape[-1] if x.dim() else 0
+    if x.shape != y.shape or x.dtype != y.dtype or x.dim() < 1:
+        raise ValueError(f"residual_norm: x {tuple(x.shape)} {x.dtype} and y {tuple(y.shape)} {y.dtype} have to be alike")
+    for name, w in (("w_post", w_post), ("w_pre", w_pre)):
+        if w is not None and (tuple(w.shape) != (d,) or w.dtype != x.dtype):
+            raise ValueError(f"residual_norm: {name} is [{d}] {x.dtype}, got {tuple(w.shape)} {w.dtype}")
+    if gate is not None:
+        rows = x.numel() // d if d else 0
+        if (gate.dim() not in (1, 2) or gate.shape[-1] != d or gate.dtype != x.dtype
+                or (gate.dim() == 2 and (gate.shape[0] == 0 or rows % gate.shape[0]))):
+            raise ValueError(f"residual_norm: gate is [{d}] or [G, {d}] {x.dtype} with G a divisor of the {rows} rows, "
+                             f"got {tuple(gate.shape)} {gate.dtype}")
+
+
+def _residual_parts(x, y, w_post, gate, rstd_post, scale):
+    d = x.shape[-1]
+    xf, yf = _f32(x).reshape(-1, d), _f32(y).reshape(-1, d)
+    p = yf if w_post is None else yf * rstd_post.reshape(-1, 1)
+    n = p if w_post is None else p * _f32(w_post)
+    if gate is None:
+        g = torch.ones((), dtype=torch.float32, device=x.device)
+    else:
+        g = _f32(gate).reshape(-1, d)
+        g = g.repeat_interleave(xf.shape[0] // g.shape[0], 0)
+    return p, n, g, scale * xf + g * n
+
+
+def _residual_norm_ref(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
+    none = x.new_empty(0)
+    no_rstd = x.new_empty(0, dtype=torch.float32)
+    rstd_post = no_rstd if w_post is None else torch.rsqrt(_f32(y).pow(2).mean(-1) + eps)
+    r = _residual_parts(x, y, w_post, gate, rstd_post, scale)[3].view(x.shape)
+    if w_pre is None:
+        return r.to(x.dtype), none, rstd_post, no_rstd.clone()
+    rstd_pre = torch.rsqrt(r.pow(2).mean(-1) + eps)
+    return r.to(x.dtype), (r * rstd_pre.unsqueeze(-1) * _f32(w_pre)).to(x.dtype), rstd_post, rstd_pre
+
+
+def _residual_norm_fake(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
+    stat = lambda w: x.new_empty((0,) if w is None else x.shape[:-1], dtype=torch.float32)
+    return x.new_empty(x.shape), x.new_empty((0,) if w_pre is None else x.shape), stat(w_post), stat(w_pre)
+
+
+residual_norm = _define(
+    "residual_norm(Tensor x, Tensor y, Tensor? w_post, Tensor? gate, Tensor? w_pre, float scale=1.0, float eps=1e-5)"
+    " -> (Tensor, Tensor, Tensor, Tensor)",
+    _residual_norm_ref, _residual_norm_fake, "residual_norm", _check_residual_norm,
+)
+
+
+def _check_residual_norm_bwd(dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre, scale=1.0, sum_dtype=None):
+    _check_residual_norm(x, y, w_post, gate, w_pre)
+    rows = x.shape[:-1]
+    for name, t in (("dr", dr), ("dh", dh if w_pre is not None else None)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"residual_norm_bwd: {name} {tuple(t.shape)} {t.dtype} is not like x")
+    for name, w, t in (("rstd_post", w_post, rstd_post), ("rstd_pre", w_pre if dh is not None else None, rstd_pre)):
+        if w is not None and (t.shape != rows or t.dtype != torch.float32):
+            raise ValueError(f"residual_norm_bwd: {name} is {tuple(rows)} float32, got {tuple(t.shape)} {t.dtype}")
+
+
+def _residual_norm_bwd_ref(dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre, scale=1.0, sum_dtype=None):
+    d = x.shape[-1]
+    p, n, g, r = _residual_parts(x, y, w_post, gate, rstd_post, scale)
+    none = x.new_empty(0)
+    dw_post = dgate = dw_pre = None
+    dR = torch.zeros_like(r) if dr is None else _f32(dr).reshape(-1, d)
+    if w_pre is not None:
+        if dh is None:
+            dw_pre = torch.zeros(d, dtype=torch.float32, device=x.device)
+        else:
+            rstd = rstd_pre.reshape(-1, 1)
+            hat, u = r * rstd, _f32(dh).reshape(-1, d)
+            dw_pre = (u * hat).sum(0)
+            u = u * _f32(w_pre)
+            dR = dR + rstd * (u - hat * (u * hat).mean(-1, keepdim=True))
+    if gate is not None:
+        groups = gate.numel() // d
+        dgate = (dR * n).reshape(groups, dR.shape[0] // groups, d).sum(1).view(gate.shape)
+    dn = dR * g
+    if w_post is None:
+        dy = dn
+    else:
+        dw_post = (dn * p).sum(0)
+        v = dn * _f32(w_post)
+        dy = rstd_post.reshape(-1, 1) * (v - p * (v * p).mean(-1, keepdim=True))
+    out = lambda t: none.clone() if t is None else t.to(sum_dtype or x.dtype)
+    return (scale * dR).to(x.dtype).view(x.shape), dy.to(x.dtype).view(x.shape), out(dw_post), out(dgate), out(dw_pre)
+
+
+def _residual_norm_bwd_fake(dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre, scale=1.0, sum_dtype=None):
+    like = lambda w: x.new_empty(0) if w is None else x.new_empty(w.shape, dtype=sum_dtype or x.dtype)
+    return x.new_empty(x.shape), x.new_empty(x.shape), like(w_post), like(gate), like(w_pre)
+
+
+# dr / dh None: nothing arrives over that output.  ``sum_dtype``: as for ``rmsnorm_bwd``.
+residual_norm_bwd = _define(
+    "residual_norm_bwd(Tensor? dr, Tensor? dh, Tensor x, Tensor y, Tensor? w_post, Tensor? gate, Tensor? w_pre, Tensor rstd_post,"
+    " Tensor rstd_pre, float scale=1.0, ScalarType? sum_dtype=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    _residual_norm_bwd_ref, _residual_norm_bwd_fake, "residual_norm_bwd", _check_residual_norm_bwd,
+)
+
+
+def _residual_norm_setup(ctx, inputs, output):
+    x, y, w_post, gate, w_pre, ctx.scale, _ = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, y, w_post, gate, w_pre, output[2], output[3])
+
+
+def _residual_norm_autograd(ctx, dr, dh, _dpost, _dpre):
+    x, y, w_post, gate, w_pre, rstd_post, rstd_pre = ctx.saved_tensors
+    if w_pre is None:
+        dh = None
+    if dr is None and dh is None:
+        return (None,) * 7
+    dr, dh = (None if t is None else t.contiguous() for t in (dr, dh))
+    dx, dy, dw_post, dgate, dw_pre = residual_norm_bwd(dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre, ctx.scale)
+    return (dx, dy, None if w_post is None else dw_post, None if gate is None else dgate, None if w_pre is None else dw_pre, None, None)
+
+
+_autograd("residual_norm", _residual_norm_autograd, _residual_norm_setup)
 
 
 # ======================================================================================
@@ -698,6 +928,122 @@ _autograd("cross_entropy", _ce_autograd, _ce_setup)
 
 
 # ======================================================================================
+# Distillation from the top logits of a teacher: a row's loss is
+#   alpha * temperature^2 * KL(q || p)  +  (1 - alpha) * cross_entropy(logits, label)
+# with p = softmax(logits / temperature) and q the teacher's distribution over the K entries that it left for the row:
+# teacher_ids [.., K] (int32 or int64; an id outside of 0 .. V-1 is no entry) and teacher_logits [.., K].
+#   teacher_lse None:  q = softmax(teacher_logits / temperature) over the row's entries
+#   teacher_lse [..]:  the log-sum-exp of ALL the teacher's logits over the temperature; q = exp(teacher_logits / temperature -
+#                      teacher_lse), and what q leaves is held against what p leaves outside of the entries, as one more class
+# An id that a row lists twice has the sum of both probabilities as far as p is concerned: each entry is a term of its own.
+# Rows without an entry have no first term, rows with a label outside of 0 .. V-1 no second one (labels None: no row has it).
+# ``distill_loss_grad`` gives the losses together with the gradient of the logits for row weights ``dloss`` that are known
+# beforehand: the logits are read once.  The gradient of ``distill_loss`` is that op too.
+# ======================================================================================
+
+def _check_distill(dloss, logits, ids, top, lse, labels, temperature=1.0, alpha=1.0):
+    rows = logits.shape[:-1]
+    if logits.dim() < 1 or ids.shape != top.shape or ids.dim() != logits.dim() or ids.shape[:-1] != rows:
+        raise ValueError(f"distill_loss: logits {tuple(logits.shape)}, teacher_ids {tuple(ids.shape)} and teacher_logits "
+                         f"{tuple(top.shape)} are [.., V], [.., K] and [.., K]")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"distill_loss: teacher_ids are int32 or int64, got {ids.dtype}")
+    if lse is not None and (lse.shape != rows or lse.dtype != torch.float32):
+        raise ValueError(f"distill_loss: teacher_lse is {tuple(rows)} float32, got {tuple(lse.shape)} {lse.dtype}")
+    if labels is not None and (labels.shape != rows or labels.dtype != torch.int64):
+        raise ValueError(f"distill_loss: labels are {tuple(rows)} int64, got {tuple(labels.shape)} {labels.dtype}")
+    if dloss is not None and dloss.shape != rows:
+        raise ValueError(f"distill_loss_grad: dloss is {tuple(rows)}, got {tuple(dloss.shape)}")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"distill_loss: temperature has to be positive, got {temperature}")
+    if not 0 <= alpha <= 1:
+        raise ValueError(f"distill_loss: alpha has to lie between 0 and 1, got {alpha}")
+
+
+def _distill_ref(dloss, logits, ids, top, lse, labels, temperature, alpha):
+    shape, V, t = logits.shape, logits.shape[-1], temperature
+    z = _f32(logits).reshape(-1, V)
+    ids, top = ids.reshape(z.shape[0], ids.shape[-1]).long(), _f32(top).reshape(z.shape[0], top.shape[-1]) / t
+    ninf = torch.full((), float("-inf"), device=z.device)
+    valid = (ids >= 0) & (ids < V) & (top != ninf)
+    some = valid.any(-1, keepdim=True)
+    ids, top = ids.masked_fill(~valid, 0), torch.where(valid, top, ninf)
+    logp = torch.log_softmax(z / t, -1)
+    if lse is None:
+        logq = torch.log_softmax(torch.where(some, top, torch.zeros_like(top)), -1) if top.shape[1] else top
+    else:
+        logq = top - lse.reshape(-1, 1)
+    q = torch.where(valid, logq.exp(), torch.zeros_like(top))
+    soft = torch.where(q > 0, q * (logq - logp.gather(-1, ids)), torch.zeros_like(q)).sum(-1)
+    p = logp.exp()
+    mass = q.sum(-1)
+    if lse is not None:
+        q_rest = (1.0 - q.sum(-1, dtype=torch.float64)).clamp(min=0).float()
+        inside = torch.zeros_like(z).scatter_add(-1, ids, valid.float()) > 0
+        p_rest = p.masked_fill(inside, 0.0).sum(-1)
+        rest = (q_rest > 0) & (p_rest > 0)
+        one = torch.ones_like(p_rest)
+        ratio = torch.where(rest, q_rest / torch.where(rest, p_rest, one), torch.zeros_like(one))
+        soft = soft + torch.where(rest, q_rest * torch.where(rest, ratio, one).log(), torch.zeros_like(one))
+        mass = mass + torch.where(rest, q_rest, torch.zeros_like(one))
+        p = p * torch.where(inside, mass.unsqueeze(-1), (mass - ratio).unsqueeze(-1))
+    else:
+        p = p * mass.unsqueeze(-1)
+    has = some.squeeze(-1)
+    loss = torch.where(has, alpha * t * t * soft, torch.zeros_like(soft))
+    dz = None
+    if dloss is not None:
+        dz = torch.where(some, alpha * t * p.scatter_add(-1, ids, -q), torch.zeros_like(p))
+    if labels is not None and alpha < 1:
+        lab = labels.reshape(-1)
+        on = (lab >= 0) & (lab < V)
+        lab = lab.masked_fill(~on, 0).unsqueeze(-1)
+        logp = torch.log_softmax(z, -1)
+        loss = loss + torch.where(on, -(1 - alpha) * logp.gather(-1, lab).squeeze(-1), torch.zeros_like(loss))
+        if dz is not None:
+            d = logp.exp().scatter_add(-1, lab, -torch.ones_like(logp[:, :1]))
+            dz = dz + torch.where(on.unsqueeze(-1), (1 - alpha) * d, torch.zeros_like(d))
+    loss = loss.view(shape[:-1])
+    if dloss is None:
+        return loss
+    # a row of weight zero has no gradient, whatever its logits are
+    w = _f32(dloss).reshape(-1, 1)
+    return loss, torch.where(w != 0, dz * w, torch.zeros_like(dz)).to(logits.dtype).view(shape)
+
+
+distill_loss = _define(
+    "distill_loss(Tensor logits, Tensor teacher_ids, Tensor teacher_logits, Tensor? teacher_lse, Tensor? labels,"
+    " float temperature=1.0, float alpha=1.0) -> Tensor",
+    lambda logits, ids, top, lse, labels, temperature=1.0, alpha=1.0: _distill_ref(None, logits, ids, top, lse, labels, temperature, alpha),
+    lambda logits, ids, top, lse, labels, temperature=1.0, alpha=1.0: logits.new_empty(logits.shape[:-1], dtype=torch.float32),
+    "distill_loss", lambda *args: _check_distill(None, *args),
+)
+distill_loss_grad = _define(
+    "distill_loss_grad(Tensor dloss, Tensor logits, Tensor teacher_ids, Tensor teacher_logits, Tensor? teacher_lse, Tensor? labels,"
+    " float temperature=1.0, float alpha=1.0) -> (Tensor, Tensor)",
+    lambda dloss, logits, ids, top, lse, labels, temperature=1.0, alpha=1.0: _distill_ref(
+        dloss, logits, ids, top, lse, labels, temperature, alpha),
+    lambda dloss, logits, ids, top, lse, labels, temperature=1.0, alpha=1.0: (
+        logits.new_empty(logits.shape[:-1], dtype=torch.float32), logits.new_empty(logits.shape)),
+    "distill_loss_grad", _check_distill,
+)
+
+
+def _distill_setup(ctx, inputs, output):
+    logits, ids, top, lse, labels, ctx.temperature, ctx.alpha = inputs
+    ctx.save_for_backward(logits, ids, top, lse, labels)
+
+
+def _distill_autograd(ctx, dloss):
+    # nothing flows to the teacher
+    dz = distill_loss_grad(dloss.contiguous(), *ctx.saved_tensors, ctx.temperature, ctx.alpha)[1]
+    return dz, None, None, None, None, None, None
+
+
+_autograd("distill_loss", _distill_autograd, _distill_setup)
+
+
+# ======================================================================================
 # Embedding gather / scatter-add
 # ======================================================================================
 embedding = _define(
@@ -798,5 +1144,6 @@ def mse_loss(out: Tensor, target: Tensor) -> Tensor:
 __all__ = [
     "linear", "linear_dgrad", "linear_wgrad", "colsum", "rmsnorm", "rmsnorm_bwd", "layernorm", "layernorm_bwd",
     "gelu", "gelu_bwd", "swiglu", "swiglu_bwd", "rope", "attention", "attention_bwd", "cross_entropy",
-    "cross_entropy_bwd", "embedding", "embedding_bwd", "sum_squares", "adamw", "mse_loss",
+    "cross_entropy_bwd", "embedding", "embedding_bwd", "sum_squares", "adamw", "mse_loss", "linear_ragged", "linear_ragged_dgrad",
+    "linear_ragged_wgrad", "residual_norm", "residual_norm_bwd", "distill_loss", "distill_loss_grad",
 ]

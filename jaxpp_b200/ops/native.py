@@ -383,6 +383,49 @@ def layernorm_bwd(dy, x, w, mean, rstd, sum_dtype=None):
     return dx, dw, db
 
 
+def _gate_groups(gate) -> int:
+    return 1 if gate is None or gate.dim() == 1 else gate.shape[0]
+
+
+def residual_norm(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
+    _here("residual_norm", x, y, w_post, gate, w_pre)
+    x, y, w_post, gate, w_pre = (_vectors(t) for t in (x, y, w_post, gate, w_pre))
+    stat = lambda w: torch.empty((0,) if w is None else x.shape[:-1], dtype=torch.float32, device=x.device)
+    r, rstd_post, rstd_pre = torch.empty_like(x), stat(w_post), stat(w_pre)
+    h = torch.empty_like(x) if w_pre is not None else torch.empty(0, dtype=x.dtype, device=x.device)
+    d = x.shape[-1]
+    lib = load()
+    lib.jpb_residual_norm_fwd.argtypes = [_c_int] + [_c_p] * 9 + [_c_ll, _c_int, _c_int, _c_f, _c_f, _c_p]
+    if x.numel():
+        _check(lib.jpb_residual_norm_fwd(_dt(x), x.data_ptr(), y.data_ptr(), _p(w_post), _p(gate), _p(w_pre), r.data_ptr(), h.data_ptr(),
+                                         rstd_post.data_ptr(), rstd_pre.data_ptr(), x.numel() // d, d, _gate_groups(gate), float(scale),
+                                         float(eps), _stream()), "residual_norm")
+    return r, h, rstd_post, rstd_pre
+
+
+def residual_norm_bwd(dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre, scale=1.0, sum_dtype=None):
+    _here("residual_norm_bwd", dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre)
+    dr, dh, x, y, w_post, gate, w_pre = (_vectors(t) for t in (dr, dh, x, y, w_post, gate, w_pre))
+    rstd_post, rstd_pre = rstd_post.contiguous(), rstd_pre.contiguous()
+    wide, sums = _wide(sum_dtype, x), sum_dtype or x.dtype
+    like = lambda w: torch.empty(0, dtype=x.dtype, device=x.device) if w is None else torch.empty(w.shape, dtype=sums, device=x.device)
+    dx, dy, dw_post, dgate, dw_pre = torch.empty_like(x), torch.empty_like(x), like(w_post), like(gate), like(w_pre)
+    d = x.shape[-1]
+    if d == 0:
+        return dx, dy, dw_post, dgate, dw_pre
+    rows, groups = x.numel() // d, _gate_groups(gate)
+    lib = load()
+    lib.jpb_residual_norm_bwd.argtypes = [_c_int] + [_c_p] * 15 + [_c_ll, _c_int, _c_int, _c_f, _c_int, _c_p]
+    lib.jpb_residual_norm_bwd_scratch_elems.argtypes = [_c_int, _c_ll, _c_int, _c_int]
+    lib.jpb_residual_norm_bwd_scratch_elems.restype = _c_ll
+    scratch = torch.empty(lib.jpb_residual_norm_bwd_scratch_elems(_dt(x), rows, d, groups), dtype=torch.float32, device=x.device)
+    _check(lib.jpb_residual_norm_bwd(_dt(x), _p(dr), _p(dh), x.data_ptr(), y.data_ptr(), _p(w_post), _p(gate), _p(w_pre),
+                                     rstd_post.data_ptr(), rstd_pre.data_ptr(), dx.data_ptr(), dy.data_ptr(), dw_post.data_ptr(),
+                                     dgate.data_ptr(), dw_pre.data_ptr(), scratch.data_ptr(), rows, d, groups, float(scale), wide,
+                                     _stream()), "residual_norm_bwd", 2)
+    return dx, dy, dw_post, dgate, dw_pre
+
+
 def colsum(dy, sum_dtype=None):
     dy = dy.contiguous()
     rows, cols = _rows(dy), dy.shape[-1]
@@ -539,6 +582,55 @@ def cross_entropy_bwd(dloss, logits, labels, lse):
     _check(load().jpb_ce_bwd(_dt(logits), dloss.data_ptr(), logits.data_ptr(), labels.data_ptr(), lse.contiguous().data_ptr(),
                              out.data_ptr(), rows, V, _stream()), "cross_entropy_bwd")
     return out
+
+
+def _here(what: str, *tensors) -> None:
+    """The kernels are launched on the current stream of the current device: every operand has to be there."""
+    current = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != current):
+            raise NativeError(f"{what}: a tensor is on {t.device}, the current device is cuda:{current}")
+
+
+def _vectors(t: Optional[torch.Tensor]):
+    """``t`` contiguous and on a 16-byte boundary (views may start anywhere)."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _distill(dloss, logits, ids, top, lse, labels, temperature, alpha):
+    _here("distill_loss", dloss, logits, ids, top, lse, labels)
+    if top.dtype not in (torch.float32, torch.bfloat16):
+        raise NativeError(f"distill_loss takes teacher logits in float32 or bfloat16, got {top.dtype}")
+    dt = _dt(logits)
+    logits = logits.contiguous() if dloss is None else _vectors(logits)
+    ids, top = ids.contiguous(), top.contiguous()
+    lse, labels = (None if t is None else t.contiguous() for t in (lse, labels))
+    V, K = logits.shape[-1], ids.shape[-1]
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    out = None
+    if dloss is not None:
+        dloss = dloss.float().contiguous()
+        out = torch.empty_like(logits)
+    rows = loss.numel()
+    if rows == 0:
+        return loss, out
+    lib = load()
+    lib.jpb_distill.argtypes = [_c_int] + [_c_p] * 3 + [_c_int, _c_p, _c_int, _c_p, _c_p, _c_f, _c_f, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_p]
+    _check(lib.jpb_distill(dt, _p(dloss), logits.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), top.data_ptr(),
+                           int(top.dtype == torch.float32), _p(lse), _p(labels), float(temperature), float(alpha), loss.data_ptr(),
+                           _p(out), rows, V, K, _stream()), "distill_loss")
+    return loss, out
+
+
+def distill_loss(logits, ids, top, lse, labels, temperature=1.0, alpha=1.0):
+    return _distill(None, logits, ids, top, lse, labels, temperature, alpha)[0]
+
+
+def distill_loss_grad(dloss, logits, ids, top, lse, labels, temperature=1.0, alpha=1.0):
+    return _distill(dloss, logits, ids, top, lse, labels, temperature, alpha)
 
 
 def sum_squares(tensors):

@@ -211,6 +211,9 @@ def _native():
         lib.jpb_moe_dispatch_rows.argtypes = [i, p, p, p, i, i, i, p]
         lib.jpb_moe_combine_rows.argtypes = [i, p, p, p, p, i, i, i, i, p]
         lib.jpb_moe_combine_rows_bwd.argtypes = [i, p, p, p, p, p, p, i, i, i, p]
+        lib.jpb_expert_order.argtypes = [p, p, p, p, p, i, i, p]
+        lib.jpb_expert_order_scratch_elems.argtypes = [i, i]
+        lib.jpb_expert_order_scratch_elems.restype = ctypes.c_longlong
         _bound = True
     return lib, native
 
@@ -368,6 +371,68 @@ def combine(y_buf: Tensor, dest: Tensor, weights: Tensor, top_k: int) -> Tensor:
     flat = torch.cat([y_buf.reshape(E * C, d), torch.zeros(1, d, dtype=y_buf.dtype, device=y_buf.device)], 0)
     picked = flat.index_select(0, dest).view(-1, top_k, d)
     return (picked.float() * weights.unsqueeze(-1)).sum(1).to(y_buf.dtype)
+
+
+# ---- sorting the picks by expert, for layers that drop none ------------------------------------------------------------
+def _expert_order_ref(top_i: Tensor, n_experts: int):
+    flat = top_i.reshape(-1)
+    n = flat.numel()
+    known = (flat >= 0) & (flat < n_experts)
+    inv = torch.sort(torch.where(known, flat, torch.full_like(flat, n_experts)), stable=True).indices
+    counts = torch.bincount(flat[known], minlength=n_experts)
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).to(torch.int32)
+    dest = torch.empty_like(flat).index_copy_(0, inv, torch.arange(n, device=flat.device, dtype=flat.dtype))
+    dest = torch.where(known, dest, torch.full_like(dest, n))
+    filled = torch.arange(n, device=flat.device) < counts.sum()
+    return dest, torch.where(filled, inv, torch.full_like(inv, -1)).to(torch.int32), offsets
+
+
+MAX_ORDER_EXPERTS = 256
+
+
+def _check_expert_order(top_i: Tensor, n_experts: int):
+    if top_i.dtype != torch.int64:
+        raise ValueError(f"expert_order: picks are int64, got {top_i.dtype}")
+    if not 1 <= n_experts <= MAX_ORDER_EXPERTS:
+        raise ValueError(f"expert_order: 1 to {MAX_ORDER_EXPERTS} experts, got {n_experts}")
+    if top_i.numel() >= 2 ** 31:
+        raise ValueError(f"expert_order: fewer than 2^31 picks, got {top_i.numel()}")
+
+
+def _expert_order_impl(top_i: Tensor, n_experts: int):
+    _check_expert_order(top_i, n_experts)
+    if not ops._use_native(top_i):
+        return _expert_order_ref(top_i, n_experts)
+    lib, native = _native()
+    flat = top_i.contiguous()
+    n = flat.numel()
+    dest = torch.empty(n, dtype=torch.int64, device=flat.device)
+    inv = torch.empty(n, dtype=torch.int32, device=flat.device)
+    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=flat.device)
+    scratch = torch.empty(lib.jpb_expert_order_scratch_elems(n, n_experts), dtype=torch.int32, device=flat.device)
+    native._check(lib.jpb_expert_order(flat.data_ptr(), dest.data_ptr(), inv.data_ptr(), offsets.data_ptr(), scratch.data_ptr(), n,
+                                       n_experts, native._stream()), "jpb_expert_order", 2)
+    return dest, inv, offsets
+
+
+def _expert_order_fake(top_i: Tensor, n_experts: int):
+    _check_expert_order(top_i, n_experts)
+    return (torch.empty(top_i.numel(), dtype=torch.int64, device=top_i.device),
+            torch.empty(top_i.numel(), dtype=torch.int32, device=top_i.device),
+            torch.empty(n_experts + 1, dtype=torch.int32, device=top_i.device))
+
+
+_lib.define("expert_order(Tensor top_i, int n_experts) -> (Tensor, Tensor, Tensor)")
+_lib.impl("expert_order", _expert_order_impl, "CompositeExplicitAutograd")
+torch.library.register_fake("b200moe::expert_order", _expert_order_fake)
+
+
+def expert_order(top_i: Tensor, n_experts: int):
+    """The picks ``top_i`` (int64, any shape, token-major) sorted by expert, those of one expert in their own order:
+    ``dest`` [picks] int64 says where each pick goes, ``inv`` [picks] int32 which pick a place holds, and expert ``e`` has
+    places ``offsets[e]`` to ``offsets[e + 1]`` (``offsets`` [n_experts + 1] int32).  No capacity: no pick is dropped.  A pick
+    that names no expert has ``dest`` = picks, and the places left over at the end hold none (``inv`` -1)."""
+    return torch.ops.b200moe.expert_order(top_i, n_experts)
 
 
 # ---- the same three steps as kernels, where the experts are on this device -------------------------------------------
@@ -539,6 +604,7 @@ def _register_direct_calls():
     _core.DIRECT[torch.ops.b200moe.route_tokens.default] = _route_tokens_impl
     _core.DIRECT[torch.ops.b200moe.route_tokens_bwd.default] = _route_tokens_bwd_impl
     _core.DIRECT[torch.ops.b200moe.slots.default] = _slots_impl
+    _core.DIRECT[torch.ops.b200moe.expert_order.default] = _expert_order_impl
     _core.DIRECT[torch.ops.b200moe.dispatch_rows.default] = _dispatch_rows_impl
     _core.DIRECT[torch.ops.b200moe.combine_rows.default] = _combine_rows_impl
     _core.DIRECT[torch.ops.b200moe.combine_rows_bwd.default] = _combine_rows_bwd_impl

@@ -38,9 +38,20 @@ int jpb_make_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, int 
     estr[i] = 1;
   }
   for (int i = 0; i + 1 < rank; ++i) gstrides[i] = strides_bytes[i];
-  CUresult r = g_encode(out, dt, rank, const_cast<void*>(base), gdims, gstrides, gbox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle_128b ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return g_encode(out, dt, rank, const_cast<void*>(base), gdims, gstrides, gbox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    swizzle_128b ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // the first CUDA call of this thread (autograd runs backward passes on threads of its own): the runtime binds the
+    // device's context to a thread when the device is set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaSetDevice(dev);
+    r = encode();
+  }
   return r == CUDA_SUCCESS ? 0 : -(1000 + int(r));
 }
 

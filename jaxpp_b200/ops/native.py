@@ -58,6 +58,13 @@ def load() -> ctypes.CDLL:
     lib.jpb_sum_squares_parts.restype = _c_ll
     lib.jpb_sum_squares_partial.argtypes = [_c_int, _c_int, _c_p, _c_p, _c_p, _c_p]
     lib.jpb_sum_partials.argtypes = [_c_p, _c_int, _c_p, _c_p]
+    lib.jpb_linear_ragged.argtypes = [_c_p] * 4 + [_c_int] * 5 + [_c_p]
+    lib.jpb_linear_ragged_wgrad.argtypes = [_c_p] * 4 + [_c_int] * 6 + [_c_p]
+    lib.jpb_residual_norm_fwd.argtypes = [_c_int] + [_c_p] * 9 + [_c_ll, _c_int, _c_int, _c_f, _c_f, _c_p]
+    lib.jpb_residual_norm_bwd.argtypes = [_c_int] + [_c_p] * 15 + [_c_ll, _c_int, _c_int, _c_f, _c_int, _c_p]
+    lib.jpb_residual_norm_bwd_scratch_elems.argtypes = [_c_int, _c_ll, _c_int, _c_int]
+    lib.jpb_residual_norm_bwd_scratch_elems.restype = _c_ll
+    lib.jpb_distill.argtypes = [_c_int] + [_c_p] * 3 + [_c_int, _c_p, _c_int, _c_p, _c_p, _c_f, _c_f, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_p]
     lib.jpb_read_status.argtypes = [_c_int]
     lib.jpb_build_info.restype = ctypes.c_char_p
     for name in ("jpb_attention_fwd", "jpb_attention_bwd"):
@@ -284,6 +291,47 @@ def linear_wgrad_batched(dy, x, out_dtype=None, counts=None, seg_rows=0, out=Non
     return _gemm_batched(dy, x, out, E, N, K, M, True, True)
 
 
+def _ragged_operands(what, offsets, *ts):
+    _here(what, offsets, *ts)
+    for t in ts:
+        if t.dtype != torch.bfloat16:
+            raise NativeError(f"{what}: the tcgen05 GEMM takes bfloat16 operands, got {t.dtype}")
+        if t.shape[-1] % 8 or t.shape[-2] % 8 and t.dim() == 3:
+            raise NativeError(f"{what}: feature sizes have to be multiples of 8, got {tuple(t.shape)}")
+    return (offsets.contiguous(), *(_vectors(t) for t in ts))
+
+
+def _linear_ragged(what, rows, w, offsets, transposed):
+    offsets, rows, w = _ragged_operands(what, offsets, rows, w)
+    E, N, K = w.shape
+    out = torch.empty(rows.shape[0], K if transposed else N, dtype=torch.bfloat16, device=rows.device)
+    _check(load().jpb_linear_ragged(rows.data_ptr(), w.data_ptr(), offsets.data_ptr(), out.data_ptr(), rows.shape[0], E, N, K,
+                                    int(transposed), _stream()), what)
+    return out
+
+
+def linear_ragged(x, w, offsets):
+    return _linear_ragged("linear_ragged", x, w, offsets, False)
+
+
+def linear_ragged_dgrad(dy, w, offsets):
+    return _linear_ragged("linear_ragged_dgrad", dy, w, offsets, True)
+
+
+def linear_ragged_wgrad(dy, x, offsets, out_dtype=None, out=None, accumulate=False):
+    """``out`` (fp32, contiguous) with ``accumulate``: the products are added onto it."""
+    offsets, dy, x = _ragged_operands("linear_ragged_wgrad", offsets, dy, x)
+    E, N, K = offsets.shape[0] - 1, dy.shape[1], x.shape[1]
+    if out is None:
+        out_dtype = out_dtype or dy.dtype
+        if out_dtype not in (torch.bfloat16, torch.float32):
+            raise NativeError(f"linear_ragged_wgrad writes bfloat16 or float32, not {out_dtype}")
+        out = torch.empty(E, N, K, dtype=out_dtype, device=dy.device)
+    _check(load().jpb_linear_ragged_wgrad(dy.data_ptr(), x.data_ptr(), offsets.data_ptr(), out.data_ptr(), dy.shape[0], E, N, K,
+                                          int(out.dtype == torch.float32), int(accumulate), _stream()), "linear_ragged_wgrad")
+    return out
+
+
 def linear_dgrad(dy, w):
     dy2 = _as_2d_bf16(dy)
     w2 = _as_2d_bf16(w)  # [N_out, K_in]: reduction over N_out, so w is the MN-major B operand
@@ -395,7 +443,6 @@ def residual_norm(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
     h = torch.empty_like(x) if w_pre is not None else torch.empty(0, dtype=x.dtype, device=x.device)
     d = x.shape[-1]
     lib = load()
-    lib.jpb_residual_norm_fwd.argtypes = [_c_int] + [_c_p] * 9 + [_c_ll, _c_int, _c_int, _c_f, _c_f, _c_p]
     if x.numel():
         _check(lib.jpb_residual_norm_fwd(_dt(x), x.data_ptr(), y.data_ptr(), _p(w_post), _p(gate), _p(w_pre), r.data_ptr(), h.data_ptr(),
                                          rstd_post.data_ptr(), rstd_pre.data_ptr(), x.numel() // d, d, _gate_groups(gate), float(scale),
@@ -415,9 +462,6 @@ def residual_norm_bwd(dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre, sc
         return dx, dy, dw_post, dgate, dw_pre
     rows, groups = x.numel() // d, _gate_groups(gate)
     lib = load()
-    lib.jpb_residual_norm_bwd.argtypes = [_c_int] + [_c_p] * 15 + [_c_ll, _c_int, _c_int, _c_f, _c_int, _c_p]
-    lib.jpb_residual_norm_bwd_scratch_elems.argtypes = [_c_int, _c_ll, _c_int, _c_int]
-    lib.jpb_residual_norm_bwd_scratch_elems.restype = _c_ll
     scratch = torch.empty(lib.jpb_residual_norm_bwd_scratch_elems(_dt(x), rows, d, groups), dtype=torch.float32, device=x.device)
     _check(lib.jpb_residual_norm_bwd(_dt(x), _p(dr), _p(dh), x.data_ptr(), y.data_ptr(), _p(w_post), _p(gate), _p(w_pre),
                                      rstd_post.data_ptr(), rstd_pre.data_ptr(), dx.data_ptr(), dy.data_ptr(), dw_post.data_ptr(),
@@ -618,7 +662,6 @@ def _distill(dloss, logits, ids, top, lse, labels, temperature, alpha):
     if rows == 0:
         return loss, out
     lib = load()
-    lib.jpb_distill.argtypes = [_c_int] + [_c_p] * 3 + [_c_int, _c_p, _c_int, _c_p, _c_p, _c_f, _c_f, _c_p, _c_p, _c_ll, _c_int, _c_int, _c_p]
     _check(lib.jpb_distill(dt, _p(dloss), logits.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), top.data_ptr(),
                            int(top.dtype == torch.float32), _p(lse), _p(labels), float(temperature), float(alpha), loss.data_ptr(),
                            _p(out), rows, V, K, _stream()), "distill_loss")

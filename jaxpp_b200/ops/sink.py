@@ -17,7 +17,8 @@ from . import core as ops
 
 def sink_targets() -> tuple:
     """Op overloads whose result may be redirected into an accumulator."""
-    out = [torch.ops.b200.linear_wgrad.default, torch.ops.b200.embedding_bwd.default, torch.ops.b200.linear_wgrad_batched.default]
+    out = [torch.ops.b200.linear_wgrad.default, torch.ops.b200.embedding_bwd.default, torch.ops.b200.linear_wgrad_batched.default,
+           torch.ops.b200.linear_ragged_wgrad.default]
     try:
         from ..parallel import tp  # noqa: F401  (registers the b200tp ops)
 
@@ -64,6 +65,12 @@ def accumulate(op, acc: torch.Tensor, *args, **kwargs) -> torch.Tensor:
                 and acc.dim() == 3 and tuple(acc.shape) == (dy.shape[0], dy.shape[2], x.shape[2])):
             if ops._native().linear_wgrad_batched(dy, x, None, counts, seg_rows, out=acc, accumulate=True) is not None:
                 return acc
+    elif op is torch.ops.b200.linear_ragged_wgrad.default:
+        dy, x, offsets = args[:3]
+        if (ops._use_native(dy) and acc.dtype == torch.float32 and acc.is_contiguous() and acc.data_ptr() % 16 == 0
+                and dy.dtype == x.dtype == torch.bfloat16 and tuple(acc.shape) == (offsets.shape[0] - 1, dy.shape[1], x.shape[1])):
+            ops._check_ragged_wgrad(dy, x, offsets)
+            return ops._native().linear_ragged_wgrad(dy, x, offsets, out=acc, accumulate=True)
     elif op is torch.ops.b200tp.ag_wgrad.default:
         dy, x_shard, axis = args[0], args[1], args[2]
         out_dtype = args[3] if len(args) > 3 else kwargs.get("out_dtype")

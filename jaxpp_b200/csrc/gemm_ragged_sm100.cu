@@ -25,9 +25,8 @@ constexpr int MAX_GROUPS = 1024;
 constexpr int TABLE_BYTES = 2 * (MAX_GROUPS + 1) * 4 + 8;
 constexpr int GROUP_BLOCKS = 2048;             // token rows that are walked together: they stay in L2 while W streams
 
-// The groups' row bounds (clamped to 0 .. rows and to be non-decreasing) and running tile counts in shared memory, by one warp.
-template <typename Tiles>
-__device__ __forceinline__ void make_table(const int* __restrict__ offsets, int groups, int rows, int* off, int* first, Tiles tiles_of) {
+// The groups' row bounds (clamped to 0 .. rows and to be non-decreasing) in shared memory, by one warp.
+__device__ __forceinline__ void make_bounds(const int* __restrict__ offsets, int groups, int rows, int* off) {
   const int lane = threadIdx.x & 31;
   int carry = 0;
   for (int i0 = 0; i0 <= groups; i0 += 32) {
@@ -42,6 +41,12 @@ __device__ __forceinline__ void make_table(const int* __restrict__ offsets, int 
     if (i <= groups) off[i] = v;
     carry = __shfl_sync(0xffffffffu, v, 31);
   }
+}
+// The same, and the running numbers of tiles.
+template <typename Tiles>
+__device__ __forceinline__ void make_table(const int* __restrict__ offsets, int groups, int rows, int* off, int* first, Tiles tiles_of) {
+  const int lane = threadIdx.x & 31;
+  make_bounds(offsets, groups, rows, off);
   __syncwarp();
   int base = 0;
   for (int i0 = 0; i0 < groups; i0 += 32) {
@@ -66,6 +71,7 @@ template <int CG, int BT>
 struct RowsCfg {
   static constexpr int T_ROWS = BT / CG;       // token rows per CTA and stage
   static constexpr int T_BYTES = T_ROWS * BK * 2;
+  static constexpr int BOX = T_ROWS < 64 ? T_ROWS : 64;   // token rows per copy: a short block takes as many as it needs
   static constexpr int STAGE_BYTES = W_BYTES + T_BYTES;
   static constexpr int FIT = (SMEM_MAX - 1024 - BAR_BYTES - TABLE_BYTES) / STAGE_BYTES;
   static constexpr int STAGES = FIT < 12 ? FIT : 12;
@@ -85,14 +91,10 @@ struct RowsParams {
   int* status;
 };
 
-// A group of n rows: blocks of at most BT rows, all but the last of the same size.
-template <int BT, int GRAIN>
+// A group of n rows is cut into blocks of at most BT rows, as even as the grain allows: a stage of the ring carries 128 rows of
+// weights whatever the block's size, so that a short block costs at least half of a whole one.
+template <int BT>
 __device__ __forceinline__ int blocks_of(int n) { return (n + BT - 1) / BT; }
-template <int BT, int GRAIN>
-__device__ __forceinline__ int block_rows(int n) {
-  const int b = (n + BT - 1) / BT, q = (n + b - 1) / b;
-  return (q + GRAIN - 1) / GRAIN * GRAIN;
-}
 
 struct RowsTile {
   int group, m_blk, t0, n;   // rows t0 .. t0 + n of the tokens
@@ -100,12 +102,13 @@ struct RowsTile {
 template <int BT, int GRAIN>
 __device__ __forceinline__ RowsTile rows_tile(const RowsParams& p, const int* off, const int* first, int tile, int& e) {
   while (tile >= first[e + 1]) ++e;
-  const int n = off[e + 1] - off[e], blocks = blocks_of<BT, GRAIN>(n), q = block_rows<BT, GRAIN>(n);
+  const int n = off[e + 1] - off[e], blocks = blocks_of<BT>(n), grains = (n + GRAIN - 1) / GRAIN;
   constexpr int GB = GROUP_BLOCKS / BT;
   const int i = tile - first[e], per = GB * p.tiles_m, g = i / per, in = i - g * per;
   const int gb = min(GB, blocks - g * GB);
   const int m_blk = in / gb, b = g * GB + in - m_blk * gb;
-  return {e, m_blk, off[e] + b * q, min(q, n - b * q)};
+  const int lo = int((long long)grains * b / blocks) * GRAIN, hi = int((long long)grains * (b + 1) / blocks) * GRAIN;
+  return {e, m_blk, off[e] + lo, min(hi, n) - lo};
 }
 
 template <int CG, int BT, bool W_MN>
@@ -149,7 +152,7 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     tmem_relinquish_cg<CG>();
   }
   if (warp == 2)
-    make_table(p.offsets, p.groups, p.rows, off, first, [&](int n) { return n > 0 ? blocks_of<BT, GRAIN>(n) * p.tiles_m : 0; });
+    make_table(p.offsets, p.groups, p.rows, off, first, [&](int n) { return n > 0 ? blocks_of<BT>(n) * p.tiles_m : 0; });
   tc_fence_before();
   __syncthreads();
   if (CG == 2) cluster_sync();
@@ -165,7 +168,8 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
       const RowsTile t = rows_tile<BT, GRAIN>(p, off, first, tile, e);
       const int n_mma = (t.n + GRAIN - 1) / GRAIN * GRAIN;
-      const int m0 = (t.m_blk * CG + rank) * 128, t0 = t.t0 + rank * (n_mma / CG);
+      const int m0 = (t.m_blk * CG + rank) * 128, t_rows = n_mma / CG, t0 = t.t0 + rank * t_rows;
+      const uint32_t bytes = W_BYTES + (t_rows + C::BOX - 1) / C::BOX * (C::BOX * BK * 2);
       for (int kb = 0; kb < k_blocks; ++kb) {
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
@@ -177,7 +181,7 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const int k0 = kb * BK;
         if (elect_one()) {
           // (pair: all copies report to the leader's barrier, which announces both CTAs' bytes; the peer's may land first)
-          if (CG == 1 || rank == 0) mbar_expect_tx(&full[s], STAGE_BYTES * CG);
+          if (CG == 1 || rank == 0) mbar_expect_tx(&full[s], bytes * CG);
           const uint32_t bar = CG == 2 ? mapa_u32(&full[s], 0) : smem_u32(&full[s]);
           if constexpr (CG == 2) {
             if (!W_MN) tma_load_3d_pair(sw, &map_w, bar, k0, m0, t.group);                       // box {64 k, 128 rows}
@@ -186,7 +190,9 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
               tma_load_3d_pair(sw, &map_w, bar, m0, k0, t.group);
               tma_load_3d_pair(sw + 8192, &map_w, bar, m0 + 64, k0, t.group);
             }
-            tma_load_2d_pair(st, &map_t, bar, k0, t0);
+#pragma unroll
+            for (int j = 0; j < C::T_ROWS; j += C::BOX)
+              if (j < t_rows) tma_load_2d_pair(st + j * 128, &map_t, bar, k0, t0 + j);
           } else {
             if (!W_MN) tma_load_3d(sw, &map_w, &full[s], k0, m0, t.group);
             else if (p.w_blocked) tma_load_4d(sw, &map_w, &full[s], 0, k0, m0 >> 6, t.group);
@@ -194,7 +200,9 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
               tma_load_3d(sw, &map_w, &full[s], m0, k0, t.group);
               tma_load_3d(sw + 8192, &map_w, &full[s], m0 + 64, k0, t.group);
             }
-            tma_load_2d(st, &map_t, &full[s], k0, t0);
+#pragma unroll
+            for (int j = 0; j < C::T_ROWS; j += C::BOX)
+              if (j < t_rows) tma_load_2d(st + j * 128, &map_t, &full[s], k0, t0 + j);
           }
         }
         __syncwarp();
@@ -321,10 +329,17 @@ struct WgradCfg {
   static constexpr int X_COLS = BN / CG;       // columns of x per CTA
   static constexpr int X_BYTES = X_COLS * BK * 2;
   static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
-  static constexpr int STAGES = (SMEM_MAX - 1024 - BAR_BYTES - TABLE_BYTES - EPI_BYTES) / STAGE_BYTES;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + BAR_BYTES + TABLE_BYTES + 1024;
+  static constexpr int MAX_STAGES = 6;
   static constexpr int TMEM_COLS = 2 * BN;
-  static_assert(STAGES >= 4 && STAGES <= 8 && TMEM_COLS <= 512, "");
+  static constexpr int smem_bytes(int stages, int groups) {
+    return stages * STAGE_BYTES + EPI_BYTES + BAR_BYTES + ((groups + 1) * 4 + 15) / 16 * 16 + 1024;
+  }
+  static int stages(int groups) {              // 6 for up to 400 groups (pairs)
+    int n = MAX_STAGES;
+    while (smem_bytes(n, groups) > SMEM_MAX) --n;
+    return n;
+  }
+  static_assert(smem_bytes(4, MAX_GROUPS) <= SMEM_MAX && TMEM_COLS <= 512 && (4 * MAX_STAGES + 5) * 8 <= BAR_BYTES, "");
 };
 
 struct WgradParams {
@@ -332,9 +347,21 @@ struct WgradParams {
   int groups, rows;
   int N, K;                  // rows and columns of a group's result
   int dy_blocked, x_blocked; // operand through a 3-D map {64, rows, columns / 64}: one copy per stage
-  int tiles_n, tiles_k;
+  int tiles_n, tiles_k, stages;
   int out_fp32, accumulate;
   int* status;
+};
+
+// A stage of the ring and its phase.  The barriers of blocks that end a group (`tail`) are used only there, so that their
+// phases have a bit for each stage.
+struct RingPos {
+  int s = 0;
+  uint32_t ph = 0, tail_ph = 0;
+  __device__ __forceinline__ uint32_t tail() const { return (tail_ph >> s) & 1u; }
+  __device__ __forceinline__ void next(int stages, bool tail) {
+    if (tail) tail_ph ^= 1u << s;
+    if (++s == stages) { s = 0; ph ^= 1; }
+  }
 };
 
 template <int CG, int BN>
@@ -342,20 +369,20 @@ __global__ void __launch_bounds__(224, 1)
 ragged_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x,
                     const __grid_constant__ CUtensorMap map_d, const __grid_constant__ WgradParams p) {
   using C = WgradCfg<CG, BN>;
-  constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES;
+  constexpr int STAGE_BYTES = C::STAGE_BYTES, MS = C::MAX_STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* epi = smem + STAGES * STAGE_BYTES;
+  uint8_t* epi = smem + p.stages * STAGE_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(epi + EPI_BYTES);
-  uint64_t* full = bars;                    // [STAGES] TMA -> this CTA's masking warp
-  uint64_t* ready = bars + STAGES;          // [STAGES] masking warps (both CTAs') -> MMA, the leader's
-  uint64_t* empty = bars + 2 * STAGES;
-  uint64_t* acc_full = bars + 3 * STAGES;
-  uint64_t* acc_empty = bars + 3 * STAGES + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 4);
+  uint64_t* full = bars;                    // [stages] TMA -> MMA (pair: the leader's counts both CTAs' bytes)
+  uint64_t* empty = bars + MS;              // [stages] MMA -> TMA
+  uint64_t* tail_full = bars + 2 * MS;      // [stages] a block with masked rows: TMA -> this CTA's masking warp
+  uint64_t* tail_ready = bars + 3 * MS;     // [stages] and the masking warps of both CTAs -> MMA (the leader's)
+  uint64_t* acc_full = bars + 4 * MS;
+  uint64_t* acc_empty = bars + 4 * MS + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * MS + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* off = reinterpret_cast<int*>(epi + EPI_BYTES + BAR_BYTES);
-  int* first = off + p.groups + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CG == 2 ? int(cluster_ctarank()) : 0;
@@ -363,10 +390,11 @@ ragged_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_con
   const int per_group = p.tiles_n * p.tiles_k, num_tiles = per_group * p.groups;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&ready[s], CG);
       mbar_init(&empty[s], 1);
+      mbar_init(&tail_full[s], 1);
+      mbar_init(&tail_ready[s], CG);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -382,7 +410,7 @@ ragged_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_con
     tmem_alloc_cg<CG>(tmem_slot, C::TMEM_COLS);
     tmem_relinquish_cg<CG>();
   }
-  if (warp == 2) make_table(p.offsets, p.groups, p.rows, off, first, [](int) { return 0; });
+  if (warp == 2) make_bounds(p.offsets, p.groups, p.rows, off);
   tc_fence_before();
   __syncthreads();
   if (CG == 2) cluster_sync();
@@ -402,74 +430,100 @@ ragged_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_con
 
   if (warp == 0) {
     // ------------------------------- TMA producer --------------------------------------------
-    uint32_t it = 0, armed = 0, armed_phase = 0;
+    RingPos at;
+    uint32_t armed = 0, armed_phase = 0, tail_armed = 0;
     bool ok = true;
     for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
       int e, nb, kb;
       place(tile, e, nb, kb);
       const int n0 = (nb * CG + rank) * 128, c0 = kb * BN + rank * C::X_COLS;
-      for (int r = off[e]; r < off[e + 1]; r += BK) {
-        const int s = it % STAGES;
-        const uint32_t ph = (it / STAGES) & 1;
-        if (!mbar_wait_bounded_warp(&empty[s], ph ^ 1, abort_flag, p.status)) { ok = false; break; }
+      const int end = off[e + 1];
+      for (int r = off[e]; r < end; r += BK) {
+        const int s = at.s;
+        if (!mbar_wait_bounded_warp(&empty[s], at.ph ^ 1, abort_flag, p.status)) { ok = false; break; }
+        const bool tail = (end - r) < BK && (end - r) % UMMA_K != 0;   // rows to be masked
         uint8_t* sa = smem + s * STAGE_BYTES;
         uint8_t* sb = sa + W_BYTES;
         armed |= 1u << s;
-        armed_phase = (armed_phase & ~(1u << s)) | (ph << s);
+        armed_phase = (armed_phase & ~(1u << s)) | ((tail ? at.tail() : at.ph) << s);
+        tail_armed = (tail_armed & ~(1u << s)) | (uint32_t(tail) << s);
         if (elect_one()) {
-          mbar_expect_tx(&full[s], STAGE_BYTES);
-          if (p.dy_blocked) tma_load_3d(sa, &map_dy, &full[s], 0, r, n0 >> 6);
-          else {
-            tma_load_2d(sa, &map_dy, &full[s], n0, r);
-            tma_load_2d(sa + 8192, &map_dy, &full[s], n0 + 64, r);
+          // Blocks without masked rows report to the leader's `full`, which announces both CTAs' bytes.  The others report to
+          // `tail_full` of their own CTA, and `full` takes a plain arrival, to keep its phase.
+          if (tail) {
+            mbar_expect_tx(&tail_full[s], STAGE_BYTES);
+            if (CG == 1 || rank == 0) mbar_arrive(&full[s]);
+          } else if (CG == 1 || rank == 0) {
+            mbar_expect_tx(&full[s], STAGE_BYTES * CG);
           }
-          if (p.x_blocked) tma_load_3d(sb, &map_x, &full[s], 0, r, c0 >> 6);
+          const uint32_t bar = tail ? smem_u32(&tail_full[s]) : CG == 2 ? mapa_u32(&full[s], 0) : smem_u32(&full[s]);
+          auto load2 = [&](uint8_t* dst, const CUtensorMap* map, int x, int y) {
+            if constexpr (CG == 2) tma_load_2d_pair(dst, map, bar, x, y);
+            else tma_load_2d(dst, map, tail ? &tail_full[s] : &full[s], x, y);
+          };
+          auto load3 = [&](uint8_t* dst, const CUtensorMap* map, int y, int z) {
+            if constexpr (CG == 2) tma_load_3d_pair(dst, map, bar, 0, y, z);
+            else tma_load_3d(dst, map, tail ? &tail_full[s] : &full[s], 0, y, z);
+          };
+          if (p.dy_blocked) load3(sa, &map_dy, r, n0 >> 6);
+          else {
+            load2(sa, &map_dy, n0, r);
+            load2(sa + 8192, &map_dy, n0 + 64, r);
+          }
+          if (p.x_blocked) load3(sb, &map_x, r, c0 >> 6);
           else {
 #pragma unroll
-            for (int j = 0; j < C::X_COLS / 64; ++j) tma_load_2d(sb + j * 8192, &map_x, &full[s], c0 + j * 64, r);
+            for (int j = 0; j < C::X_COLS / 64; ++j) load2(sb + j * 8192, &map_x, c0 + j * 64, r);
           }
         }
         __syncwarp();
-        ++it;
+        at.next(p.stages, tail);
       }
     }
     if (!ok) {
+      // wait (bounded) for the copies in flight before the shared memory is released
       const uint64_t begin = globaltimer_ns();
-      for (int s = 0; s < STAGES; ++s) {
-        if (!(armed & (1u << s))) continue;
-        const uint32_t ph = (armed_phase >> s) & 1;
-        while (!mbar_try_wait(&full[s], ph) && globaltimer_ns() - begin < wait_budget_ns()) {
+      if (CG == 2 && rank != 0) {
+        while (globaltimer_ns() - begin < 2000000) {   // most report to the leader's barriers: many times a copy's time
+        }
+      } else {
+        for (int s = 0; s < p.stages; ++s) {
+          if (!(armed & (1u << s))) continue;
+          const uint32_t ph = (armed_phase >> s) & 1;
+          uint64_t* bar = (tail_armed >> s) & 1 ? &tail_full[s] : &full[s];
+          while (!mbar_try_wait(bar, ph) && globaltimer_ns() - begin < wait_budget_ns()) {
+          }
         }
       }
     }
   } else if (warp == 6) {
-    // ------------------------------- masking warp ------------------------------------------------
-    uint32_t it = 0;
+    // ------------------------------- masking warp: one block per tile at most ---------------------
+    RingPos at;
     bool ok = true;
     for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-      const int e = tile / per_group;
-      for (int r = off[e]; r < off[e + 1]; r += BK) {
-        const int s = it % STAGES;
-        const uint32_t ph = (it / STAGES) & 1;
-        if (!mbar_wait_bounded_warp(&full[s], ph, abort_flag, p.status)) { ok = false; break; }
-        const int live = off[e + 1] - r;
-        if (live < BK) {
+      const int e = tile / per_group, end = off[e + 1];
+      for (int r = off[e]; r < end; r += BK) {
+        const int live = end - r;
+        const bool tail = live < BK && live % UMMA_K != 0;
+        if (tail) {
+          const int s = at.s;
+          if (!mbar_wait_bounded_warp(&tail_full[s], at.tail(), abort_flag, p.status)) { ok = false; break; }
           // rows live .. of the last step of 16.  A token is a 128-byte row of each 64-column block; the swizzle moves pieces
           // within the row only
-          const int end = (live + UMMA_K - 1) / UMMA_K * UMMA_K, pieces = (end - live) * 8;
           constexpr int BLOCKS = STAGE_BYTES / 8192;
-          for (int i = lane; i < pieces * BLOCKS; i += 32) {
-            const int b = i / pieces, in = i - b * pieces;
-            *reinterpret_cast<uint4*>(smem + s * STAGE_BYTES + b * 8192 + live * 128 + in * 16) = make_uint4(0, 0, 0, 0);
+          uint8_t* at_row = smem + s * STAGE_BYTES + live * 128 + lane * 16;      // four rows a step
+          for (int dead = UMMA_K - live % UMMA_K - (lane >> 3); dead > 0; dead -= 4, at_row += 512) {
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) *reinterpret_cast<uint4*>(at_row + b * 8192) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            if (CG == 2) mbar_arrive_cluster(mapa_u32(&tail_ready[s], 0));
+            else mbar_arrive(&tail_ready[s]);
           }
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) {
-          if (CG == 2) mbar_arrive_cluster(mapa_u32(&ready[s], 0));
-          else mbar_arrive(&ready[s]);
-        }
-        ++it;
+        at.next(p.stages, tail);
       }
     }
   } else if (warp == 1) {
@@ -479,7 +533,8 @@ ragged_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_con
       constexpr uint32_t STEP = 2048 >> 4;
       const SmemDesc a_desc = make_smem_desc2(smem_u32(smem), 8192, 1024);
       const SmemDesc b_desc = make_smem_desc2(smem_u32(smem) + W_BYTES, 8192, 1024);
-      uint32_t it = 0, tile_i = 0;
+      RingPos at;
+      uint32_t tile_i = 0;
       bool ok = true;
       for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
         const int e = tile / per_group, begin = off[e], end = off[e + 1];
@@ -488,22 +543,30 @@ ragged_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_con
         if (!mbar_wait_bounded_warp(&acc_empty[acc], acc_ph ^ 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
+        bool fresh = true;
         for (int r = begin; r < end; r += BK) {
-          const int s = it % STAGES;
-          const uint32_t ph = (it / STAGES) & 1;
-          if (!mbar_wait_bounded_warp(&ready[s], ph, abort_flag, p.status)) { ok = false; break; }
+          const int s = at.s;
+          const bool tail = (end - r) < BK && (end - r) % UMMA_K != 0;
+          if (!mbar_wait_bounded_warp(&full[s], at.ph, abort_flag, p.status)) { ok = false; break; }
+          if (tail && !mbar_wait_bounded_warp(&tail_ready[s], at.tail(), abort_flag, p.status)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t at = uint32_t(s * STAGE_BYTES) >> 4;
+          const uint32_t word = uint32_t(s * STAGE_BYTES) >> 4;
           if (elect_one()) {
+            if (end - r > BK - UMMA_K) {       // (no test between the products of a whole block: they are issued one by one)
 #pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k)
-              if (r + k * UMMA_K < end)
-                umma_bf16_ss2_cg<CG>(d_tmem, a_desc.lo + at + k * STEP, a_desc.hi, b_desc.lo + at + k * STEP, b_desc.hi, idesc,
-                                     r > begin || k > 0);
+              for (int k = 0; k < BK / UMMA_K; ++k)
+                umma_bf16_ss2_cg<CG>(d_tmem, a_desc.lo + word + k * STEP, a_desc.hi, b_desc.lo + word + k * STEP, b_desc.hi, idesc,
+                                     !(fresh && k == 0));
+            } else {
+              for (int k = 0; r + k * UMMA_K < end; ++k)
+                umma_bf16_ss2_cg<CG>(d_tmem, a_desc.lo + word + k * STEP, a_desc.hi, b_desc.lo + word + k * STEP, b_desc.hi, idesc,
+                                     !(fresh && k == 0));
+            }
             umma_commit_cg<CG>(&empty[s], 3);
           }
+          fresh = false;
           __syncwarp();
-          ++it;
+          at.next(p.stages, tail);
         }
         if (ok && elect_one()) umma_commit_cg<CG>(&acc_full[acc], 3);
         __syncwarp();
@@ -643,7 +706,8 @@ static int launch_rows(const void* w, const void* tokens, RowsParams& p, int w_m
   }
   if (rc) return rc;
   const uint64_t dims[2] = {K, uint64_t(p.rows)}, strides[1] = {K * 2};
-  const uint32_t box[2] = {BK, uint32_t(C::T_ROWS)};
+  // (the token rows of a stage come in copies of 64; 16-row copies for the remainder made 14336 x 4096 dgrad 10 % slower)
+  const uint32_t box[2] = {BK, uint32_t(C::BOX)};
   if ((rc = jpb_make_tensor_map(&mt, tokens, 2, 2, dims, strides, box, 1))) return rc;
   p.tiles_m = (p.M + 128 * CG - 1) / (128 * CG);
   const long long tiles = ((long long)(p.rows + BT - 1) / BT + p.groups) * p.tiles_m;
@@ -678,7 +742,8 @@ static int launch_wgrad(const void* dy, const void* x, void* D, WgradParams& p, 
   p.tiles_k = (p.K + BN - 1) / BN;
   const long long tiles = (long long)p.tiles_n * p.tiles_k * p.groups;
   if (tiles > 0x7fffffffll) return -JPB_ERR_BAD_ARGUMENT;
-  return launch(ragged_wgrad_kernel<CG, BN>, CG, C::SMEM_BYTES, 224, tiles, stream, ma, mb, md, p);
+  p.stages = C::stages(p.groups);
+  return launch(ragged_wgrad_kernel<CG, BN>, CG, C::smem_bytes(p.stages, p.groups), 224, tiles, stream, ma, mb, md, p);
 }
 
 static bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }

@@ -24,15 +24,51 @@ struct ResNormParams {
   void *dx, *dy;
   float* scratch;
   long long rows;
-  int d;
+  int d, stages;
   long long group_rows;   // rows of x for each row of the gate
-  int groups, chunks;     // backward: every group's rows are cut into `chunks` units
+  int groups, chunks;     // backward: every group's rows are cut into `chunks` parts, a CTA each (or a CTA has whole groups)
+  int stream_gate;        // the gate's row comes with every row of x, else it is loaded when it changes
   void* dgate;            // written by the main kernel where chunks == 1
   int wide;
   float scale, eps;
+  int* status;
 };
 
-constexpr int RN_VECS = 2;   // 16-byte pieces of a row per thread
+constexpr int RN_THREADS = 512;     // threads of an SM: as many rows at a time as there are CTAs of them
+constexpr int RN_MAX_STAGES = 4;
+constexpr int RN_HEAD = 512;        // shared memory in front of the ring: barriers, sums of a CTA
+
+// Rows stream through a ring in shared memory, copied whole by the bulk-copy unit (one thread asks for them): what is in
+// flight does not depend on registers or on how many threads wait for a sum.  A stage holds one row of each operand that there
+// is, in the order y, x, dh, dr, gate.
+struct RowRing {
+  uint64_t* full;
+  uint8_t* ring;
+  uint32_t row_bytes, stage_bytes;
+  const void *y, *x, *dh, *dr, *gate;
+  long long group_rows;
+  volatile int* abort_flag;
+  int* status;
+
+  __device__ __forceinline__ uint32_t at_dr() const { return (1 + (x != nullptr) + (dh != nullptr)) * row_bytes; }
+  __device__ __forceinline__ uint32_t at_gate() const { return at_dr() + (dr != nullptr) * row_bytes; }
+  __device__ __forceinline__ void one(uint8_t*& dst, const void* src, long long row, int s) const {
+    if (src == nullptr) return;
+    bulk_load(dst, static_cast<const uint8_t*>(src) + size_t(row) * row_bytes, row_bytes, &full[s]);
+    dst += row_bytes;
+  }
+  __device__ __forceinline__ void issue(int s, long long row) const {   // one thread
+    mbar_expect_tx(&full[s], stage_bytes);
+    uint8_t* dst = ring + size_t(s) * stage_bytes;
+    one(dst, y, row, s);
+    one(dst, x, row, s);
+    one(dst, dh, row, s);
+    one(dst, dr, row, s);
+    if (gate != nullptr) one(dst, gate, row / group_rows, s);
+  }
+  // (a time-out is reported and the kernel goes on, over rows that nothing will use)
+  __device__ __forceinline__ void wait(int s, uint32_t phase) const { mbar_wait_bounded(&full[s], phase, abort_flag, status); }
+};
 
 template <typename T>
 __device__ __forceinline__ void load_vec(const void* base, size_t at, float (&f)[Vec<T>::N]) {
@@ -46,182 +82,405 @@ __device__ __forceinline__ void store_vec(void* base, size_t at, const float (&f
   v.from_float(f);
   v.store(static_cast<T*>(base) + at);
 }
-
 template <typename T>
-__global__ void __launch_bounds__(1024) residual_norm_fwd_kernel(const __grid_constant__ ResNormParams p) {
+__device__ __forceinline__ Vec<T> ones() {
+  Vec<T> v;
+  float f[Vec<T>::N];
+#pragma unroll
+  for (int j = 0; j < Vec<T>::N; ++j) f[j] = 1.f;
+  v.from_float(f);
+  return v;
+}
+
+// Sums over a CTA with one barrier: `slot` alternates between two halves of the scratch.  Shuffles are what a sum costs (an SM
+// does one a cycle, for all its warps): after the barrier a lane picks up one warp's part and as many steps follow as there are
+// warps, not as there are lanes; `span` is the number of warps rounded up to a power of two, the parts behind it are zeros.
+__device__ __forceinline__ float cta_sum(float v, float* scratch, int& slot, int span) {
+  float* s = scratch + slot * 32;
+  slot ^= 1;
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = s[threadIdx.x & (span - 1)];
+  for (int o = 1; o < span; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Four sums at once: lanes trade values so that each ends up with one of the four (6 shuffles instead of 20), and after the
+// barrier the same way (parts as [warp][4]).
+__device__ __forceinline__ void cta_sum4(float (&v)[4], float* scratch, int& slot, int span) {
+  const int lane = threadIdx.x & 31;
+  float* s = scratch + slot * 128;
+  slot ^= 1;
+  const bool b0 = lane & 1, b1 = lane & 2;
+  float a = b0 ? v[2] : v[0], c = b0 ? v[3] : v[1];
+  a += __shfl_xor_sync(0xffffffffu, b0 ? v[0] : v[2], 1);
+  c += __shfl_xor_sync(0xffffffffu, b0 ? v[1] : v[3], 1);
+  float x = b1 ? c : a;
+  x += __shfl_xor_sync(0xffffffffu, b1 ? a : c, 2);
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  // lane & 3 = 0, 1, 2, 3 has the sums of v[0], v[2], v[1], v[3]
+  if (lane < 4) s[(threadIdx.x >> 5) * 4 + lane] = x;
+  __syncthreads();
+  x = 0.f;
+  for (int i = lane; i < span * 4; i += 32) x += s[i];
+  for (int o = 4; o < 32 && o < span * 4; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  v[0] = __shfl_sync(0xffffffffu, x, 0);
+  v[2] = __shfl_sync(0xffffffffu, x, 1);
+  v[1] = __shfl_sync(0xffffffffu, x, 2);
+  v[3] = __shfl_sync(0xffffffffu, x, 3);
+}
+__device__ __forceinline__ int warps_span() {
+  int n = 1;
+  while (n * 32 < int(blockDim.x)) n <<= 1;
+  return n;
+}
+
+template <typename T, int VECS>
+__global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const __grid_constant__ ResNormParams p) {
   constexpr int VN = Vec<T>::N;
-  __shared__ float scratch[64];
-  const int nvec = p.d / VN;
-  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const size_t base = size_t(row) * p.d;
-    const size_t gate_base = p.gate ? size_t(row / p.group_rows) * p.d : 0;
-    float y[RN_VECS][VN], r[RN_VECS][VN];
-    float s[1] = {0.f};
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int abort_flag;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
+  float* scratch = reinterpret_cast<float*>(smem + 128);    // [2][32]
+  const int tid = threadIdx.x, nvec = p.d / VN, span = warps_span();
+  for (int i = tid; i < 64; i += blockDim.x) scratch[i] = 0.f;
+  const long long lo = p.rows * blockIdx.x / gridDim.x, hi = p.rows * (blockIdx.x + 1) / gridDim.x;
+  const uint32_t row_bytes = uint32_t(p.d) * sizeof(T);
+  const RowRing ring = {full, smem + RN_HEAD, row_bytes, row_bytes * (p.stream_gate ? 3 : 2), p.y, p.x, nullptr, nullptr,
+                        p.stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+    for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.issue(s, lo + s);
+  }
+  Vec<T> w_post[VECS], gate[VECS], w_pre[VECS];
 #pragma unroll
-    for (int i = 0; i < RN_VECS; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
+  for (int i = 0; i < VECS; ++i) {
+    const int v = tid + i * blockDim.x;
+    w_post[i] = gate[i] = w_pre[i] = ones<T>();
+    if (v >= nvec) continue;
+    if (p.w_post) w_post[i].load(static_cast<const T*>(p.w_post) + size_t(v) * VN);
+    if (p.w_pre) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
+  }
+  __syncthreads();
+  int slot = 0, s = 0;
+  uint32_t phase = 0;
+  long long gate_end = p.gate && !p.stream_gate ? lo : hi;   // row from which on another row of the gate counts
+  for (long long row = lo; row < hi; ++row) {
+    if (row == gate_end) {
+      const long long g = row / p.group_rows;
+      gate_end = (g + 1) * p.group_rows;
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        const int v = tid + i * blockDim.x;
+        if (v < nvec) gate[i].load(static_cast<const T*>(p.gate) + size_t(g) * p.d + size_t(v) * VN);
+      }
+    }
+    ring.wait(s, phase);
+    const uint8_t* stage = ring.ring + size_t(s) * ring.stage_bytes;
+    const T* sy = reinterpret_cast<const T*>(stage);
+    const T* sx = reinterpret_cast<const T*>(stage + row_bytes);
+    float y[VECS][VN], r[VECS][VN];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = tid + i * blockDim.x;
       if (v >= nvec) continue;
-      load_vec<T>(p.y, base + v * VN, y[i]);
-      load_vec<T>(p.x, base + v * VN, r[i]);
+      load_vec<T>(sy, size_t(v) * VN, y[i]);
+      load_vec<T>(sx, size_t(v) * VN, r[i]);
+      if (p.stream_gate) gate[i].load(reinterpret_cast<const T*>(stage + ring.at_gate()) + size_t(v) * VN);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) s[0] += y[i][j] * y[i][j];
+      for (int j = 0; j < VN; ++j) sum += y[i][j] * y[i][j];
     }
     float rstd1 = 1.f;
     if (p.w_post) {
-      block_sum<1>(s, scratch);
-      rstd1 = rsqrtf(s[0] / p.d + p.eps);
-      if (threadIdx.x == 0) p.rstd_post[row] = rstd1;
+      rstd1 = rsqrtf(cta_sum(sum, scratch, slot, span) / p.d + p.eps);
+      if (tid == 0) p.rstd_post[row] = rstd1;
+    } else {
+      __syncthreads();
     }
-    float q[1] = {0.f};
+    // the row is in registers by now, of every thread: its stage takes the next one
+    if (tid == 0 && row + p.stages < hi) ring.issue(s, row + p.stages);
+    sum = 0.f;
+    const size_t base = size_t(row) * p.d;
 #pragma unroll
-    for (int i = 0; i < RN_VECS; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
+    for (int i = 0; i < VECS; ++i) {
+      const int v = tid + i * blockDim.x;
       if (v >= nvec) continue;
       float w[VN], g[VN];
-#pragma unroll
-      for (int j = 0; j < VN; ++j) w[j] = g[j] = 1.f;
-      if (p.w_post) load_vec<T>(p.w_post, size_t(v) * VN, w);
-      if (p.gate) load_vec<T>(p.gate, gate_base + v * VN, g);
+      w_post[i].to_float(w);
+      gate[i].to_float(g);
 #pragma unroll
       for (int j = 0; j < VN; ++j) {
         r[i][j] = p.scale * r[i][j] + g[j] * (y[i][j] * rstd1 * w[j]);
-        q[0] += r[i][j] * r[i][j];
+        sum += r[i][j] * r[i][j];
       }
-      store_vec<T>(p.r, base + v * VN, r[i]);
+      store_vec<T>(p.r, base + size_t(v) * VN, r[i]);
     }
-    if (!p.w_pre) continue;
-    block_sum<1>(q, scratch);
-    const float rstd2 = rsqrtf(q[0] / p.d + p.eps);
-    if (threadIdx.x == 0) p.rstd_pre[row] = rstd2;
+    if (p.w_pre) {
+      const float rstd2 = rsqrtf(cta_sum(sum, scratch, slot, span) / p.d + p.eps);
+      if (tid == 0) p.rstd_pre[row] = rstd2;
 #pragma unroll
-    for (int i = 0; i < RN_VECS; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v >= nvec) continue;
-      float w[VN];
-      load_vec<T>(p.w_pre, size_t(v) * VN, w);
+      for (int i = 0; i < VECS; ++i) {
+        const int v = tid + i * blockDim.x;
+        if (v >= nvec) continue;
+        float w[VN];
+        w_pre[i].to_float(w);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) w[j] *= r[i][j] * rstd2;
-      store_vec<T>(p.h, base + v * VN, w);
+        for (int j = 0; j < VN; ++j) w[j] *= r[i][j] * rstd2;
+        store_vec<T>(p.h, base + size_t(v) * VN, w);
+      }
+    }
+    if (++s == p.stages) { s = 0; phase ^= 1; }
+  }
+  if (abort_flag) {     // copies may still be in flight: many times their time
+    const uint64_t begin = globaltimer_ns();
+    while (globaltimer_ns() - begin < 2000000) {
     }
   }
 }
 
-// A unit is a run of rows that share a gate row; a CTA takes units in turn.  The sums for the gate leave with each unit (as
-// the result, where a unit is a whole group), those for the weights when the CTA is done.
-template <typename T>
-__global__ void __launch_bounds__(1024) residual_norm_bwd_kernel(const __grid_constant__ ResNormParams p) {
-  constexpr int VN = Vec<T>::N;
-  __shared__ float scratch[64];
-  const int nvec = p.d / VN;
-  float* part_post = p.scratch;
-  float* part_pre = part_post + size_t(gridDim.x) * p.d;
-  float* part_gate = part_pre + size_t(gridDim.x) * p.d;
-  float a_post[RN_VECS][VN], a_pre[RN_VECS][VN], a_gate[RN_VECS][VN];
+// Backward.  With c = gate * w_post * y (so that r = scale * x + rstd1 * c) the two means need one round of sums, and one
+// barrier, over the row:
+//   mean1 = mean(u * hat) = rstd2 * sum(u r) / d
+//   mean2 = mean(v * p)   = rstd1 * (sum(c dr) + rstd2 * (sum(c u) - rstd2 * mean1 * sum(c r))) / d
+// and the sums over the rows of dR * p alone, S, give both dgate = w_post * S and dw_post = gate * S.  A CTA has consecutive
+// rows: a part of one group of rows that share a gate row, or whole groups.  The sums for the gate leave at the end of a group
+// (as the result, where the CTA has all of it), those for the weights when the CTA is done.
+// With packed arithmetic the kernel is bound by HBM again: two rounds of sums and scalar arithmetic took three times as long.
+template <typename T, int VECS>
+__global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const __grid_constant__ ResNormParams p) {
+  constexpr int VN = Vec<T>::N, NP = VN / 2;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int abort_flag;
+  __shared__ __align__(16) float scratch[2 * 32 * 4];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
+  const int tid = threadIdx.x, nvec = p.d / VN, span = warps_span();
+  for (int i = tid; i < 2 * 32 * 4; i += blockDim.x) scratch[i] = 0.f;
+  const bool pre = p.w_pre && p.dh;
+  float* part_post = p.scratch + size_t(blockIdx.x) * p.d;
+  float* part_pre = p.scratch + size_t(gridDim.x + blockIdx.x) * p.d;
+  float* part_gate = p.scratch + size_t(2 * gridDim.x + blockIdx.x) * p.d;
+  long long lo, hi;
+  if (p.chunks > 1) {
+    const long long g = blockIdx.x / p.chunks, c = blockIdx.x - g * p.chunks;
+    lo = g * p.group_rows + p.group_rows * c / p.chunks;
+    hi = g * p.group_rows + p.group_rows * (c + 1) / p.chunks;
+  } else {
+    lo = (long long)p.groups * blockIdx.x / gridDim.x * p.group_rows;
+    hi = (long long)p.groups * (blockIdx.x + 1) / gridDim.x * p.group_rows;
+  }
+  const uint32_t row_bytes = uint32_t(p.d) * sizeof(T);
+  const int operands = 1 + 2 * pre + (p.dr != nullptr) + p.stream_gate;
+  const RowRing ring = {full, smem + RN_HEAD, row_bytes, row_bytes * operands, p.y, pre ? p.x : nullptr, pre ? p.dh : nullptr, p.dr,
+                        p.stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+    for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.issue(s, lo + s);
+  }
+  const F2 zero = f2(0.f);
+  Vec<T> w_pre[VECS];
+  F2 gw[VECS][NP], S[VECS][NP], a_pre[VECS][NP];    // gate * w_post; sums of dR * p (of the group) and dh * hat
+  auto load_gate = [&](const T* gate) {                      // gate: this row's, or null
 #pragma unroll
-  for (int i = 0; i < RN_VECS; ++i)
+    for (int i = 0; i < VECS; ++i) {
+      const int v = tid + i * blockDim.x;
+      if (v >= nvec) continue;
+      Vec<T> w = ones<T>(), g = ones<T>();
+      if (p.w_post) w.load(static_cast<const T*>(p.w_post) + size_t(v) * VN);
+      if (gate) g.load(gate + size_t(v) * VN);
+      F2 f[NP];
+      to_pairs(w, f);
+      to_pairs(g, gw[i]);
 #pragma unroll
-    for (int j = 0; j < VN; ++j) a_post[i][j] = a_pre[i][j] = 0.f;
-  const long long units = (long long)p.groups * p.chunks;
-  for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const long long group = unit / p.chunks, chunk = unit - group * p.chunks;
-    const long long first = group * p.group_rows + p.group_rows * chunk / p.chunks;
-    const long long last = group * p.group_rows + p.group_rows * (chunk + 1) / p.chunks;
+      for (int j = 0; j < NP; ++j) gw[i][j] = gw[i][j] * f[j];
+    }
+  };
 #pragma unroll
-    for (int i = 0; i < RN_VECS; ++i)
+  for (int i = 0; i < VECS; ++i) {
+    const int v = tid + i * blockDim.x;
 #pragma unroll
-      for (int j = 0; j < VN; ++j) a_gate[i][j] = 0.f;
-    for (long long row = first; row < last; ++row) {
-      const size_t base = size_t(row) * p.d;
-      const float rstd1 = p.w_post ? p.rstd_post[row] : 1.f;
-      const bool pre = p.w_pre && p.dh;
-      const float rstd2 = pre ? p.rstd_pre[row] : 0.f;
-      float s[1] = {0.f};
-      float P[RN_VECS][VN], G[RN_VECS][VN], W[RN_VECS][VN], hat[RN_VECS][VN], u[RN_VECS][VN];
+    for (int j = 0; j < NP; ++j) S[i][j] = a_pre[i][j] = gw[i][j] = zero;
+    w_pre[i] = ones<T>();
+    if (v < nvec && p.w_pre) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
+  }
+  if (!p.gate) load_gate(nullptr);
+  long long group = lo < hi ? lo / p.group_rows : 0;
+  bool first_group = true;
+  // end of a group: S goes to dgate (or its partial sum) and, times the gate, to the partial sum of dw_post
+  auto flush = [&](const T* gate) {
 #pragma unroll
-      for (int i = 0; i < RN_VECS; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
+    for (int i = 0; i < VECS; ++i) {
+      const int v = tid + i * blockDim.x;
+      if (v >= nvec) continue;
+      Vec<T> w = ones<T>(), g = ones<T>();
+      if (p.w_post) w.load(static_cast<const T*>(p.w_post) + size_t(v) * VN);
+      if (gate) g.load(gate + size_t(v) * VN);
+      F2 f[NP], o[NP];
+      if (gate) {
+        to_pairs(w, f);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) o[j] = f[j] * S[i][j];
+        if (p.chunks == 1 && !p.wide) {
+          from_pairs(w, o);
+          w.store(static_cast<T*>(p.dgate) + size_t(group) * p.d + size_t(v) * VN);
+        } else {
+          float2* to = reinterpret_cast<float2*>(p.chunks > 1 ? part_gate : static_cast<float*>(p.dgate) + size_t(group) * p.d) + v * NP;
+#pragma unroll
+          for (int j = 0; j < NP; ++j) to[j] = make_float2(o[j].lo(), o[j].hi());
+        }
+      }
+      if (p.w_post) {
+        float2* to = reinterpret_cast<float2*>(part_post) + v * NP;
+        to_pairs(g, f);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          F2 sum = f[j] * S[i][j];
+          if (!first_group) { const float2 old = to[j]; sum = sum + f2(old.x, old.y); }
+          to[j] = make_float2(sum.lo(), sum.hi());
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NP; ++j) S[i][j] = zero;
+    }
+    first_group = false;
+  };
+  __syncthreads();
+  int slot = 0, s = 0;
+  uint32_t phase = 0;
+  long long left = 0;             // rows of the current group that are still to come
+  const float inv_d = 1.f / p.d;
+  const F2 scale = f2(p.scale);
+  float next1 = lo < hi && p.w_post ? p.rstd_post[lo] : 1.f, next2 = lo < hi && pre ? p.rstd_pre[lo] : 0.f;
+  for (long long row = lo; row < hi; ++row) {
+    if (p.gate && left == 0) {
+      left = p.group_rows;        // (a part of a group ends with the CTA's rows)
+      if (!p.stream_gate) load_gate(static_cast<const T*>(p.gate) + size_t(group) * p.d);
+    }
+    const float rstd1 = next1, rstd2 = next2;
+    if (row + 1 < hi) {
+      if (p.w_post) next1 = p.rstd_post[row + 1];
+      if (pre) next2 = p.rstd_pre[row + 1];
+    }
+    ring.wait(s, phase);
+    const uint8_t* stage = ring.ring + size_t(s) * ring.stage_bytes;
+    const T* sy = reinterpret_cast<const T*>(stage);
+    const T* sx = reinterpret_cast<const T*>(stage + row_bytes);          // read where there is a gradient of h
+    const T* sdh = reinterpret_cast<const T*>(stage + 2 * row_bytes);
+    const T* sdr = reinterpret_cast<const T*>(stage + ring.at_dr());
+    const T* sgate = p.stream_gate ? reinterpret_cast<const T*>(stage + ring.at_gate()) : nullptr;
+    if (sgate) load_gate(sgate);
+    const F2 r1 = f2(rstd1);
+    float sums[4];
+    {
+      F2 ur = zero, cd = zero, cu = zero, cr = zero;
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        const int v = tid + i * blockDim.x;
         if (v >= nvec) continue;
+        Vec<T> raw;
+        F2 y[NP], x[NP], u[NP], w[NP], dr[NP];
+        raw.load(sy + size_t(v) * VN);
+        to_pairs(raw, y);
 #pragma unroll
-        for (int j = 0; j < VN; ++j) { G[i][j] = W[i][j] = 1.f; u[i][j] = 0.f; hat[i][j] = 0.f; }
-        load_vec<T>(p.y, base + v * VN, P[i]);
-        if (p.w_post) load_vec<T>(p.w_post, size_t(v) * VN, W[i]);
-        if (p.gate) load_vec<T>(p.gate, size_t(group) * p.d + v * VN, G[i]);
+        for (int j = 0; j < NP; ++j) y[j] = y[j] * gw[i][j];               // c
+        if (p.dr) {
+          raw.load(sdr + size_t(v) * VN);
+          to_pairs(raw, dr);
 #pragma unroll
-        for (int j = 0; j < VN; ++j) P[i][j] *= rstd1;
+          for (int j = 0; j < NP; ++j) cd = fma2(y[j], dr[j], cd);
+        }
         if (pre) {
-          float w[VN];
-          load_vec<T>(p.x, base + v * VN, hat[i]);
-          load_vec<T>(p.dh, base + v * VN, u[i]);
-          load_vec<T>(p.w_pre, size_t(v) * VN, w);
+          raw.load(sx + size_t(v) * VN);
+          to_pairs(raw, x);
+          raw.load(sdh + size_t(v) * VN);
+          to_pairs(raw, u);
+          to_pairs(w_pre[i], w);
 #pragma unroll
-          for (int j = 0; j < VN; ++j) {
-            hat[i][j] = (p.scale * hat[i][j] + G[i][j] * (P[i][j] * W[i][j])) * rstd2;
-            a_pre[i][j] += u[i][j] * hat[i][j];
-            u[i][j] *= w[j];
-            s[0] += u[i][j] * hat[i][j];
+          for (int j = 0; j < NP; ++j) {
+            const F2 uw = u[j] * w[j], r = fma2(r1, y[j], scale * x[j]);
+            ur = fma2(uw, r, ur);
+            cu = fma2(y[j], uw, cu);
+            cr = fma2(y[j], r, cr);
           }
         }
       }
-      if (pre) block_sum<1>(s, scratch);
-      const float mean1 = s[0] / p.d;
-      float q[1] = {0.f};
-#pragma unroll
-      for (int i = 0; i < RN_VECS; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v >= nvec) continue;
-        float dR[VN], o[VN];
-#pragma unroll
-        for (int j = 0; j < VN; ++j) dR[j] = 0.f;
-        if (p.dr) load_vec<T>(p.dr, base + v * VN, dR);
-#pragma unroll
-        for (int j = 0; j < VN; ++j) {
-          dR[j] += rstd2 * (u[i][j] - hat[i][j] * mean1);
-          o[j] = p.scale * dR[j];
-          a_gate[i][j] += dR[j] * (P[i][j] * W[i][j]);
-          const float dn = dR[j] * G[i][j];
-          a_post[i][j] += dn * P[i][j];
-          u[i][j] = dn * W[i][j];            // from here on v
-          q[0] += u[i][j] * P[i][j];
-        }
-        store_vec<T>(p.dx, base + v * VN, o);
-      }
-      float mean2 = 0.f;
-      if (p.w_post) {
-        block_sum<1>(q, scratch);
-        mean2 = q[0] / p.d;
-      }
-#pragma unroll
-      for (int i = 0; i < RN_VECS; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v >= nvec) continue;
-        float o[VN];
-#pragma unroll
-        for (int j = 0; j < VN; ++j) o[j] = rstd1 * (u[i][j] - P[i][j] * mean2);
-        store_vec<T>(p.dy, base + v * VN, o);
-      }
+      sums[0] = ur.lo() + ur.hi(); sums[1] = cd.lo() + cd.hi(); sums[2] = cu.lo() + cu.hi(); sums[3] = cr.lo() + cr.hi();
     }
-    if (p.gate) {
+    cta_sum4(sums, scratch, slot, span);
+    // dR = dr + rstd2 * u - k1 * r,   dy = rstd1 * (gate * w_post * dR) - k2 * y
+    const float k1 = rstd2 * rstd2 * rstd2 * sums[0] * inv_d;
+    const float mean2 = p.w_post ? rstd1 * (sums[1] + (rstd2 * sums[2] - k1 * sums[3])) * inv_d : 0.f;
+    const F2 r2 = f2(rstd2), m1 = f2(-k1), m2 = f2(-mean2 * rstd1 * rstd1);
+    const size_t base = size_t(row) * p.d;
 #pragma unroll
-      for (int i = 0; i < RN_VECS; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v >= nvec) continue;
-        if (p.chunks == 1 && !p.wide) store_vec<T>(p.dgate, size_t(group) * p.d + v * VN, a_gate[i]);
-        else {
-          float* to = (p.chunks == 1 ? static_cast<float*>(p.dgate) + size_t(group) * p.d : part_gate + size_t(unit) * p.d) + v * VN;
+    for (int i = 0; i < VECS; ++i) {
+      const int v = tid + i * blockDim.x;
+      if (v >= nvec) continue;
+      Vec<T> raw;
+      F2 y[NP], dR[NP], o[NP];
+      raw.load(sy + size_t(v) * VN);
+      to_pairs(raw, y);
+      if (p.dr) {
+        raw.load(sdr + size_t(v) * VN);
+        to_pairs(raw, dR);
+      } else {
 #pragma unroll
-          for (int j = 0; j < VN; ++j) to[j] = a_gate[i][j];
+        for (int j = 0; j < NP; ++j) dR[j] = zero;
+      }
+      if (pre) {
+        F2 x[NP], u[NP], w[NP];
+        raw.load(sx + size_t(v) * VN);
+        to_pairs(raw, x);
+        raw.load(sdh + size_t(v) * VN);
+        to_pairs(raw, u);
+        to_pairs(w_pre[i], w);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          const F2 r = fma2(r1, y[j] * gw[i][j], scale * x[j]);
+          a_pre[i][j] = fma2(u[j], r * r2, a_pre[i][j]);
+          dR[j] = fma2(m1, r, fma2(r2, u[j] * w[j], dR[j]));
         }
       }
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        o[j] = scale * dR[j];
+        const F2 pj = y[j] * r1;
+        S[i][j] = fma2(dR[j], pj, S[i][j]);
+        dR[j] = fma2(m2, y[j], r1 * (dR[j] * gw[i][j]));
+      }
+      from_pairs(raw, o);
+      raw.store(static_cast<T*>(p.dx) + base + size_t(v) * VN);
+      from_pairs(raw, dR);
+      raw.store(static_cast<T*>(p.dy) + base + size_t(v) * VN);
     }
+    if (p.gate && (--left == 0 || row + 1 == hi)) {
+      flush(sgate ? sgate : static_cast<const T*>(p.gate) + size_t(group) * p.d);
+      ++group;
+    }
+    __syncthreads();              // every thread has read this stage
+    if (tid == 0 && row + p.stages < hi) ring.issue(s, row + p.stages);
+    if (++s == p.stages) { s = 0; phase ^= 1; }
   }
+  if (!p.gate) flush(nullptr);
 #pragma unroll
-  for (int i = 0; i < RN_VECS; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
+  for (int i = 0; i < VECS; ++i) {
+    const int v = tid + i * blockDim.x;
     if (v >= nvec) continue;
+    float2* to = reinterpret_cast<float2*>(part_pre) + v * NP;
 #pragma unroll
-    for (int j = 0; j < VN; ++j) {
-      if (p.w_post) part_post[size_t(blockIdx.x) * p.d + v * VN + j] = a_post[i][j];
-      if (p.w_pre) part_pre[size_t(blockIdx.x) * p.d + v * VN + j] = a_pre[i][j];
+    for (int j = 0; j < NP; ++j)
+      if (p.w_pre) to[j] = make_float2(a_pre[i][j].lo(), a_pre[i][j].hi());
+  }
+  if (p.gate && lo >= hi && p.w_post)     // a CTA without rows (none at all, or a gate of more groups than rows)
+    for (int c = tid; c < p.d; c += blockDim.x) part_post[c] = 0.f;
+  if (abort_flag) {
+    const uint64_t begin = globaltimer_ns();
+    while (globaltimer_ns() - begin < 2000000) {
     }
   }
 }
@@ -261,32 +520,52 @@ __global__ void __launch_bounds__(256) residual_norm_sums_kernel(const float* sc
 }
 
 static int rn_sms() {
-  static int n = 0;
-  if (!n) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  }
+  int dev = 0, n = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
   return n;
 }
-static int rn_threads(int d, int vn) {
-  const int t = (d / vn + RN_VECS - 1) / RN_VECS;
-  return t <= 32 ? 32 : (t + 31) / 32 * 32;
+// Threads of a CTA, 16-byte pieces of a row per thread, CTAs per SM, stages of the ring and bytes of shared memory.
+struct RnShape {
+  int threads, vecs, per_sm, stages, smem;
+};
+static RnShape rn_shape(int d, int elem, int operands) {
+  RnShape s;
+  const int nvec = d * elem / 16;
+  s.vecs = nvec > 1024 ? 4 : 2;
+  s.threads = ((nvec + s.vecs - 1) / s.vecs + 31) / 32 * 32;
+  s.per_sm = RN_THREADS / s.threads < 8 ? RN_THREADS / s.threads : 8;
+  const int stage = operands * d * elem;
+  s.stages = (226 * 1024 / s.per_sm - 2560 - RN_HEAD) / stage;   // (2560: static and reserved shared memory of a CTA)
+  if (s.stages > RN_MAX_STAGES) s.stages = RN_MAX_STAGES;
+  if (s.stages < 1) s.stages = 1;
+  s.smem = RN_HEAD + s.stages * stage;
+  return s;
 }
 struct RnPlan {
   int grid, chunks;
 };
-// CTAs of the backward, and the units that a group's rows are cut into: about as many units as CTAs.
-static RnPlan rn_bwd_plan(long long rows, int d, int groups, int vn) {
-  const int threads = rn_threads(d, vn);
-  const int per_sm = threads >= 512 ? 1 : 512 / threads < 8 ? 512 / threads : 8;
-  const long long want = (long long)rn_sms() * per_sm;
-  const long long group_rows = groups ? rows / groups : 0;
-  long long chunks = groups ? want / groups : 1;
+// CTAs of the backward, and the parts that a group's rows are cut into: one CTA each, or whole groups to a CTA.
+static RnPlan rn_bwd_plan(long long rows, int groups, int per_sm) {
+  const long long want = (long long)rn_sms() * per_sm, group_rows = rows / groups;
+  long long chunks = want / groups;
   if (chunks > group_rows) chunks = group_rows;
   if (chunks < 1) chunks = 1;
   const long long units = groups * chunks;
   return {int(units < want ? units : want), int(chunks)};
+}
+// A gate whose rows change after a few rows of x comes with them through the ring; one that changes seldom is loaded then.
+static int rn_stream_gate(const void* gate, long long rows, int groups) { return gate && groups > 1 && rows / groups < 16; }
+// (as many operands as the backward can have: the plan must not depend on which are absent, since the scratch goes by it)
+static int rn_bwd_operands(long long rows, int groups) { return 4 + (groups > 1 && rows / groups < 16); }
+template <typename Kernel>
+static int rn_launch(Kernel kernel, int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t stream) {
+  if (shape.smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shape.smem);
+    if (e != cudaSuccess) return int(e);
+  }
+  kernel<<<grid, shape.threads, shape.smem, stream>>>(p);
+  return int(cudaGetLastError());
 }
 template <typename F>
 static int rn_dtype(int dt, F&& f) {
@@ -313,22 +592,27 @@ JPB_API int jpb_residual_norm_fwd(int dt, const void* x, const void* y, const vo
   return rn_dtype(dt, [&](auto tag) {
     using T = decltype(tag);
     constexpr int VN = Vec<T>::N;
-    if (d <= 0 || d % VN || d / VN > RN_VECS * 1024 || groups < 1 || rows % groups || !rn_aligned({x, y, w_post, gate, w_pre, r, h}))
+    if (d <= 0 || d % VN || d / VN > 2 * 1024 || groups < 1 || rows % groups || !rn_aligned({x, y, w_post, gate, w_pre, r, h}))
       return -int(JPB_ERR_BAD_ARGUMENT);
     ResNormParams p = {};
     p.x = x; p.y = y; p.w_post = w_post; p.gate = gate; p.w_pre = w_pre; p.r = r; p.h = h;
     p.rstd_post = rstd_post; p.rstd_pre = rstd_pre; p.rows = rows; p.d = d; p.group_rows = rows / groups;
-    p.scale = scale; p.eps = eps;
-    const int threads = rn_threads(d, VN);
-    const long long most = (long long)rn_sms() * (2048 / threads < 16 ? 2048 / threads : 16);
-    residual_norm_fwd_kernel<T><<<int(rows < most ? rows : most), threads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    return int(cudaGetLastError());
+    p.scale = scale; p.eps = eps; p.status = jpb_status_device_ptr();
+    p.stream_gate = rn_stream_gate(gate, rows, groups);
+    const RnShape shape = rn_shape(d, sizeof(T), 2 + p.stream_gate);
+    p.stages = shape.stages;
+    const long long most = (long long)rn_sms() * shape.per_sm;
+    const int grid = int(rows < most ? rows : most);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return shape.vecs == 2 ? rn_launch(residual_norm_fwd_kernel<T, 2>, grid, shape, p, s)
+                           : rn_launch(residual_norm_fwd_kernel<T, 4>, grid, shape, p, s);
   });
 }
 
 // fp32 elements of scratch for jpb_residual_norm_bwd.
 JPB_API long long jpb_residual_norm_bwd_scratch_elems(int dt, long long rows, int d, int groups) {
-  const jpb::RnPlan plan = jpb::rn_bwd_plan(rows, d, groups, dt == 0 ? 4 : 8);
+  const jpb::RnShape shape = jpb::rn_shape(d, dt == 0 ? 4 : 2, jpb::rn_bwd_operands(rows, groups));
+  const jpb::RnPlan plan = jpb::rn_bwd_plan(rows, groups, shape.per_sm);
   return (2ll * plan.grid + (plan.chunks > 1 ? (long long)groups * plan.chunks : 0)) * d;
 }
 
@@ -341,17 +625,22 @@ JPB_API int jpb_residual_norm_bwd(int dt, const void* dr, const void* dh, const 
   return rn_dtype(dt, [&](auto tag) {
     using T = decltype(tag);
     constexpr int VN = Vec<T>::N;
-    if (rows < 0 || d <= 0 || d % VN || d / VN > RN_VECS * 1024 || groups < 1 || rows % groups ||
+    if (rows < 0 || d <= 0 || d % VN || d / VN > 2 * 1024 || groups < 1 || rows % groups ||
         !rn_aligned({dr, dh, x, y, w_post, gate, w_pre, dx, dy, dgate}))
       return -int(JPB_ERR_BAD_ARGUMENT);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const RnPlan plan = rn_bwd_plan(rows, d, groups, VN);
+    const RnShape shape = rn_shape(d, sizeof(T), rn_bwd_operands(rows, groups));
+    const RnPlan plan = rn_bwd_plan(rows, groups, shape.per_sm);
     ResNormParams p = {};
     p.x = x; p.y = y; p.w_post = w_post; p.gate = gate; p.w_pre = w_pre;
     p.rstd_post = const_cast<float*>(rstd_post); p.rstd_pre = const_cast<float*>(rstd_pre);
     p.dr = dr; p.dh = dh; p.dx = dx; p.dy = dy; p.scratch = scratch; p.rows = rows; p.d = d; p.group_rows = rows / groups;
     p.groups = groups; p.chunks = plan.chunks; p.dgate = dgate; p.wide = wide; p.scale = scale;
-    residual_norm_bwd_kernel<T><<<plan.grid, rn_threads(d, VN), 0, s>>>(p);
+    p.stages = shape.stages; p.stream_gate = rn_stream_gate(gate, rows, groups); p.status = jpb_status_device_ptr();
+    if (rows == 0 && gate) cudaMemsetAsync(dgate, 0, size_t(groups) * d * (wide ? 4 : sizeof(T)), s);
+    const int rc = shape.vecs == 2 ? rn_launch(residual_norm_bwd_kernel<T, 2>, plan.grid, shape, p, s)
+                                   : rn_launch(residual_norm_bwd_kernel<T, 4>, plan.grid, shape, p, s);
+    if (rc) return rc;
     const bool gate_sums = gate && plan.chunks > 1;
     if (w_post || w_pre || gate_sums)
       residual_norm_sums_kernel<T><<<dim3((d + 31) / 32, gate_sums ? 2 + groups : 2), 256, 0, s>>>(

@@ -34,6 +34,49 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Pairs of fp32 values: one instruction for both (half the issue slots of a kernel that is bound by them).
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ float lo() const { return __uint_as_float(uint32_t(v)); }
+  __device__ __forceinline__ float hi() const { return __uint_as_float(uint32_t(v >> 32)); }
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float x) { return f2(x, x); }
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// 16 bytes of T as pairs, and back.
+__device__ __forceinline__ void to_pairs(const Vec<float>& v, F2 (&f)[2]) {
+  f[0] = f2(v.raw.x, v.raw.y);
+  f[1] = f2(v.raw.z, v.raw.w);
+}
+__device__ __forceinline__ void to_pairs(const Vec<__nv_bfloat16>& v, F2 (&f)[4]) {
+  const uint32_t w[4] = {v.raw.x, v.raw.y, v.raw.z, v.raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = f2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void from_pairs(Vec<float>& v, const F2 (&f)[2]) { v.raw = make_float4(f[0].lo(), f[0].hi(), f[1].lo(), f[1].hi()); }
+__device__ __forceinline__ void from_pairs(Vec<__nv_bfloat16>& v, const F2 (&f)[4]) {
+  v.raw = make_uint4(pack_bf16(f[0].lo(), f[0].hi()), pack_bf16(f[1].lo(), f[1].hi()), pack_bf16(f[2].lo(), f[2].hi()),
+                     pack_bf16(f[3].lo(), f[3].hi()));
+}
+
 // Sum (and optionally a second sum) over a CTA; result broadcast to all threads.
 template <int NV>
 __device__ __forceinline__ void block_sum(float (&v)[NV], float* scratch /* >= NV*32 floats */) {

@@ -6,8 +6,18 @@
 //   d soft / d z_v = ((Q + q_o) p_v - (sum of q_j with i_j = v)) / t      for v in S
 //                    ((Q + q_o) - q_o / p_o) p_v / t                      for the others
 // p_o is summed over the entries outside of S, never as a difference: a student that agrees with the teacher leaves almost
-// nothing there.  A bit per vocabulary entry in shared memory says what S holds; it also tells repeated ids.
+// nothing there.
+//
+// A row is copied into shared memory once (bulk copy), by one CTA or, where it is long or there are few rows, a cluster whose
+// CTAs have a part each and trade eight sums.  The elements of S are taken out of it first (-inf in their place), so that the
+// passes over the row, its maximum, the sums and the gradient, have no special cases; S is added by itself and its gradients
+// are written last.
+// What bounds it: HBM (a row read, and one written), then the exponentials, of which an SM does 16 a cycle: one per element for
+// the sums and one for the gradient.  With both temperatures in play the plain exponential is a power of the softened one where
+// t is 2 or 4, else it is taken too.
 #include "vec.cuh"
+
+#include <type_traits>
 
 namespace jpb {
 
@@ -23,9 +33,11 @@ struct DistillParams {
   int V, K;
   int ids64, top_fp32;
   float temperature, alpha;
+  int cluster;                 // CTAs of a row
+  int buffer;                  // bytes of a CTA's part of a row
+  int* status;
 };
 
-constexpr int DISTILL_THREADS = 512;
 constexpr int DISTILL_MAX_K = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -34,163 +46,315 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// The logarithms of a row's sums are taken once a row, in 64 bits: the fast fp32 logarithm is off by 4e-7 near 1, as much as
-// a small loss may be.
-__device__ __forceinline__ float log_exact(float x) { return float(log(double(x))); }
-
-__device__ __forceinline__ float block_max(float v, float* scratch) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
-  v = warp_max(v);
-  __syncthreads();
-  if (lane == 0) scratch[warp] = v;
-  __syncthreads();
-  return warp_max(lane < nwarps ? scratch[lane] : -INFINITY);
+// log(x) for x > 0 to half a unit in the last place or so: x = 2^e m with m in [0.75, 1.5), log m = 2 atanh(s) with s = (m - 1) /
+// (m + 1), |s| <= 0.2, by its series up to s^13 / 13.  (The approximate logarithm is off by 4e-7 near 1, as much as a small loss
+// may be; the 64-bit one takes a microsecond, a tenth of a row's time.)
+__device__ __forceinline__ float log_exact(float x) {
+  if (!(x > 0.f) || x == INFINITY) return x == 0.f ? -INFINITY : x;
+  int e = 0;
+  if (x < 1.2e-38f) { x *= 16777216.f; e = -24; }
+  const int bits = __float_as_int(x), shift = (bits - 0x3f400000) >> 23;      // 0x3f400000 = 0.75
+  const float m = __int_as_float(bits - (shift << 23));
+  e += shift;
+  const float s = __fdiv_rn(m - 1.f, m + 1.f), q = s * s;
+  float r = 1.f / 13.f;
+  r = fmaf(r, q, 1.f / 11.f);
+  r = fmaf(r, q, 1.f / 9.f);
+  r = fmaf(r, q, 1.f / 7.f);
+  r = fmaf(r, q, 1.f / 5.f);
+  r = fmaf(r, q, 1.f / 3.f);
+  r = fmaf(2.f * s * q, r, 2.f * s);
+  return fmaf(float(e), 0.693359375f, fmaf(float(e), -2.12194440e-4f, r));    // log 2 in two parts, the first of 10 bits
 }
 
-// exp(z - m) summed with m running: (m, s_t, s_1) of the scaled and the plain exponentials
-struct Online {
-  float m = -INFINITY, st = 0.f, s1 = 0.f;
-  __device__ __forceinline__ void raise(float to, float it2) {   // to >= m
-    if (to > m) {
-      if (m != -INFINITY) {
-        st *= exp2_fast((m - to) * it2);
-        s1 *= exp2_fast((m - to) * LOG2E);
-      }
-      m = to;
+// Sums and maxima over a CTA of WARPS warps (4 or 8), one barrier each; two halves of the scratch take turns.
+template <int WARPS>
+struct CtaReduce {
+  float* scratch;   // [2][WARPS][8]
+  int slot;
+  template <bool MAX>
+  __device__ __forceinline__ float one(float v) {
+    float* s = scratch + slot * WARPS * 8;
+    slot ^= 1;
+    v = MAX ? warp_max(v) : warp_sum(v);
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = s[threadIdx.x & (WARPS - 1)];
+#pragma unroll
+    for (int o = 1; o < WARPS; o <<= 1) {
+      const float u = __shfl_xor_sync(0xffffffffu, v, o);
+      v = MAX ? fmaxf(v, u) : v + u;
     }
+    return v;
   }
-  __device__ __forceinline__ void add(float f, float it2) {      // after raise(f) or more
-    if (f == -INFINITY) return;
-    st += exp2_fast((f - m) * it2);
-    s1 += exp2_fast((f - m) * LOG2E);
+  // Eight sums: lanes trade values until each has one of the eight, 9 shuffles instead of 40, and 10 after the barrier.
+  __device__ __forceinline__ void eight(float (&v)[8]) {
+    const int lane = threadIdx.x & 31;
+    float* s = scratch + slot * WARPS * 8;
+    slot ^= 1;
+    float a[4], b[2];
+    const bool h = lane & 16, q = lane & 8, e = lane & 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = (h ? v[i + 4] : v[i]) + __shfl_xor_sync(0xffffffffu, h ? v[i] : v[i + 4], 16);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) b[i] = (q ? a[i + 2] : a[i]) + __shfl_xor_sync(0xffffffffu, q ? a[i] : a[i + 2], 8);
+    float x = (e ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, e ? b[0] : b[1], 4);
+    x += __shfl_xor_sync(0xffffffffu, x, 2);
+    x += __shfl_xor_sync(0xffffffffu, x, 1);
+    if ((lane & 3) == 0) s[(threadIdx.x >> 5) * 8 + (lane >> 2)] = x;     // value number: bits 4, 3, 2 of the lane
+    __syncthreads();
+    x = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS / 4; ++k) x += s[k * 32 + lane];            // value lane & 7, every fourth warp
+    x += __shfl_xor_sync(0xffffffffu, x, 8);
+    x += __shfl_xor_sync(0xffffffffu, x, 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __shfl_sync(0xffffffffu, x, i);
   }
 };
 
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(DISTILL_THREADS) distill_kernel(const __grid_constant__ DistillParams p) {
-  constexpr int VN = Vec<T>::N;
-  extern __shared__ uint32_t dyn[];
-  __shared__ float scratch[4 * 32];
-  __shared__ int repeated;
-  int* s_id = reinterpret_cast<int*>(dyn);                 // [K]
-  float* s_q = reinterpret_cast<float*>(dyn + p.K);        // [K]
-  uint32_t* bits = dyn + 2 * p.K;                          // a bit per entry, counted from the first aligned one
-  const int words = (p.V + 31) / 32 + 1;
+__device__ __forceinline__ float piece_max(const Vec<float>& v) { return fmaxf(fmaxf(v.raw.x, v.raw.y), fmaxf(v.raw.z, v.raw.w)); }
+__device__ __forceinline__ float piece_max(const Vec<__nv_bfloat16>& v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v.raw);
+  const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  return fmaxf(f.x, f.y);
+}
+
+// What a CTA tells the others about its part of a row; sums are relative to its maximum m (0 where it has nothing but -inf).
+struct PartSums {
+  float m, out_t, out_1, in_t, in_1, cross, mass, label;
+};
+
+// MODE: exponentials of a gradient and a loss in which 0 only one temperature counts, 1 / 2 both and t = 2 / 4, 3 both, any t
+template <int MODE>
+__device__ __forceinline__ float plain_exp(float e, float f, float m1) {   // exp(f - m) from e = exp((f - m) / t)
+  if (MODE == 0) return e;
+  if (MODE == 1) return e * e;
+  if (MODE == 2) { const float s = e * e; return s * s; }
+  return exp2_fast(fmaf(f, LOG2E, -m1));
+}
+
+template <typename T, bool GRAD, int MODE, int THREADS>
+__global__ void __launch_bounds__(THREADS) distill_kernel(const __grid_constant__ DistillParams p) {
+  constexpr int VN = Vec<T>::N, ES = sizeof(T);
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float scratch[2 * THREADS / 32 * 8];
+  __shared__ __align__(16) PartSums parts[2];
+  __shared__ uint64_t full;
+  __shared__ int abort_flag, repeated;
+  uint8_t* buf = smem;                                             // this CTA's part of the row
+  int* s_id = reinterpret_cast<int*>(smem + p.buffer);             // [K] ids of this part as element numbers of it, or -1
+  float* s_q = reinterpret_cast<float*>(s_id + p.K);               // [K] log q, then q
+  float* s_z = s_q + p.K;                                          // [K] the row's logits there
   const int tid = threadIdx.x, V = p.V, K = p.K;
+  const int C = p.cluster, rank = C > 1 ? int(cluster_ctarank()) : 0;
+  const long long row0 = blockIdx.x / C, row_step = gridDim.x / C;
   const float it = 1.f / p.temperature, it2 = it * LOG2E;
-  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  CtaReduce<THREADS / 32> reduce{scratch, 0};
+  const T ninf = from_f<T>(-INFINITY);
+
+  // This CTA's part of row r: 16-byte pieces lo .. hi of the whole tensor, and the byte of the row's first element from lo on.
+  struct Part {
+    long long lo;
+    int pieces, lead;
+  };
+  auto part_of = [&](long long r) {
+    const long long begin = r * V * ES, g0 = begin >> 4, g1 = (begin + (long long)V * ES + 15) >> 4, n = g1 - g0;
+    Part q;
+    q.lo = g0 + n * rank / C;
+    q.pieces = int(g0 + n * (rank + 1) / C - q.lo);
+    q.lead = int(begin - q.lo * 16);
+    return q;
+  };
+  // pieces that are wholly in the row: copied at once; the one or two others hold elements of the next rows
+  auto first_whole = [&](const Part& q) { return q.lead > 0 ? 1 : 0; };
+  auto last_whole = [&](const Part& q) { return min(q.pieces, (q.lead + V * ES) >> 4); };
+  auto fetch = [&](const Part& q) {     // one thread
+    const int a = first_whole(q), b = last_whole(q);
+    if (b > a) {
+      mbar_expect_tx(&full, uint32_t(b - a) * 16);
+      bulk_load(buf + a * 16, static_cast<const uint8_t*>(p.logits) + (q.lo + a) * 16, uint32_t(b - a) * 16, &full);
+    } else {
+      mbar_arrive(&full);
+    }
+  };
+  struct Entry {
+    long long id;
+    float top;
+  };
+  auto entry = [&](long long r, int j) {
+    const size_t at = size_t(r) * K + j;
+    Entry e;
+    e.id = p.ids64 ? static_cast<const long long*>(p.ids)[at] : (long long)static_cast<const int*>(p.ids)[at];
+    e.top = it * (p.top_fp32 ? static_cast<const float*>(p.top)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.top)[at]));
+    return e;
+  };
+  if (tid == 0) {
+    abort_flag = 0;
+    mbar_init(&full, 1);
+    fence_barrier_init();
+    if (row0 < p.rows) fetch(part_of(row0));
+  }
+  Entry next = {-1, 0.f};         // the first entries of a row are asked for a row ahead
+  if (tid < K && row0 < p.rows) next = entry(row0, tid);
+  __syncthreads();
+  uint32_t phase = 0;
+  for (long long row = row0; row < p.rows; row += row_step) {
+    const Part q = part_of(row);
+    T* elem = reinterpret_cast<T*>(buf);
+    const int lead = q.lead / ES;                    // element of the buffer that the row's first one would be (or is)
+    const int n = q.pieces * VN;
+    const int v_lo = max(lead, 0), v_hi = min(n, lead + V);        // buffer elements of the row
     const T* z = static_cast<const T*>(p.logits) + size_t(row) * V;
-    // vectors start at the first element on a 16-byte boundary
-    const int head = min(V, int((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / int(sizeof(T)));
-    const int nvec = (V - head) / VN, tail = head + nvec * VN;
-    auto bit_at = [&](int v) { return v - head + 32; };    // the head's bits come first, from 32 - head on
-    // ---- the teacher's entries ----
-    __syncthreads();
-    if (tid == 0) repeated = 0;
-    for (int w = tid; w < words; w += DISTILL_THREADS) bits[w] = 0;
+    // ---- the teacher's entries, and the row's logits there (from memory: the row is on its way) ----
+    const long long label = p.labels ? p.labels[row] : -1;
+    const float lse = p.lse ? p.lse[row] : 0.f;
+    const bool label_here = label >= 0 && label < V && label + lead >= v_lo && label + lead < v_hi;
+    const int label_at = label_here ? int(label + lead) : -1;
+    float z_label = label_here ? to_f(z[label]) : 0.f;
     float tmax = -INFINITY;
-    for (int j = tid; j < K; j += DISTILL_THREADS) {
-      const size_t at = size_t(row) * K + j;
-      const long long id = p.ids64 ? static_cast<const long long*>(p.ids)[at] : (long long)static_cast<const int*>(p.ids)[at];
-      const float top = p.top_fp32 ? static_cast<const float*>(p.top)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.top)[at]);
-      const bool valid = id >= 0 && id < V && top != -INFINITY;
-      s_id[j] = valid ? int(id) : -1;
-      s_q[j] = top * it;
-      if (valid) tmax = fmaxf(tmax, top * it);
+    for (int j = tid; j < K; j += THREADS) {
+      const Entry en = j == tid ? next : entry(row, j);
+      const bool valid = en.id >= 0 && en.id < V && en.top != -INFINITY;
+      const long long e = en.id + lead;
+      const int at = !valid ? -2 : e >= v_lo && e < v_hi ? int(e) : -1;   // -2: no entry, -1: one of another part
+      s_id[j] = at;
+      s_q[j] = en.top;
+      if (at >= 0) s_z[j] = to_f(z[en.id]);
+      if (valid) tmax = fmaxf(tmax, en.top);
     }
-    tmax = block_max(tmax, scratch);
-    const bool some = tmax != -INFINITY;                   // (also where an entry is NaN beside others; all NaN: no entry)
-    float sums[2] = {0.f, 0.f};
-    if (p.lse == nullptr) {
-      for (int j = tid; j < K; j += DISTILL_THREADS)
-        if (s_id[j] >= 0) sums[0] += exp2_fast((s_q[j] - tmax) * LOG2E);
-      block_sum<1>(reinterpret_cast<float(&)[1]>(sums[0]), scratch);
+    {
+      // pieces at the ends of the row: its elements, and -inf around them
+      const int a = first_whole(q) * VN, b = max(a, last_whole(q) * VN);
+      for (int i = tid; i < a + n - b; i += THREADS) {
+        const int v = i < a ? i : b + i - a;
+        elem[v] = v >= v_lo && v < v_hi ? z[v - lead] : ninf;
+      }
     }
-    // log q_j = s_q[j] - tmax - log of the sum, or s_q[j] - lse
-    const float q_sub = p.lse ? p.lse[row] : tmax, q_log = p.lse || !some ? 0.f : log_exact(sums[0]);
-    for (int j = tid; j < K; j += DISTILL_THREADS) {
-      const int id = s_id[j];
-      if (id < 0) continue;
-      const int b = bit_at(id);
-      if (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31) & 1) { repeated = 1; }
+    if (tid == 0) repeated = 0;
+    if (tid < K && row + row_step < p.rows) next = entry(row + row_step, tid);
+    tmax = reduce.template one<true>(tmax);
+    const bool some = tmax != -INFINITY;
+    float q_sum = 1.f;                                 // log q = top - lse, or top - tmax - log of this sum
+    if (p.lse == nullptr && some) {
+      float sum = 0.f;
+      for (int j = tid; j < K; j += THREADS)
+        if (s_id[j] != -2) sum += exp2_fast((s_q[j] - tmax) * LOG2E);
+      q_sum = reduce.template one<false>(sum);
     }
+    const float q_sub = p.lse ? lse : tmax, q_inv = __fdiv_rn(1.f, q_sum);
+    // ---- the row ----
+    mbar_wait_bounded(&full, phase, &abort_flag, p.status);
+    phase ^= 1;
+    // S is taken out of the row: every entry leaves its number in its place, and the one whose number is found there stands for
+    // the id and leaves -inf (whose bits are no entry's number)
+    using Bits = typename std::conditional<ES == 2, uint16_t, uint32_t>::type;
+    volatile Bits* place = reinterpret_cast<volatile Bits*>(buf);
+    for (int j = tid; j < K; j += THREADS)
+      if (s_id[j] >= 0) place[s_id[j]] = Bits(j);
     __syncthreads();
-    // ---- sums over the row: outside of S, then S ----
-    Online o;
-    auto inside = [&](int v) { const int b = bit_at(v); return (bits[b >> 5] >> (b & 31)) & 1u; };
-    for (int v = tid; v < nvec; v += DISTILL_THREADS) {
-      Vec<T> x;
-      x.load(z + head + v * VN);
+    unsigned owner = 0;                                // bit i: this thread's i-th entry stands for its id (K <= 1024)
+    float mx = -INFINITY;
+    for (int j = tid, i = 0; j < K; j += THREADS, ++i)
+      if (s_id[j] >= 0) {
+        if (place[s_id[j]] == Bits(j)) {
+          owner |= 1u << i;
+          place[s_id[j]] = ES == 2 ? Bits(0xff80u) : Bits(0xff800000u);
+          mx = fmaxf(mx, s_z[j]);
+        } else {
+          repeated = 1;
+        }
+      }
+    __syncthreads();
+    const Vec<T>* piece = reinterpret_cast<const Vec<T>*>(buf);
+#pragma unroll 4
+    for (int i = tid; i < q.pieces; i += THREADS) mx = fmaxf(mx, piece_max(piece[i]));
+    mx = reduce.template one<true>(mx);
+    const float m = mx == -INFINITY ? 0.f : mx;
+    const float mt = m * it2, m1 = m * LOG2E;
+    // out_t, out_1: sums over the others; in_t, in_1: over S; cross = sum of q (log q - (z - m) / t); mass = sum of q
+    float acc[8] = {};
+#pragma unroll 2
+    for (int i = tid; i < q.pieces; i += THREADS) {
       float f[VN];
-      x.to_float(f);
-      const int b = bit_at(head + v * VN);
-      const uint32_t in = (bits[b >> 5] >> (b & 31)) & ((1u << VN) - 1u);
-      if (in) {
+      piece[i].to_float(f);
 #pragma unroll
-        for (int j = 0; j < VN; ++j)
-          if (in >> j & 1) f[j] = -INFINITY;
+      for (int j = 0; j < VN; ++j) {
+        const float e = exp2_fast(fmaf(f[j], it2, -mt));
+        acc[0] += e;
+        if (MODE != 0) acc[1] += plain_exp<MODE>(e, f[j], m1);
       }
-      float mx = f[0];
-#pragma unroll
-      for (int j = 1; j < VN; ++j) mx = fmaxf(mx, f[j]);
-      o.raise(mx, it2);
-#pragma unroll
-      for (int j = 0; j < VN; ++j) o.add(f[j], it2);
     }
-    for (int c = tid; c < head + (V - tail); c += DISTILL_THREADS) {
-      const int v = c < head ? c : tail + c - head;
-      if (inside(v)) continue;
-      const float f = to_f(z[v]);
-      o.raise(f, it2);
-      o.add(f, it2);
+    for (int j = tid, i = 0; j < K; j += THREADS, ++i) {
+      if (s_id[j] == -2) continue;
+      const float logq = s_q[j] - q_sub, qj = exp2_fast(logq * LOG2E) * q_inv;     // (without the logarithm of q_sum)
+      s_q[j] = qj;
+      if (s_id[j] < 0) continue;
+      if (qj > 0.f) acc[4] += qj * (logq - (s_z[j] - m) * it);
+      acc[5] += qj;
+      if (owner >> i & 1) {
+        const float e = exp2_fast(fmaf(s_z[j], it2, -mt));
+        acc[2] += e;
+        if (MODE != 0) acc[3] += plain_exp<MODE>(e, s_z[j], m1);
+      }
     }
-    float m = o.m;
-    for (int j = tid; j < K; j += DISTILL_THREADS)
-      if (s_id[j] >= 0) m = fmaxf(m, to_f(z[s_id[j]]));
-    m = block_max(m, scratch);
-    if (m == -INFINITY) m = 0.f;                           // a row of nothing but -inf: sums of zero
-    const float keep = o.m == -INFINITY ? 0.f : 1.f;
-    float acc[4] = {keep * o.st * exp2_fast(keep == 0.f ? 0.f : (o.m - m) * it2), keep * o.s1 * exp2_fast(keep == 0.f ? 0.f : (o.m - m) * LOG2E), 0.f, 0.f};
-    // S: an id that is listed twice counts once, for its first entry
+    reduce.eight(acc);
     const bool twice = repeated != 0;
-    for (int j = tid; j < K; j += DISTILL_THREADS) {
-      const int id = s_id[j];
-      if (id < 0) continue;
-      bool first = true;
-      if (twice) for (int i = 0; i < j; ++i) if (s_id[i] == id) { first = false; break; }
-      if (!first) continue;
-      const float f = to_f(z[id]) - m;
-      acc[2] += exp2_fast(f * it2);
-      acc[3] += exp2_fast(f * LOG2E);
-    }
-    block_sum<4>(acc, scratch);
-    const float s_out = acc[0], s_t = acc[0] + acc[2], s_1 = acc[1] + acc[3];
-    const float log_t = log_exact(s_t);
-    // ---- the loss ----
-    sums[0] = sums[1] = 0.f;
-    for (int j = tid; j < K; j += DISTILL_THREADS) {
-      const int id = s_id[j];
-      if (id < 0) continue;
-      const float logq = s_q[j] - q_sub - q_log, q = exp2_fast(logq * LOG2E);
-      if (q > 0.f) sums[0] += q * (logq - ((to_f(z[id]) - m) * it - log_t));
-      sums[1] += q;
-      s_q[j] = q;
-    }
-    block_sum<2>(sums, scratch);
-    float soft = sums[0], mass = sums[1], ratio = 0.f;
-    if (p.lse) {
-      const float q_o = fmaxf(0.f, 1.f - mass), p_o = s_out / s_t;
-      if (q_o > 0.f && p_o > 0.f) {
-        ratio = q_o / p_o;
-        soft += q_o * log_exact(ratio);
-        mass += q_o;
+    // ---- together with the other parts ----
+    float M = m;                                       // maximum of the row
+    if (C > 1) {
+      PartSums* mine = &parts[int((row - row0) / row_step) & 1];
+      if (tid == 0) *mine = {mx, acc[0], acc[1], acc[2], acc[3], acc[4], acc[5], label_here ? z_label : -INFINITY};
+      __syncwarp();
+      cluster_sync();
+      PartSums all[8];
+      M = -INFINITY;
+      for (int c = 0; c < C; ++c) {
+        uint32_t at;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(c));
+        float4 a, b;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w) : "r"(at) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w) : "r"(at + 16) : "memory");
+        all[c] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        M = fmaxf(M, a.x);
       }
+      if (M == -INFINITY) M = 0.f;
+#pragma unroll
+      for (int i = 0; i < 6; ++i) acc[i] = 0.f;
+      z_label = -INFINITY;
+      for (int c = 0; c < C; ++c) {
+        const PartSums& o = all[c];
+        z_label = fmaxf(z_label, o.label);
+        const bool none = o.m == -INFINITY;
+        const float own_m = none ? 0.f : o.m;
+        if (!none) {
+          const float et = exp2_fast((own_m - M) * it2), e1 = exp2_fast((own_m - M) * LOG2E);
+          acc[0] += o.out_t * et;
+          acc[1] += o.out_1 * e1;
+          acc[2] += o.in_t * et;
+          acc[3] += o.in_1 * e1;
+        }
+        acc[4] += o.cross + o.mass * ((M - own_m) * it);
+        acc[5] += o.mass;
+      }
+    } else if (!label_here) {
+      z_label = 0.f;
     }
-    const long long lab = p.labels ? p.labels[row] : -1;
-    const bool hard = lab >= 0 && lab < V;
-    if (tid == 0) {
-      float l = some ? p.alpha * p.temperature * p.temperature * soft : 0.f;
-      if (hard) l += (1.f - p.alpha) * (log_exact(s_1) - (to_f(z[lab]) - m));
+    const float s_t = acc[0] + acc[2], s_1 = MODE == 0 ? s_t : acc[1] + acc[3], p_o = acc[0] / s_t;
+    const float q_in = acc[5], q_o = p.lse ? fmaxf(0.f, 1.f - q_in) : 0.f;
+    const bool rest = q_o > 0.f && p_o > 0.f;
+    const float ratio = rest ? q_o / p_o : 0.f, mass = rest ? q_in + q_o : q_in;
+    const bool hard = label >= 0 && label < V && p.alpha < 1.f;
+    if (tid == 0 && rank == 0) {
+      const float log_t = log_exact(s_t);
+      float l = 0.f;
+      if (some && p.alpha > 0.f) {
+        float soft = acc[4];
+        if (q_in > 0.f) soft += q_in * (p.lse ? log_t : log_t - log_exact(q_sum));
+        if (rest) soft += q_o * log_exact(ratio);
+        l = p.alpha * p.temperature * p.temperature * soft;
+      }
+      if (hard) l += (1.f - p.alpha) * ((MODE == 0 ? log_t : log_exact(s_1)) - (z_label - M));
       p.loss[row] = l;
     }
     if constexpr (GRAD) {
@@ -198,92 +362,148 @@ __global__ void __launch_bounds__(DISTILL_THREADS) distill_kernel(const __grid_c
       const float g = p.dloss[row];
       const float gs = some ? g * p.alpha * p.temperature : 0.f;   // alpha t^2 / t
       const float gh = hard ? g * (1.f - p.alpha) : 0.f;
-      const float ct = gs * (mass - ratio) / s_t, c1 = gh / s_1, ct_in = gs * mass / s_t;
+      // gradient = ct * exp((z - M) / t) + c1 * exp(z - M); a row of weight zero has none, whatever it holds
       const bool zero = g == 0.f || (gs == 0.f && gh == 0.f);
-      auto grad = [&](float f, int v) {
-        float d = 0.f;
-        if (gs != 0.f) d = ct * exp2_fast((f - m) * it2);
-        if (gh != 0.f) {
-          d += c1 * exp2_fast((f - m) * LOG2E);
-          if (v == lab) d -= gh;
-        }
-        return d;
+      float ct = gs != 0.f ? gs * (mass - ratio) / s_t : 0.f, ct_in = gs != 0.f ? gs * mass / s_t : 0.f, c1 = gh != 0.f ? gh / s_1 : 0.f;
+      if (MODE == 0) { ct += c1; ct_in += c1; c1 = 0.f; }
+      const float Mt = M * it2, M1 = M * LOG2E;
+      auto grad = [&](float f, float c) {
+        const float e = exp2_fast(fmaf(f, it2, -Mt));
+        return MODE == 0 ? c * e : fmaf(c, e, c1 * plain_exp<MODE>(e, f, M1));
       };
-      for (int v = tid; v < nvec; v += DISTILL_THREADS) {
-        Vec<T> x;
-        float f[VN];
-        if (zero) {
+      uint8_t* out = static_cast<uint8_t*>(p.dlogits) + q.lo * 16;
+      const int a = first_whole(q), b = last_whole(q);
+      if (zero) {
+        for (int i = a + tid; i < b; i += THREADS) *reinterpret_cast<uint4*>(out + size_t(i) * 16) = make_uint4(0, 0, 0, 0);
+      } else {
+#pragma unroll 2
+        for (int i = a + tid; i < b; i += THREADS) {
+          float f[VN];
+          piece[i].to_float(f);
 #pragma unroll
-          for (int j = 0; j < VN; ++j) f[j] = 0.f;
-        } else {
-          x.load(z + head + v * VN);
-          x.to_float(f);
-#pragma unroll
-          for (int j = 0; j < VN; ++j) f[j] = grad(f[j], head + v * VN + j);
-        }
-        x.from_float(f);
-        x.store(dz + head + v * VN);
-      }
-      for (int c = tid; c < head + (V - tail); c += DISTILL_THREADS) {
-        const int v = c < head ? c : tail + c - head;
-        dz[v] = from_f<T>(zero ? 0.f : grad(to_f(z[v]), v));
-      }
-      if (!zero && gs != 0.f) {
-        __syncthreads();          // the entries of S are written again
-        for (int j = tid; j < K; j += DISTILL_THREADS) {
-          const int id = s_id[j];
-          if (id < 0) continue;
-          float q = s_q[j];
-          bool first = true;
-          if (twice) {
-            for (int i = 0; i < j; ++i) if (s_id[i] == id) { first = false; break; }
-            if (first) for (int i = j + 1; i < K; ++i) if (s_id[i] == id) q += s_q[i];
-          }
-          if (!first) continue;
-          const float f = to_f(z[id]) - m;
-          float d = ct_in * exp2_fast(f * it2) - gs * q;
-          if (gh != 0.f) d += c1 * exp2_fast(f * LOG2E) - (id == lab ? gh : 0.f);
-          dz[id] = from_f<T>(d);
+          for (int j = 0; j < VN; ++j) f[j] = grad(f[j], ct);
+          Vec<T> o;
+          o.from_float(f);
+          o.store(reinterpret_cast<T*>(out + size_t(i) * 16));
         }
       }
+      const int ae = a * VN, be = max(ae, b * VN);
+      for (int i = tid; i < ae + n - be; i += THREADS) {
+        const int v = i < ae ? i : be + i - ae;
+        if (v >= v_lo && v < v_hi) dz[v - lead] = from_f<T>(zero ? 0.f : grad(to_f(elem[v]), ct));
+      }
+      __syncthreads();            // the elements of S and the label's are written again; the row in shared memory is done with
+      if (!zero) {
+        for (int j = tid, i = 0; j < K; j += THREADS, ++i) {
+          if (!(owner >> i & 1)) continue;
+          const int e = s_id[j];
+          float qj = s_q[j];
+          if (twice)
+            for (int k = 0; k < K; ++k)
+              if (k != j && s_id[k] == e) qj += s_q[k];
+          float d = grad(s_z[j], ct_in) - gs * qj;
+          if (e == label_at) d -= gh;
+          dz[e - lead] = from_f<T>(d);
+        }
+        if (tid == THREADS - 1 && label_here && gh != 0.f) {
+          bool listed = false;
+          for (int k = 0; k < K; ++k) listed |= s_id[k] == label_at;
+          if (!listed) dz[label_at - lead] = from_f<T>(grad(to_f(elem[label_at]), ct) - gh);
+        }
+      }
+    }
+    fence_proxy_async();          // elements of the row were written here, the next row comes by the bulk-copy unit
+    __syncthreads();              // nothing of this row is read any more
+    if (tid == 0 && row + row_step < p.rows) fetch(part_of(row + row_step));
+  }
+  __syncwarp();
+  if (C > 1) cluster_sync();      // a CTA's sums are read by the others
+  if (abort_flag) {               // a copy may still be in flight: many times its time
+    const uint64_t begin = globaltimer_ns();
+    while (globaltimer_ns() - begin < 2000000) {
     }
   }
 }
 
-template <typename T>
-static int distill_launch(const DistillParams& p, cudaStream_t stream) {
-  const int smem = (2 * p.K + (p.V + 31) / 32 + 2) * 4;
+// How many CTAs share a row, and their size.  A CTA's part is what fits three or more times into an SM's shared memory, so that
+// some CTAs copy while others compute; fewer rows than SMs are cut further, down to 4 KB.
+struct DistillShape {
+  int cluster, buffer, smem, threads, per_sm;
+};
+static DistillShape distill_shape(long long rows, int V, int K, int es, int sms) {
+  DistillShape s;
+  const long long bytes = (long long)V * es + 32;
+  s.cluster = 1;
+  while (s.cluster < 8 && (bytes / s.cluster > 70 * 1024 || (rows * s.cluster * 2 <= sms && bytes / s.cluster > 8 * 1024))) s.cluster *= 2;
+  s.buffer = int((bytes / s.cluster + 32 + 127) / 128 * 128);
+  s.smem = s.buffer + 12 * K;
+  s.threads = s.buffer > 16 * 1024 ? 256 : 128;
+  const int by_smem = 226 * 1024 / (s.smem + 2560), by_threads = 1024 / s.threads;   // (registers for 1024 threads)
+  s.per_sm = by_smem < by_threads ? by_smem : by_threads;
+  if (s.per_sm < 1) s.per_sm = 1;
+  return s;
+}
+
+template <typename T, bool GRAD, int MODE, int THREADS>
+static int distill_go(const DistillParams& p, const DistillShape& shape, int sms, cudaStream_t stream) {
+  auto kernel = distill_kernel<T, GRAD, MODE, THREADS>;
+  if (shape.smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shape.smem);
+    if (e != cudaSuccess) return int(e);
+  }
+  const long long slots = (long long)sms * shape.per_sm / shape.cluster;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(int(p.rows < slots ? p.rows : slots) * shape.cluster);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = shape.smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = shape.cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = shape.cluster > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  return e != cudaSuccess ? int(e) : int(cudaGetLastError());
+}
+template <typename T, bool GRAD, int MODE>
+static int distill_threads(const DistillParams& p, const DistillShape& s, int sms, cudaStream_t stream) {
+  return s.threads == 256 ? distill_go<T, GRAD, MODE, 256>(p, s, sms, stream) : distill_go<T, GRAD, MODE, 128>(p, s, sms, stream);
+}
+template <typename T, bool GRAD>
+static int distill_mode(DistillParams p, cudaStream_t stream) {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int grid = int(p.rows < 4ll * sms ? p.rows : 4ll * sms);
-  auto go = [&](auto kernel) {
-    if (smem > 40 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (e != cudaSuccess) return int(e);
-    }
-    kernel<<<grid, DISTILL_THREADS, smem, stream>>>(p);
-    return int(cudaGetLastError());
-  };
-  return p.dlogits ? go(distill_kernel<T, true>) : go(distill_kernel<T, false>);
+  const DistillShape s = distill_shape(p.rows, p.V, p.K, sizeof(T), sms);
+  if (s.smem > 220 * 1024) return -JPB_ERR_BAD_ARGUMENT;
+  p.cluster = s.cluster;
+  p.buffer = s.buffer;
+  p.status = jpb_status_device_ptr();
+  if (p.alpha == 0.f) p.temperature = 1.f;          // the cross entropy alone
+  if (p.labels == nullptr || p.alpha == 1.f || p.temperature == 1.f) return distill_threads<T, GRAD, 0>(p, s, sms, stream);
+  if (p.temperature == 2.f) return distill_threads<T, GRAD, 1>(p, s, sms, stream);
+  if (p.temperature == 4.f) return distill_threads<T, GRAD, 2>(p, s, sms, stream);
+  return distill_threads<T, GRAD, 3>(p, s, sms, stream);
 }
 
 }  // namespace jpb
 
-// logits [rows, V] of dtype 0 = fp32 or 1 = bf16, contiguous; ids [rows, K] int64 (ids64) or int32; top [rows, K] fp32 (top_fp32)
-// or bf16; lse [rows] or null; labels [rows] or null; loss [rows].  With dlogits (like logits, its address alike modulo 16) the
-// gradient for the row weights dloss is written too.  K <= 1024; V at most 1.4 million.
+// logits [rows, V] of dtype 0 = fp32 or 1 = bf16, contiguous, on a 16-byte boundary; ids [rows, K] int64 (ids64) or int32; top
+// [rows, K] fp32 (top_fp32) or bf16; lse [rows] or null; labels [rows] or null; loss [rows].  With dlogits (like logits) the
+// gradient for the row weights dloss is written too.  K <= 1024; a row of logits takes at most 1.6 MB.
 JPB_API int jpb_distill(int dt, const float* dloss, const void* logits, const void* ids, int ids64, const void* top, int top_fp32,
                         const float* lse, const long long* labels, float temperature, float alpha, float* loss, void* dlogits,
                         long long rows, int V, int K, void* stream) {
   using namespace jpb;
   if (rows <= 0) return 0;
-  if (V <= 0 || K < 0 || K > DISTILL_MAX_K || V > 1400000 || (dlogits && !dloss) ||
-      (dlogits && ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15)))
+  if (V <= 0 || K < 0 || K > DISTILL_MAX_K || V > (8 * 200 * 1024) / (dt == 0 ? 4 : 2) || (dlogits && !dloss) ||
+      ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) & 15))
     return -JPB_ERR_BAD_ARGUMENT;
-  DistillParams p = {logits, ids, top, lse, labels, dloss, loss, dlogits, rows, V, K, ids64, top_fp32, temperature, alpha};
+  DistillParams p = {logits, ids, top, lse, labels, dloss, loss, dlogits, rows, V, K, ids64, top_fp32, temperature, alpha, 1, 0, nullptr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dt == 0) return distill_launch<float>(p, s);
-  if (dt == 1) return distill_launch<__nv_bfloat16>(p, s);
+  if (dt == 0) return dlogits ? distill_mode<float, true>(p, s) : distill_mode<float, false>(p, s);
+  if (dt == 1) return dlogits ? distill_mode<__nv_bfloat16, true>(p, s) : distill_mode<__nv_bfloat16, false>(p, s);
   return -JPB_ERR_BAD_ARGUMENT;
 }

@@ -649,7 +649,7 @@ def _distill(dloss, logits, ids, top, lse, labels, temperature, alpha):
     if top.dtype not in (torch.float32, torch.bfloat16):
         raise NativeError(f"distill_loss takes teacher logits in float32 or bfloat16, got {top.dtype}")
     dt = _dt(logits)
-    logits = logits.contiguous() if dloss is None else _vectors(logits)
+    logits = _vectors(logits)
     ids, top = ids.contiguous(), top.contiguous()
     lse, labels = (None if t is None else t.contiguous() for t in (lse, labels))
     V, K = logits.shape[-1], ids.shape[-1]

@@ -33,8 +33,8 @@ struct DistillParams {
   int V, K;
   int ids64, top_fp32;
   float temperature, alpha;
-  int cluster;                 // CTAs of a row
-  int buffer;                  // bytes of a CTA's part of a row
+  int log_cluster;             // CTAs of a row: 1, 2, 4 or 8
+  int buffer, buffers;         // bytes of a CTA's part of a row, and how many rows a CTA holds (1 or 2)
   int* status;
 };
 
@@ -87,6 +87,21 @@ struct CtaReduce {
     }
     return v;
   }
+  __device__ __forceinline__ void max2(float& a, float& b) {
+    float* s = scratch + slot * WARPS * 8;
+    slot ^= 1;
+    a = warp_max(a);
+    b = warp_max(b);
+    if ((threadIdx.x & 31) == 0) { s[threadIdx.x >> 5] = a; s[WARPS + (threadIdx.x >> 5)] = b; }
+    __syncthreads();
+    a = s[threadIdx.x & (WARPS - 1)];
+    b = s[WARPS + (threadIdx.x & (WARPS - 1))];
+#pragma unroll
+    for (int o = 1; o < WARPS; o <<= 1) {
+      a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+      b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+    }
+  }
   // Eight sums: lanes trade values until each has one of the eight, 9 shuffles instead of 40, and 10 after the barrier.
   __device__ __forceinline__ void eight(float (&v)[8]) {
     const int lane = threadIdx.x & 31;
@@ -120,7 +135,7 @@ __device__ __forceinline__ float piece_max(const Vec<__nv_bfloat16>& v) {
   return fmaxf(f.x, f.y);
 }
 
-// What a CTA tells the others about its part of a row; sums are relative to its maximum m (0 where it has nothing but -inf).
+// What a CTA tells the others about its part of a row; the sums of exponentials are relative to m.
 struct PartSums {
   float m, out_t, out_1, in_t, in_1, cross, mass, label;
 };
@@ -133,95 +148,143 @@ __device__ __forceinline__ float plain_exp(float e, float f, float m1) {   // ex
   if (MODE == 2) { const float s = e * e; return s * s; }
   return exp2_fast(fmaf(f, LOG2E, -m1));
 }
+// The same for pairs; k = log2(e) / t, -m / t and -m in units of log 2.
+__device__ __forceinline__ F2 exp2_pair(F2 x) { return f2(exp2_fast(x.lo()), exp2_fast(x.hi())); }
 
 template <typename T, bool GRAD, int MODE, int THREADS>
-__global__ void __launch_bounds__(THREADS) distill_kernel(const __grid_constant__ DistillParams p) {
+__global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const __grid_constant__ DistillParams p) {
   constexpr int VN = Vec<T>::N, ES = sizeof(T);
+  using Bits = typename std::conditional<ES == 2, uint16_t, uint32_t>::type;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float scratch[2 * THREADS / 32 * 8];
   __shared__ __align__(16) PartSums parts[2];
-  __shared__ uint64_t full;
-  __shared__ int abort_flag, repeated;
-  uint8_t* buf = smem;                                             // this CTA's part of the row
-  int* s_id = reinterpret_cast<int*>(smem + p.buffer);             // [K] ids of this part as element numbers of it, or -1
-  float* s_q = reinterpret_cast<float*>(s_id + p.K);               // [K] log q, then q
-  float* s_z = s_q + p.K;                                          // [K] the row's logits there
+  __shared__ uint64_t full[2];
+  __shared__ int abort_flag, repeated[2];
   const int tid = threadIdx.x, V = p.V, K = p.K;
-  const int C = p.cluster, rank = C > 1 ? int(cluster_ctarank()) : 0;
-  const long long row0 = blockIdx.x / C, row_step = gridDim.x / C;
+  const int rank = p.log_cluster ? int(cluster_ctarank()) : 0, C = 1 << p.log_cluster;
+  const long long row0 = blockIdx.x >> p.log_cluster, row_step = gridDim.x >> p.log_cluster;
+  const long long row_bytes = (long long)V * ES, step_bytes = row_step * row_bytes;
   const float it = 1.f / p.temperature, it2 = it * LOG2E;
   CtaReduce<THREADS / 32> reduce{scratch, 0};
   const T ninf = from_f<T>(-INFINITY);
 
-  // This CTA's part of row r: 16-byte pieces lo .. hi of the whole tensor, and the byte of the row's first element from lo on.
+  // This CTA's part of the row that begins at byte `begin`: 16-byte pieces lo .. of the whole tensor, and the byte of the row's
+  // first element from lo on.
   struct Part {
     long long lo;
     int pieces, lead;
   };
-  auto part_of = [&](long long r) {
-    const long long begin = r * V * ES, g0 = begin >> 4, g1 = (begin + (long long)V * ES + 15) >> 4, n = g1 - g0;
-    Part q;
-    q.lo = g0 + n * rank / C;
-    q.pieces = int(g0 + n * (rank + 1) / C - q.lo);
-    q.lead = int(begin - q.lo * 16);
-    return q;
+  auto part_of = [&](long long begin) {
+    const int lead = int(begin & 15), n = (lead + int(row_bytes) + 15) >> 4, a = (n * rank) >> p.log_cluster;
+    return Part{(begin >> 4) + a, ((n * (rank + 1)) >> p.log_cluster) - a, lead - a * 16};
   };
   // pieces that are wholly in the row: copied at once; the one or two others hold elements of the next rows
   auto first_whole = [&](const Part& q) { return q.lead > 0 ? 1 : 0; };
-  auto last_whole = [&](const Part& q) { return min(q.pieces, (q.lead + V * ES) >> 4); };
-  auto fetch = [&](const Part& q) {     // one thread
+  auto last_whole = [&](const Part& q) { return min(q.pieces, (q.lead + int(row_bytes)) >> 4); };
+  auto fetch = [&](long long begin, int which) {     // one thread
+    const Part q = part_of(begin);
     const int a = first_whole(q), b = last_whole(q);
     if (b > a) {
-      mbar_expect_tx(&full, uint32_t(b - a) * 16);
-      bulk_load(buf + a * 16, static_cast<const uint8_t*>(p.logits) + (q.lo + a) * 16, uint32_t(b - a) * 16, &full);
+      mbar_expect_tx(&full[which], uint32_t(b - a) * 16);
+      bulk_load(smem + which * p.buffer + a * 16, static_cast<const uint8_t*>(p.logits) + (q.lo + a) * 16, uint32_t(b - a) * 16, &full[which]);
     } else {
-      mbar_arrive(&full);
+      mbar_arrive(&full[which]);
     }
   };
-  struct Entry {
-    long long id;
-    float top;
+  // What a row needs beside its logits is asked for a row ahead: first the entries (one a thread; further ones when their turn
+  // comes), the label and the row's numbers, and when these are there the logits that they name.  All of it is kept as it comes:
+  // a conversion would wait for the load.
+  struct Ahead {
+    uint32_t id_lo, id_hi, top, z, z_label;
+    float lse, g;
+    long long label;
   };
-  auto entry = [&](long long r, int j) {
+  auto raw_entry = [&](long long r, int j, Ahead& h) {
     const size_t at = size_t(r) * K + j;
-    Entry e;
-    e.id = p.ids64 ? static_cast<const long long*>(p.ids)[at] : (long long)static_cast<const int*>(p.ids)[at];
-    e.top = it * (p.top_fp32 ? static_cast<const float*>(p.top)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.top)[at]));
-    return e;
+    if (p.ids64) {
+      const uint2 w = static_cast<const uint2*>(p.ids)[at];
+      h.id_lo = w.x; h.id_hi = w.y;
+    } else {
+      h.id_lo = static_cast<const uint32_t*>(p.ids)[at];
+    }
+    h.top = p.top_fp32 ? static_cast<const uint32_t*>(p.top)[at] : static_cast<const uint16_t*>(p.top)[at];
   };
+  auto id_of = [&](const Ahead& h) { return p.ids64 ? (long long)(uint64_t(h.id_hi) << 32 | h.id_lo) : (long long)int(h.id_lo); };
+  auto raw_logit = [&](long long r, long long v) { return uint32_t(static_cast<const Bits*>(p.logits)[size_t(r) * V + v]); };
+  auto logit_of = [&](uint32_t raw) { return __uint_as_float(ES == 2 ? raw << 16 : raw); };
+  auto ahead_ids = [&](long long r) {
+    Ahead h;
+    h.id_lo = h.id_hi = 0xffffffffu;        // no entry
+    h.top = h.z = h.z_label = 0;
+    if (tid < K) raw_entry(r, tid, h);
+    h.label = p.labels ? p.labels[r] : -1;
+    h.lse = p.lse ? p.lse[r] : 0.f;
+    h.g = GRAD ? p.dloss[r] : 0.f;
+    return h;
+  };
+  auto ahead_logits = [&](long long r, Ahead& h) {
+    const long long id = id_of(h);
+    if (id >= 0 && id < V) h.z = raw_logit(r, id);
+    if (h.label >= 0 && h.label < V) h.z_label = raw_logit(r, h.label);
+  };
+  long long begin = row0 * row_bytes;
+  const int buffers = p.buffers;
   if (tid == 0) {
     abort_flag = 0;
-    mbar_init(&full, 1);
+    repeated[0] = repeated[1] = 0;
+    mbar_init(&full[0], 1);
+    mbar_init(&full[1], 1);
     fence_barrier_init();
-    if (row0 < p.rows) fetch(part_of(row0));
+    if (row0 < p.rows) fetch(begin, 0);
+    if (buffers == 2 && row0 + row_step < p.rows) fetch(begin + step_bytes, 1);
   }
-  Entry next = {-1, 0.f};         // the first entries of a row are asked for a row ahead
-  if (tid < K && row0 < p.rows) next = entry(row0, tid);
+  Ahead next;
+  if (row0 < p.rows) {
+    next = ahead_ids(row0);
+    ahead_logits(row0, next);
+  }
   __syncthreads();
-  uint32_t phase = 0;
-  for (long long row = row0; row < p.rows; row += row_step) {
-    const Part q = part_of(row);
+  uint32_t phase = 0;             // bit of each buffer
+  int which = 0, turn = 0;
+  for (long long row = row0; row < p.rows; row += row_step, begin += step_bytes, turn ^= 1, which = buffers == 2 ? which ^ 1 : 0) {
+    const Part q = part_of(begin);
+    uint8_t* buf = smem + which * p.buffer;          // this CTA's part of the row
+    // [K] elements of the part where the entries' ids are (-2: no entry, -1: in another part), their logits and probabilities;
+    // two sets take turns, so that the last gradients of a row need not be waited for
+    int* s_id = reinterpret_cast<int*>(smem + buffers * p.buffer) + turn * 3 * K;
+    float* s_q = reinterpret_cast<float*>(s_id + K);
+    float* s_z = s_q + K;
     T* elem = reinterpret_cast<T*>(buf);
-    const int lead = q.lead / ES;                    // element of the buffer that the row's first one would be (or is)
+    const int lead = q.lead / ES;                    // element of the part that the row's first one would be (or is)
     const int n = q.pieces * VN;
-    const int v_lo = max(lead, 0), v_hi = min(n, lead + V);        // buffer elements of the row
-    const T* z = static_cast<const T*>(p.logits) + size_t(row) * V;
-    // ---- the teacher's entries, and the row's logits there (from memory: the row is on its way) ----
-    const long long label = p.labels ? p.labels[row] : -1;
-    const float lse = p.lse ? p.lse[row] : 0.f;
+    const int v_lo = max(lead, 0), v_hi = min(n, lead + V);        // elements that are of the row
+    const T* z = reinterpret_cast<const T*>(static_cast<const uint8_t*>(p.logits) + begin);
+    // ---- the teacher's entries, and the row's logits there ----
+    const Ahead now = next;
+    const long long label = now.label;
     const bool label_here = label >= 0 && label < V && label + lead >= v_lo && label + lead < v_hi;
     const int label_at = label_here ? int(label + lead) : -1;
-    float z_label = label_here ? to_f(z[label]) : 0.f;
-    float tmax = -INFINITY;
+    const float z_own = logit_of(now.z_label);
+    float z_label = z_own;
+    const bool more = row + row_step < p.rows;
+    if (more) next = ahead_ids(row + row_step);
+    // the largest of the teacher's values, and of the row's logits at the same places
+    float top_max = -INFINITY, ref = -INFINITY;
     for (int j = tid; j < K; j += THREADS) {
-      const Entry en = j == tid ? next : entry(row, j);
-      const bool valid = en.id >= 0 && en.id < V && en.top != -INFINITY;
-      const long long e = en.id + lead;
-      const int at = !valid ? -2 : e >= v_lo && e < v_hi ? int(e) : -1;   // -2: no entry, -1: one of another part
-      s_id[j] = at;
-      s_q[j] = en.top;
-      if (at >= 0) s_z[j] = to_f(z[en.id]);
-      if (valid) tmax = fmaxf(tmax, en.top);
+      Ahead h = now;
+      if (j != tid) raw_entry(row, j, h);
+      const long long id = id_of(h);
+      const float top = it * __uint_as_float(p.top_fp32 ? h.top : h.top << 16);
+      const bool valid = id >= 0 && id < V && top != -INFINITY;
+      if (valid) {
+        const float zj = logit_of(j == tid ? h.z : raw_logit(row, id));
+        s_z[j] = zj;
+        top_max = fmaxf(top_max, top);
+        ref = fmaxf(ref, zj);
+      }
+      const long long e = id + lead;
+      s_id[j] = !valid ? -2 : e >= v_lo && e < v_hi ? int(e) : -1;
+      s_q[j] = top;
     }
     {
       // pieces at the ends of the row: its elements, and -inf around them
@@ -231,159 +294,175 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const __grid_constant_
         elem[v] = v >= v_lo && v < v_hi ? z[v - lead] : ninf;
       }
     }
-    if (tid == 0) repeated = 0;
-    if (tid < K && row + row_step < p.rows) next = entry(row + row_step, tid);
-    tmax = reduce.template one<true>(tmax);
-    const bool some = tmax != -INFINITY;
-    float q_sum = 1.f;                                 // log q = top - lse, or top - tmax - log of this sum
+    reduce.max2(top_max, ref);
+    const bool some = top_max != -INFINITY;
+    // The exponentials are taken relative to the largest logit among the entries (the label's, or 0, where there are none): the
+    // row's maximum is no further above it than fp32 has room for, or is looked up after all (below).
+    if (ref == -INFINITY) ref = label >= 0 && label < V && z_own != -INFINITY ? z_own : 0.f;
+    float q_sum = 1.f;                                 // log q = top - lse, or top - top_max - log of this sum
     if (p.lse == nullptr && some) {
       float sum = 0.f;
       for (int j = tid; j < K; j += THREADS)
-        if (s_id[j] != -2) sum += exp2_fast((s_q[j] - tmax) * LOG2E);
+        if (s_id[j] != -2) sum += exp2_fast((s_q[j] - top_max) * LOG2E);
       q_sum = reduce.template one<false>(sum);
     }
-    const float q_sub = p.lse ? lse : tmax, q_inv = __fdiv_rn(1.f, q_sum);
+    // out_t, out_1: sums over the others; in_t, in_1: over S; cross = sum of q (log q - (z - ref) / t) without the logarithm of
+    // q_sum; mass = sum of q
+    float out_t, out_1, in_t = 0.f, in_1 = 0.f, cross = 0.f, mass_in = 0.f;
+    {
+      const float q_sub = p.lse ? now.lse : top_max, q_inv = 1.f / q_sum;
+      for (int j = tid; j < K; j += THREADS) {
+        const int at = s_id[j];
+        if (at == -2) continue;
+        const float logq = s_q[j] - q_sub, qj = exp2_fast(logq * LOG2E) * q_inv;
+        s_q[j] = qj;
+        if (at < 0) continue;
+        if (qj > 0.f) cross += qj * (logq - (s_z[j] - ref) * it);
+        mass_in += qj;
+      }
+    }
     // ---- the row ----
-    mbar_wait_bounded(&full, phase, &abort_flag, p.status);
-    phase ^= 1;
+    mbar_wait_bounded(&full[which], (phase >> which) & 1, &abort_flag, p.status);
+    phase ^= 1u << which;
     // S is taken out of the row: every entry leaves its number in its place, and the one whose number is found there stands for
     // the id and leaves -inf (whose bits are no entry's number)
-    using Bits = typename std::conditional<ES == 2, uint16_t, uint32_t>::type;
     volatile Bits* place = reinterpret_cast<volatile Bits*>(buf);
     for (int j = tid; j < K; j += THREADS)
       if (s_id[j] >= 0) place[s_id[j]] = Bits(j);
+    if (tid == 0) repeated[turn ^ 1] = 0;
     __syncthreads();
     unsigned owner = 0;                                // bit i: this thread's i-th entry stands for its id (K <= 1024)
-    float mx = -INFINITY;
     for (int j = tid, i = 0; j < K; j += THREADS, ++i)
       if (s_id[j] >= 0) {
         if (place[s_id[j]] == Bits(j)) {
           owner |= 1u << i;
           place[s_id[j]] = ES == 2 ? Bits(0xff80u) : Bits(0xff800000u);
-          mx = fmaxf(mx, s_z[j]);
         } else {
-          repeated = 1;
+          repeated[turn] = 1;
         }
       }
     __syncthreads();
+    const bool twice = repeated[turn] != 0;
+    if (twice) {                                       // the first of its kind, whichever write came last
+      owner = 0;
+      for (int j = tid, i = 0; j < K; j += THREADS, ++i) {
+        bool first = s_id[j] >= 0;
+        for (int k = 0; k < j && first; ++k) first = s_id[k] != s_id[j];
+        if (first) owner |= 1u << i;
+      }
+    }
+    if (more) ahead_logits(row + row_step, next);
     const Vec<T>* piece = reinterpret_cast<const Vec<T>*>(buf);
-#pragma unroll 4
-    for (int i = tid; i < q.pieces; i += THREADS) mx = fmaxf(mx, piece_max(piece[i]));
-    mx = reduce.template one<true>(mx);
-    const float m = mx == -INFINITY ? 0.f : mx;
-    const float mt = m * it2, m1 = m * LOG2E;
-    // out_t, out_1: sums over the others; in_t, in_1: over S; cross = sum of q (log q - (z - m) / t); mass = sum of q
-    float acc[8] = {};
+    float m = ref;
+    for (int attempt = 0;; ++attempt) {
+      const float mt = m * it2, m1 = m * LOG2E;
+      F2 sum_t = f2(0.f), sum_1 = f2(0.f);
+      const F2 k = f2(it2), k1 = f2(LOG2E), at = f2(-mt), at1 = f2(-m1);
 #pragma unroll 2
-    for (int i = tid; i < q.pieces; i += THREADS) {
-      float f[VN];
-      piece[i].to_float(f);
+      for (int i = tid; i < q.pieces; i += THREADS) {
+        F2 f[VN / 2];
+        to_pairs(piece[i], f);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) {
-        const float e = exp2_fast(fmaf(f[j], it2, -mt));
-        acc[0] += e;
-        if (MODE != 0) acc[1] += plain_exp<MODE>(e, f[j], m1);
+        for (int j = 0; j < VN / 2; ++j) {
+          const F2 e = exp2_pair(fma2(f[j], k, at));
+          sum_t = sum_t + e;
+          if (MODE == 1) sum_1 = fma2(e, e, sum_1);
+          if (MODE == 2) { const F2 h = e * e; sum_1 = fma2(h, h, sum_1); }
+          if (MODE == 3) sum_1 = sum_1 + exp2_pair(fma2(f[j], k1, at1));
+        }
       }
+      in_t = in_1 = 0.f;
+      for (int j = tid, i = 0; j < K; j += THREADS, ++i)
+        if (owner >> i & 1) {
+          const float e = exp2_fast(fmaf(s_z[j], it2, -mt));
+          in_t += e;
+          if (MODE != 0) in_1 += plain_exp<MODE>(e, s_z[j], m1);
+        }
+      float acc[8] = {sum_t.lo() + sum_t.hi(), sum_1.lo() + sum_1.hi(), in_t, in_1, attempt ? 0.f : cross, attempt ? 0.f : mass_in, 0.f, 0.f};
+      if (!GRAD) fence_proxy_async();   // elements of the row were written here, the next row comes by the bulk-copy unit
+      reduce.eight(acc);
+      out_t = acc[0]; out_1 = acc[1]; in_t = acc[2]; in_1 = acc[3];
+      if (attempt == 0) { cross = acc[4]; mass_in = acc[5]; }
+      const float s_t = out_t + in_t, s_1 = MODE == 0 ? s_t : out_1 + in_1;
+      if (attempt || (s_t > 1e-30f && s_t < 1e30f && s_1 > 1e-30f && s_1 < 1e30f)) break;
+      // out of range: relative to this part's own maximum (the same in all threads: the sums are)
+      float mx = -INFINITY;
+      for (int i = tid; i < q.pieces; i += THREADS) mx = fmaxf(mx, piece_max(piece[i]));
+      for (int j = tid; j < K; j += THREADS)
+        if (s_id[j] >= 0) mx = fmaxf(mx, s_z[j]);
+      mx = reduce.template one<true>(mx);
+      if (mx == -INFINITY) break;       // nothing here but -inf: sums of zero, relative to anything
+      m = mx;
     }
-    for (int j = tid, i = 0; j < K; j += THREADS, ++i) {
-      if (s_id[j] == -2) continue;
-      const float logq = s_q[j] - q_sub, qj = exp2_fast(logq * LOG2E) * q_inv;     // (without the logarithm of q_sum)
-      s_q[j] = qj;
-      if (s_id[j] < 0) continue;
-      if (qj > 0.f) acc[4] += qj * (logq - (s_z[j] - m) * it);
-      acc[5] += qj;
-      if (owner >> i & 1) {
-        const float e = exp2_fast(fmaf(s_z[j], it2, -mt));
-        acc[2] += e;
-        if (MODE != 0) acc[3] += plain_exp<MODE>(e, s_z[j], m1);
-      }
-    }
-    reduce.eight(acc);
-    const bool twice = repeated != 0;
+    if (!GRAD && tid == THREADS - 32 && row + row_step * buffers < p.rows) fetch(begin + step_bytes * buffers, which);   // (all have read it)
     // ---- together with the other parts ----
-    float M = m;                                       // maximum of the row
+    float M = m;
     if (C > 1) {
-      PartSums* mine = &parts[int((row - row0) / row_step) & 1];
-      if (tid == 0) *mine = {mx, acc[0], acc[1], acc[2], acc[3], acc[4], acc[5], label_here ? z_label : -INFINITY};
+      PartSums* mine = &parts[turn];
+      if (tid == 0) *mine = {m, out_t, out_1, in_t, in_1, cross, mass_in, label_here ? z_own : -INFINITY};
       __syncwarp();
       cluster_sync();
-      PartSums all[8];
-      M = -INFINITY;
-      for (int c = 0; c < C; ++c) {
+      auto read = [&](int c) {
         uint32_t at;
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(c));
-        float4 a, b;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w) : "r"(at) : "memory");
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w) : "r"(at + 16) : "memory");
-        all[c] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        M = fmaxf(M, a.x);
-      }
-      if (M == -INFINITY) M = 0.f;
-#pragma unroll
-      for (int i = 0; i < 6; ++i) acc[i] = 0.f;
-      z_label = -INFINITY;
-      for (int c = 0; c < C; ++c) {
-        const PartSums& o = all[c];
-        z_label = fmaxf(z_label, o.label);
-        const bool none = o.m == -INFINITY;
-        const float own_m = none ? 0.f : o.m;
-        if (!none) {
-          const float et = exp2_fast((own_m - M) * it2), e1 = exp2_fast((own_m - M) * LOG2E);
-          acc[0] += o.out_t * et;
-          acc[1] += o.out_1 * e1;
-          acc[2] += o.in_t * et;
-          acc[3] += o.in_1 * e1;
-        }
-        acc[4] += o.cross + o.mass * ((M - own_m) * it);
-        acc[5] += o.mass;
-      }
-    } else if (!label_here) {
-      z_label = 0.f;
-    }
-    const float s_t = acc[0] + acc[2], s_1 = MODE == 0 ? s_t : acc[1] + acc[3], p_o = acc[0] / s_t;
-    const float q_in = acc[5], q_o = p.lse ? fmaxf(0.f, 1.f - q_in) : 0.f;
-    const bool rest = q_o > 0.f && p_o > 0.f;
-    const float ratio = rest ? q_o / p_o : 0.f, mass = rest ? q_in + q_o : q_in;
-    const bool hard = label >= 0 && label < V && p.alpha < 1.f;
-    if (tid == 0 && rank == 0) {
-      const float log_t = log_exact(s_t);
-      float l = 0.f;
-      if (some && p.alpha > 0.f) {
-        float soft = acc[4];
-        if (q_in > 0.f) soft += q_in * (p.lse ? log_t : log_t - log_exact(q_sum));
-        if (rest) soft += q_o * log_exact(ratio);
-        l = p.alpha * p.temperature * p.temperature * soft;
-      }
-      if (hard) l += (1.f - p.alpha) * ((MODE == 0 ? log_t : log_exact(s_1)) - (z_label - M));
-      p.loss[row] = l;
-    }
-    if constexpr (GRAD) {
-      T* dz = static_cast<T*>(p.dlogits) + size_t(row) * V;
-      const float g = p.dloss[row];
-      const float gs = some ? g * p.alpha * p.temperature : 0.f;   // alpha t^2 / t
-      const float gh = hard ? g * (1.f - p.alpha) : 0.f;
-      // gradient = ct * exp((z - M) / t) + c1 * exp(z - M); a row of weight zero has none, whatever it holds
-      const bool zero = g == 0.f || (gs == 0.f && gh == 0.f);
-      float ct = gs != 0.f ? gs * (mass - ratio) / s_t : 0.f, ct_in = gs != 0.f ? gs * mass / s_t : 0.f, c1 = gh != 0.f ? gh / s_1 : 0.f;
-      if (MODE == 0) { ct += c1; ct_in += c1; c1 = 0.f; }
-      const float Mt = M * it2, M1 = M * LOG2E;
-      auto grad = [&](float f, float c) {
-        const float e = exp2_fast(fmaf(f, it2, -Mt));
-        return MODE == 0 ? c * e : fmaf(c, e, c1 * plain_exp<MODE>(e, f, M1));
+        PartSums o;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.m), "=f"(o.out_t), "=f"(o.out_1), "=f"(o.in_t) : "r"(at) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.in_1), "=f"(o.cross), "=f"(o.mass), "=f"(o.label) : "r"(at + 16) : "memory");
+        return o;
       };
+      out_t = out_1 = in_t = in_1 = cross = mass_in = 0.f;
+      M = z_label = -INFINITY;
+      for (int c = 0; c < C; ++c) M = fmaxf(M, read(c).m);
+      for (int c = 0; c < C; ++c) {
+        const PartSums o = read(c);
+        const float et = exp2_fast((o.m - M) * it2), e1 = exp2_fast((o.m - M) * LOG2E);
+        out_t += o.out_t * et;
+        out_1 += o.out_1 * e1;
+        in_t += o.in_t * et;
+        in_1 += o.in_1 * e1;
+        cross += o.cross;
+        mass_in += o.mass;
+        z_label = fmaxf(z_label, o.label);
+      }
+    }
+    const float s_t = out_t + in_t, s_1 = MODE == 0 ? s_t : out_1 + in_1, p_o = out_t / s_t;
+    const float q_o = p.lse ? fmaxf(0.f, 1.f - mass_in) : 0.f;
+    const bool rest = q_o > 0.f && p_o > 0.f;
+    const float ratio = rest ? q_o / p_o : 0.f, mass = rest ? mass_in + q_o : mass_in;
+    const bool hard = label >= 0 && label < V && p.alpha < 1.f;
+    T* dz = reinterpret_cast<T*>(static_cast<uint8_t*>(p.dlogits) + begin);
+    const float gs = some ? now.g * p.alpha * p.temperature : 0.f;   // alpha t^2 / t
+    const float gh = hard ? now.g * (1.f - p.alpha) : 0.f;
+    // gradient = ct * exp((z - M) / t) + c1 * exp(z - M); a row of weight zero has none, whatever it holds
+    const bool zero = now.g == 0.f || (gs == 0.f && gh == 0.f);
+    float ct = gs != 0.f ? gs * (mass - ratio) / s_t : 0.f, ct_in = gs != 0.f ? gs * mass / s_t : 0.f, c1 = gh != 0.f ? gh / s_1 : 0.f;
+    if (MODE == 0) { ct += c1; ct_in += c1; c1 = 0.f; }
+    const float Mt = M * it2, M1 = M * LOG2E;
+    auto grad = [&](float f, float c) {
+      const float e = exp2_fast(fmaf(f, it2, -Mt));
+      return MODE == 0 ? c * e : fmaf(c, e, c1 * plain_exp<MODE>(e, f, M1));
+    };
+    if constexpr (GRAD) {
       uint8_t* out = static_cast<uint8_t*>(p.dlogits) + q.lo * 16;
       const int a = first_whole(q), b = last_whole(q);
       if (zero) {
         for (int i = a + tid; i < b; i += THREADS) *reinterpret_cast<uint4*>(out + size_t(i) * 16) = make_uint4(0, 0, 0, 0);
       } else {
+        const F2 k = f2(it2), k1 = f2(LOG2E), at = f2(-Mt), at1 = f2(-M1), wt = f2(ct), w1 = f2(c1);
 #pragma unroll 2
         for (int i = a + tid; i < b; i += THREADS) {
-          float f[VN];
-          piece[i].to_float(f);
+          F2 f[VN / 2];
+          to_pairs(piece[i], f);
 #pragma unroll
-          for (int j = 0; j < VN; ++j) f[j] = grad(f[j], ct);
+          for (int j = 0; j < VN / 2; ++j) {
+            const F2 e = exp2_pair(fma2(f[j], k, at));
+            if (MODE == 0) f[j] = wt * e;
+            if (MODE == 1) f[j] = e * fma2(w1, e, wt);
+            if (MODE == 2) { const F2 h = e * e; f[j] = e * fma2(w1 * h, e, wt); }
+            if (MODE == 3) f[j] = fma2(wt, e, w1 * exp2_pair(fma2(f[j], k1, at1)));
+          }
           Vec<T> o;
-          o.from_float(f);
+          from_pairs(o, f);
           o.store(reinterpret_cast<T*>(out + size_t(i) * 16));
         }
       }
@@ -392,15 +471,17 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const __grid_constant_
         const int v = i < ae ? i : be + i - ae;
         if (v >= v_lo && v < v_hi) dz[v - lead] = from_f<T>(zero ? 0.f : grad(to_f(elem[v]), ct));
       }
-      __syncthreads();            // the elements of S and the label's are written again; the row in shared memory is done with
+      fence_proxy_async();
+      __syncthreads();            // the row is done with; the elements of S and the label's are written again
+      if (tid == THREADS - 32 && row + row_step * buffers < p.rows) fetch(begin + step_bytes * buffers, which);
       if (!zero) {
         for (int j = tid, i = 0; j < K; j += THREADS, ++i) {
           if (!(owner >> i & 1)) continue;
           const int e = s_id[j];
           float qj = s_q[j];
           if (twice)
-            for (int k = 0; k < K; ++k)
-              if (k != j && s_id[k] == e) qj += s_q[k];
+            for (int k = j + 1; k < K; ++k)
+              if (s_id[k] == e) qj += s_q[k];
           float d = grad(s_z[j], ct_in) - gs * qj;
           if (e == label_at) d -= gh;
           dz[e - lead] = from_f<T>(d);
@@ -408,19 +489,29 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const __grid_constant_
         if (tid == THREADS - 1 && label_here && gh != 0.f) {
           bool listed = false;
           for (int k = 0; k < K; ++k) listed |= s_id[k] == label_at;
-          if (!listed) dz[label_at - lead] = from_f<T>(grad(to_f(elem[label_at]), ct) - gh);
+          if (!listed) dz[label_at - lead] = from_f<T>(grad(z_own, ct) - gh);
         }
       }
     }
-    fence_proxy_async();          // elements of the row were written here, the next row comes by the bulk-copy unit
-    __syncthreads();              // nothing of this row is read any more
-    if (tid == 0 && row + row_step < p.rows) fetch(part_of(row + row_step));
+    if (tid < 32 && rank == 0) {  // the loss: its logarithms in four lanes
+      const float l4 = log_exact(tid == 1 ? q_sum : tid == 2 ? (rest ? ratio : 1.f) : tid == 3 ? s_1 : s_t);
+      const float log_t = __shfl_sync(0xffffffffu, l4, 0), log_q = __shfl_sync(0xffffffffu, l4, 1), log_r = __shfl_sync(0xffffffffu, l4, 2),
+                  log_1 = __shfl_sync(0xffffffffu, l4, 3);
+      float l = 0.f;
+      if (some && p.alpha > 0.f) {
+        float soft = cross + q_o * log_r;
+        if (mass_in > 0.f) soft += mass_in * (log_t + (M - ref) * it - log_q);
+        l = p.alpha * p.temperature * p.temperature * soft;
+      }
+      if (hard) l += (1.f - p.alpha) * (log_1 - (z_label - M));
+      if (tid == 0) p.loss[row] = l;
+    }
   }
   __syncwarp();
   if (C > 1) cluster_sync();      // a CTA's sums are read by the others
   if (abort_flag) {               // a copy may still be in flight: many times its time
-    const uint64_t begin = globaltimer_ns();
-    while (globaltimer_ns() - begin < 2000000) {
+    const uint64_t start = globaltimer_ns();
+    while (globaltimer_ns() - start < 2000000) {
     }
   }
 }
@@ -428,7 +519,7 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(const __grid_constant_
 // How many CTAs share a row, and their size.  A CTA's part is what fits three or more times into an SM's shared memory, so that
 // some CTAs copy while others compute; fewer rows than SMs are cut further, down to 4 KB.
 struct DistillShape {
-  int cluster, buffer, smem, threads, per_sm;
+  int cluster, buffer, buffers, smem, threads, per_sm;
 };
 static DistillShape distill_shape(long long rows, int V, int K, int es, int sms) {
   DistillShape s;
@@ -436,10 +527,12 @@ static DistillShape distill_shape(long long rows, int V, int K, int es, int sms)
   s.cluster = 1;
   while (s.cluster < 8 && (bytes / s.cluster > 70 * 1024 || (rows * s.cluster * 2 <= sms && bytes / s.cluster > 8 * 1024))) s.cluster *= 2;
   s.buffer = int((bytes / s.cluster + 32 + 127) / 128 * 128);
-  s.smem = s.buffer + 12 * K;
   s.threads = s.buffer > 16 * 1024 ? 256 : 128;
-  const int by_smem = 226 * 1024 / (s.smem + 2560), by_threads = 1024 / s.threads;   // (registers for 1024 threads)
-  s.per_sm = by_smem < by_threads ? by_smem : by_threads;
+  const int by_threads = 768 / s.threads;              // (registers for 768 threads)
+  auto by_smem = [&](int buffers) { return 226 * 1024 / (buffers * s.buffer + 24 * K + 2560); };
+  s.buffers = by_smem(2) >= by_threads ? 2 : 1;
+  s.smem = s.buffers * s.buffer + 24 * K;
+  s.per_sm = by_smem(s.buffers) < by_threads ? by_smem(s.buffers) : by_threads;
   if (s.per_sm < 1) s.per_sm = 1;
   return s;
 }
@@ -478,8 +571,9 @@ static int distill_mode(DistillParams p, cudaStream_t stream) {
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const DistillShape s = distill_shape(p.rows, p.V, p.K, sizeof(T), sms);
   if (s.smem > 220 * 1024) return -JPB_ERR_BAD_ARGUMENT;
-  p.cluster = s.cluster;
+  p.log_cluster = s.cluster == 8 ? 3 : s.cluster == 4 ? 2 : s.cluster == 2;
   p.buffer = s.buffer;
+  p.buffers = s.buffers;
   p.status = jpb_status_device_ptr();
   if (p.alpha == 0.f) p.temperature = 1.f;          // the cross entropy alone
   if (p.labels == nullptr || p.alpha == 1.f || p.temperature == 1.f) return distill_threads<T, GRAD, 0>(p, s, sms, stream);
@@ -501,7 +595,7 @@ JPB_API int jpb_distill(int dt, const float* dloss, const void* logits, const vo
   if (V <= 0 || K < 0 || K > DISTILL_MAX_K || V > (8 * 200 * 1024) / (dt == 0 ? 4 : 2) || (dlogits && !dloss) ||
       ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) & 15))
     return -JPB_ERR_BAD_ARGUMENT;
-  DistillParams p = {logits, ids, top, lse, labels, dloss, loss, dlogits, rows, V, K, ids64, top_fp32, temperature, alpha, 1, 0, nullptr};
+  DistillParams p = {logits, ids, top, lse, labels, dloss, loss, dlogits, rows, V, K, ids64, top_fp32, temperature, alpha, 0, 0, 1, nullptr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dt == 0) return dlogits ? distill_mode<float, true>(p, s) : distill_mode<float, false>(p, s);
   if (dt == 1) return dlogits ? distill_mode<__nv_bfloat16, true>(p, s) : distill_mode<__nv_bfloat16, false>(p, s);

@@ -15,6 +15,7 @@
 // What bounds it: HBM (a row read, and one written), then the exponentials, of which an SM does 16 a cycle: one per element for
 // the sums and one for the gradient.  With both temperatures in play the plain exponential is a power of the softened one where
 // t is 2 or 4, else it is taken too.
+#include "launch.cuh"
 #include "vec.cuh"
 
 #include <type_traits>
@@ -540,10 +541,8 @@ static DistillShape distill_shape(long long rows, int V, int K, int es, int sms)
 template <typename T, bool GRAD, int MODE, int THREADS>
 static int distill_go(const DistillParams& p, const DistillShape& shape, int sms, cudaStream_t stream) {
   auto kernel = distill_kernel<T, GRAD, MODE, THREADS>;
-  if (shape.smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shape.smem);
-    if (e != cudaSuccess) return int(e);
-  }
+  static SmemLimit limit;
+  if (const int rc = limit.allow(kernel, shape.smem)) return rc;
   const long long slots = (long long)sms * shape.per_sm / shape.cluster;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(int(p.rows < slots ? p.rows : slots) * shape.cluster);
@@ -566,9 +565,7 @@ static int distill_threads(const DistillParams& p, const DistillShape& s, int sm
 }
 template <typename T, bool GRAD>
 static int distill_mode(DistillParams p, cudaStream_t stream) {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = sm_count_of_device();
   const DistillShape s = distill_shape(p.rows, p.V, p.K, sizeof(T), sms);
   if (s.smem > 220 * 1024) return -JPB_ERR_BAD_ARGUMENT;
   p.log_cluster = s.cluster == 8 ? 3 : s.cluster == 4 ? 2 : s.cluster == 2;

@@ -13,6 +13,7 @@
 // (a product with zero in one alone would still be NaN where the other holds an infinity) before the product may read it.
 // Roles, ring, double-buffered accumulators and bounded waits are those of the plain GEMM.
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace jpb {
 namespace ragged {
@@ -657,18 +658,10 @@ ragged_wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_con
 // -------------------------------------------------------------------------------------------------------------
 // host side
 // -------------------------------------------------------------------------------------------------------------
-static int num_sms() {
-  int dev = 0, n = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n;
-}
-
 template <typename Kernel, typename... Args>
-static int launch(Kernel kernel, int cg, int smem, int threads, long long tiles, cudaStream_t stream, const Args&... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return int(e);
-  const int slots = num_sms() / cg;
+static int launch(SmemLimit& limit, Kernel kernel, int cg, int smem, int threads, long long tiles, cudaStream_t stream, const Args&... args) {
+  if (const int rc = limit.allow(kernel, smem)) return rc;
+  const int slots = sm_count_of_device() / cg;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(int(tiles < slots ? tiles : slots) * cg);
   cfg.blockDim = dim3(threads);
@@ -681,7 +674,7 @@ static int launch(Kernel kernel, int cg, int smem, int threads, long long tiles,
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cg > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   return e != cudaSuccess ? int(e) : int(cudaGetLastError());
 }
 
@@ -712,8 +705,9 @@ static int launch_rows(const void* w, const void* tokens, RowsParams& p, int w_m
   p.tiles_m = (p.M + 128 * CG - 1) / (128 * CG);
   const long long tiles = ((long long)(p.rows + BT - 1) / BT + p.groups) * p.tiles_m;
   if (tiles > 0x7fffffffll) return -JPB_ERR_BAD_ARGUMENT;
-  if (w_mn) return launch(ragged_rows_kernel<CG, BT, true>, CG, C::SMEM_BYTES, 192, tiles, stream, mw, mt, p);
-  return launch(ragged_rows_kernel<CG, BT, false>, CG, C::SMEM_BYTES, 192, tiles, stream, mw, mt, p);
+  static SmemLimit limit[2];
+  if (w_mn) return launch(limit[1], ragged_rows_kernel<CG, BT, true>, CG, C::SMEM_BYTES, 192, tiles, stream, mw, mt, p);
+  return launch(limit[0], ragged_rows_kernel<CG, BT, false>, CG, C::SMEM_BYTES, 192, tiles, stream, mw, mt, p);
 }
 
 static int columns_map(CUtensorMap* out, const void* t, uint64_t rows, uint64_t cols, uint32_t box_cols, int blocked) {
@@ -743,7 +737,8 @@ static int launch_wgrad(const void* dy, const void* x, void* D, WgradParams& p, 
   const long long tiles = (long long)p.tiles_n * p.tiles_k * p.groups;
   if (tiles > 0x7fffffffll) return -JPB_ERR_BAD_ARGUMENT;
   p.stages = C::stages(p.groups);
-  return launch(ragged_wgrad_kernel<CG, BN>, CG, C::smem_bytes(p.stages, p.groups), 224, tiles, stream, ma, mb, md, p);
+  static SmemLimit limit;
+  return launch(limit, ragged_wgrad_kernel<CG, BN>, CG, C::smem_bytes(p.stages, p.groups), 224, tiles, stream, ma, mb, md, p);
 }
 
 static bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -768,7 +763,7 @@ JPB_API int jpb_linear_ragged(const void* tokens, const void* w, const int* offs
   const int mean = (rows + groups - 1) / groups;
   if (mean <= 32) return launch_rows<1, 32>(w, tokens, p, transposed, s);
   const long long pairs = ((long long)rows / 256 + groups) * ((p.M + 255) / 256);
-  if (mean <= 128 || pairs < num_sms() / 4) return launch_rows<1, 128>(w, tokens, p, transposed, s);
+  if (mean <= 128 || pairs < sm_count_of_device() / 4) return launch_rows<1, 128>(w, tokens, p, transposed, s);
   return launch_rows<2, 256>(w, tokens, p, transposed, s);
 }
 
@@ -787,6 +782,6 @@ JPB_API int jpb_linear_ragged_wgrad(const void* dy, const void* x, const int* of
   p.offsets = offsets; p.groups = groups; p.rows = rows; p.N = N; p.K = K; p.dy_blocked = N % 64 == 0; p.x_blocked = K % 64 == 0;
   p.out_fp32 = out_fp32; p.accumulate = accumulate; p.status = jpb_status_device_ptr();
   const long long pairs = (long long)groups * ((N + 255) / 256) * ((K + 255) / 256);
-  if (pairs < num_sms() / 3) return launch_wgrad<1, 128>(dy, x, dw, p, s);
+  if (pairs < sm_count_of_device() / 3) return launch_wgrad<1, 128>(dy, x, dw, p, s);
   return launch_wgrad<2, 256>(dy, x, dw, p, s);
 }

@@ -1,0 +1,42 @@
+// What a launcher asks the runtime for again and again, kept per device: a call of a few microseconds of work should not spend
+// one on questions.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <atomic>
+
+namespace jpb {
+
+constexpr int MAX_DEVICES = 64;
+
+inline int current_device() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return dev >= 0 && dev < MAX_DEVICES ? dev : 0;
+}
+inline int sm_count_of_device() {
+  static std::atomic<int> sms[MAX_DEVICES];
+  const int dev = current_device();
+  int n = sms[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    sms[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+// The largest dynamic shared memory that a kernel was allowed so far (one object per kernel).
+struct SmemLimit {
+  std::atomic<int> bytes[MAX_DEVICES];
+  template <typename Kernel>
+  int allow(Kernel kernel, int want) {
+    const int dev = current_device();
+    if (want <= 48 * 1024 || want <= bytes[dev].load(std::memory_order_relaxed)) return 0;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, want);
+    if (e != cudaSuccess) return int(e);
+    bytes[dev].store(want, std::memory_order_relaxed);   // (of two threads at once the smaller value may stay: it is asked again)
+    return 0;
+  }
+};
+
+}  // namespace jpb

@@ -272,7 +272,12 @@ __global__ void __launch_bounds__(1024) order_place_kernel(const long long* __re
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   for (int e = tid; e < E; e += 1024) total[e] = before[e] = 0;
   __syncthreads();
-  for (int i = tid; i < int(gridDim.x) * E; i += 1024) {
+  if (hist == nullptr) {                                   // one run: counted here
+    for (int i = tid; i < n; i += 1024) {
+      const int e = order_pick(top_i, i, n, E);
+      if (e >= 0) atomicAdd(&total[e], 1);
+    }
+  } else for (int i = tid; i < int(gridDim.x) * E; i += 1024) {
     const int c = hist[i], r = i / E, e = i - r * E;
     if (c == 0) continue;
     atomicAdd(&total[e], c);
@@ -334,7 +339,9 @@ __global__ void __launch_bounds__(1024) order_place_kernel(const long long* __re
   }
   for (int i = placed + int(blockIdx.x) * 1024 + tid; i < n; i += int(gridDim.x) * 1024) inv[i] = -1;
 }
-static int order_run(int n) {   // picks of a CTA: whole steps of 1024, at most 128 CTAs
+// Picks of a CTA: whole steps of 1024, at most 128 CTAs.  Up to 4096 picks one CTA does both steps.
+static int order_run(int n) {
+  if (n <= 4096) return 4096;
   const long long steps = ((long long)n + 1023) / 1024;
   return int((steps + 127) / 128) * 1024;
 }
@@ -500,9 +507,9 @@ JPB_API int jpb_moe_slots(const long long* top_i, long long* dest, int* inv, int
 
 // int32 elements of scratch for jpb_expert_order.
 JPB_API long long jpb_expert_order_scratch_elems(int n, int E) {
-  if (n <= 0) return E;
   const int run = jpb::order_run(n);
-  return ((long long)n + run - 1) / run * E;
+  const long long runs = n > 0 ? ((long long)n + run - 1) / run : 0;
+  return runs > 1 ? runs * E : 0;
 }
 // top_i [n] int64 -> dest [n] int64 (place of each pick, n where it names none of the E experts), inv [n] int32 (pick of each
 // place, or -1), offsets [E + 1] int32.  E <= 256.
@@ -512,8 +519,8 @@ JPB_API int jpb_expert_order(const long long* top_i, long long* dest, int* inv, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (n == 0) return int(cudaMemsetAsync(offsets, 0, sizeof(int) * (E + 1), s));
   const int run = order_run(n), runs = int(((long long)n + run - 1) / run);
-  order_count_kernel<<<runs, 1024, 0, s>>>(top_i, scratch, n, E, run);
-  order_place_kernel<<<runs, 1024, 0, s>>>(top_i, scratch, dest, inv, offsets, n, E, run);
+  if (runs > 1) order_count_kernel<<<runs, 1024, 0, s>>>(top_i, scratch, n, E, run);
+  order_place_kernel<<<runs, 1024, 0, s>>>(top_i, runs > 1 ? scratch : nullptr, dest, inv, offsets, n, E, run);
   return int(cudaGetLastError());
 }
 

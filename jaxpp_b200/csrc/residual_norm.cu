@@ -10,6 +10,7 @@
 // its gradients are those of the forward's function and not of the rounded stream.
 //
 // What bounds it: HBM, four rows moved per row forward (x, y, r, h) and six backward (dr, dh, x, y, dx, dy).
+#include "launch.cuh"
 #include "vec.cuh"
 
 #include <initializer_list>
@@ -519,12 +520,6 @@ __global__ void __launch_bounds__(256) residual_norm_sums_kernel(const float* sc
   }
 }
 
-static int rn_sms() {
-  int dev = 0, n = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n;
-}
 // Threads of a CTA, 16-byte pieces of a row per thread, CTAs per SM, stages of the ring and bytes of shared memory.
 struct RnShape {
   int threads, vecs, per_sm, stages, smem;
@@ -547,7 +542,7 @@ struct RnPlan {
 };
 // CTAs of the backward, and the parts that a group's rows are cut into: one CTA each, or whole groups to a CTA.
 static RnPlan rn_bwd_plan(long long rows, int groups, int per_sm) {
-  const long long want = (long long)rn_sms() * per_sm, group_rows = rows / groups;
+  const long long want = (long long)sm_count_of_device() * per_sm, group_rows = rows / groups;
   long long chunks = want / groups;
   if (chunks > group_rows) chunks = group_rows;
   if (chunks < 1) chunks = 1;
@@ -558,12 +553,11 @@ static RnPlan rn_bwd_plan(long long rows, int groups, int per_sm) {
 static int rn_stream_gate(const void* gate, long long rows, int groups) { return gate && groups > 1 && rows / groups < 16; }
 // (as many operands as the backward can have: the plan must not depend on which are absent, since the scratch goes by it)
 static int rn_bwd_operands(long long rows, int groups) { return 4 + (groups > 1 && rows / groups < 16); }
-template <typename Kernel>
-static int rn_launch(Kernel kernel, int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t stream) {
-  if (shape.smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shape.smem);
-    if (e != cudaSuccess) return int(e);
-  }
+template <typename T, int VECS, bool BWD>
+static int rn_launch(int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t stream) {
+  static SmemLimit limit;
+  auto kernel = BWD ? residual_norm_bwd_kernel<T, VECS> : residual_norm_fwd_kernel<T, VECS>;
+  if (const int rc = limit.allow(kernel, shape.smem)) return rc;
   kernel<<<grid, shape.threads, shape.smem, stream>>>(p);
   return int(cudaGetLastError());
 }
@@ -601,11 +595,11 @@ JPB_API int jpb_residual_norm_fwd(int dt, const void* x, const void* y, const vo
     p.stream_gate = rn_stream_gate(gate, rows, groups);
     const RnShape shape = rn_shape(d, sizeof(T), 2 + p.stream_gate);
     p.stages = shape.stages;
-    const long long most = (long long)rn_sms() * shape.per_sm;
+    const long long most = (long long)sm_count_of_device() * shape.per_sm;
     const int grid = int(rows < most ? rows : most);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return shape.vecs == 2 ? rn_launch(residual_norm_fwd_kernel<T, 2>, grid, shape, p, s)
-                           : rn_launch(residual_norm_fwd_kernel<T, 4>, grid, shape, p, s);
+    return shape.vecs == 2 ? rn_launch<T, 2, false>(grid, shape, p, s)
+                           : rn_launch<T, 4, false>(grid, shape, p, s);
   });
 }
 
@@ -638,8 +632,8 @@ JPB_API int jpb_residual_norm_bwd(int dt, const void* dr, const void* dh, const 
     p.groups = groups; p.chunks = plan.chunks; p.dgate = dgate; p.wide = wide; p.scale = scale;
     p.stages = shape.stages; p.stream_gate = rn_stream_gate(gate, rows, groups); p.status = jpb_status_device_ptr();
     if (rows == 0 && gate) cudaMemsetAsync(dgate, 0, size_t(groups) * d * (wide ? 4 : sizeof(T)), s);
-    const int rc = shape.vecs == 2 ? rn_launch(residual_norm_bwd_kernel<T, 2>, plan.grid, shape, p, s)
-                                   : rn_launch(residual_norm_bwd_kernel<T, 4>, plan.grid, shape, p, s);
+    const int rc = shape.vecs == 2 ? rn_launch<T, 2, true>(plan.grid, shape, p, s)
+                                   : rn_launch<T, 4, true>(plan.grid, shape, p, s);
     if (rc) return rc;
     const bool gate_sums = gate && plan.chunks > 1;
     if (w_post || w_pre || gate_sums)

@@ -20,6 +20,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad as _forward_ad
 
 from ..utils import config
 
@@ -77,6 +78,29 @@ def _define(schema: str, ref_impl, fake_impl, native_name: str | None = None, ch
         torch.library.register_fake(qual, fake)
     DIRECT[getattr(torch.ops.b200, name).default] = impl
     return getattr(torch.ops.b200, name)
+
+
+class _Direct:
+    """An op whose eager calls go straight to its implementation where there is nothing for the dispatcher to do: plain tensors,
+    no gradient to record, no trace or transform under way.  The dispatcher's way to an op implemented in Python takes 15 us and
+    more, as long as many of these kernels run; everything else goes through it."""
+
+    def __init__(self, packet):
+        self.packet, self.default = packet, packet.default
+        self._impl = DIRECT[packet.default]
+        self.__name__ = str(packet)
+
+    def __call__(self, *args, **kwargs):
+        if kwargs or _dispatch_modes() or _functorch_stack() is not None or _forward_ad._current_level >= 0:
+            return self.packet(*args, **kwargs)
+        grad = torch.is_grad_enabled()
+        for a in args:
+            if isinstance(a, Tensor) and ((type(a) is not Tensor and type(a) is not torch.nn.Parameter) or (grad and a.requires_grad)):
+                return self.packet(*args)
+        return self._impl(*args)
+
+
+_dispatch_modes, _functorch_stack = torch._C._len_torch_dispatch_stack, torch._C._functorch.peek_interpreter_stack
 
 
 def _autograd(name: str, backward, setup_context):
@@ -277,24 +301,24 @@ def _linear_ragged_wgrad_ref(dy, x, offsets, out_dtype=None):
     return torch.stack(parts).to(_wg_dtype(dy, out_dtype))
 
 
-linear_ragged = _define(
+linear_ragged = _Direct(_define(
     "linear_ragged(Tensor x, Tensor w, Tensor offsets) -> Tensor",
     _linear_ragged_ref,
     lambda x, w, offsets: x.new_empty(x.shape[0], w.shape[1]),
     "linear_ragged", lambda x, w, offsets: _check_ragged(x, w, offsets, 2, "linear_ragged"),
-)
-linear_ragged_dgrad = _define(
+))
+linear_ragged_dgrad = _Direct(_define(
     "linear_ragged_dgrad(Tensor dy, Tensor w, Tensor offsets) -> Tensor",
     _linear_ragged_dgrad_ref,
     lambda dy, w, offsets: dy.new_empty(dy.shape[0], w.shape[2]),
     "linear_ragged_dgrad", lambda dy, w, offsets: _check_ragged(dy, w, offsets, 1, "linear_ragged_dgrad"),
-)
-linear_ragged_wgrad = _define(
+))
+linear_ragged_wgrad = _Direct(_define(
     "linear_ragged_wgrad(Tensor dy, Tensor x, Tensor offsets, ScalarType? out_dtype=None) -> Tensor",
     _linear_ragged_wgrad_ref,
     lambda dy, x, offsets, out_dtype=None: dy.new_empty(offsets.shape[0] - 1, dy.shape[1], x.shape[1], dtype=_wg_dtype(dy, out_dtype)),
     "linear_ragged_wgrad", _check_ragged_wgrad,
-)
+))
 
 
 def _linear_ragged_setup(ctx, inputs, output):
@@ -457,13 +481,14 @@ _autograd("layernorm", _layernorm_autograd, _layernorm_setup)
 # ======================================================================================
 
 def _check_residual_norm(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
-    d = x.shape[-1] if x.dim() else 0
-    if x.shape != y.shape or x.dtype != y.dtype or x.dim() < 1:
+    shape, dtype = x.shape, x.dtype
+    d = shape[-1] if shape else 0
+    if shape != y.shape or dtype != y.dtype or not shape:
         raise ValueError(f"residual_norm: x {tuple(x.shape)} {x.dtype} and y {tuple(y.shape)} {y.dtype} have to be alike")
     for name, w in (("w_post", w_post), ("w_pre", w_pre)):
-        if w is not None and (tuple(w.shape) != (d,) or w.dtype != x.dtype):
+        if w is not None and (w.shape != (d,) or w.dtype != dtype):
             raise ValueError(f"residual_norm: {name} is [{d}] {x.dtype}, got {tuple(w.shape)} {w.dtype}")
-    if gate is not None:
+    if gate is not None and (gate.shape != (d,) or gate.dtype != dtype):
         rows = x.numel() // d if d else 0
         if (gate.dim() not in (1, 2) or gate.shape[-1] != d or gate.dtype != x.dtype
                 or (gate.dim() == 2 and (gate.shape[0] == 0 or rows % gate.shape[0]))):
@@ -500,11 +525,11 @@ def _residual_norm_fake(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
     return x.new_empty(x.shape), x.new_empty((0,) if w_pre is None else x.shape), stat(w_post), stat(w_pre)
 
 
-residual_norm = _define(
+residual_norm = _Direct(_define(
     "residual_norm(Tensor x, Tensor y, Tensor? w_post, Tensor? gate, Tensor? w_pre, float scale=1.0, float eps=1e-5)"
     " -> (Tensor, Tensor, Tensor, Tensor)",
     _residual_norm_ref, _residual_norm_fake, "residual_norm", _check_residual_norm,
-)
+))
 
 
 def _check_residual_norm_bwd(dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre, scale=1.0, sum_dtype=None):
@@ -553,11 +578,11 @@ def _residual_norm_bwd_fake(dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_p
 
 
 # dr / dh None: nothing arrives over that output.  ``sum_dtype``: as for ``rmsnorm_bwd``.
-residual_norm_bwd = _define(
+residual_norm_bwd = _Direct(_define(
     "residual_norm_bwd(Tensor? dr, Tensor? dh, Tensor x, Tensor y, Tensor? w_post, Tensor? gate, Tensor? w_pre, Tensor rstd_post,"
     " Tensor rstd_pre, float scale=1.0, ScalarType? sum_dtype=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
     _residual_norm_bwd_ref, _residual_norm_bwd_fake, "residual_norm_bwd", _check_residual_norm_bwd,
-)
+))
 
 
 def _residual_norm_setup(ctx, inputs, output):
@@ -1011,14 +1036,14 @@ def _distill_ref(dloss, logits, ids, top, lse, labels, temperature, alpha):
     return loss, torch.where(w != 0, dz * w, torch.zeros_like(dz)).to(logits.dtype).view(shape)
 
 
-distill_loss = _define(
+distill_loss = _Direct(_define(
     "distill_loss(Tensor logits, Tensor teacher_ids, Tensor teacher_logits, Tensor? teacher_lse, Tensor? labels,"
     " float temperature=1.0, float alpha=1.0) -> Tensor",
     lambda logits, ids, top, lse, labels, temperature=1.0, alpha=1.0: _distill_ref(None, logits, ids, top, lse, labels, temperature, alpha),
     lambda logits, ids, top, lse, labels, temperature=1.0, alpha=1.0: logits.new_empty(logits.shape[:-1], dtype=torch.float32),
     "distill_loss", lambda *args: _check_distill(None, *args),
-)
-distill_loss_grad = _define(
+))
+distill_loss_grad = _Direct(_define(
     "distill_loss_grad(Tensor dloss, Tensor logits, Tensor teacher_ids, Tensor teacher_logits, Tensor? teacher_lse, Tensor? labels,"
     " float temperature=1.0, float alpha=1.0) -> (Tensor, Tensor)",
     lambda dloss, logits, ids, top, lse, labels, temperature=1.0, alpha=1.0: _distill_ref(
@@ -1026,7 +1051,7 @@ distill_loss_grad = _define(
     lambda dloss, logits, ids, top, lse, labels, temperature=1.0, alpha=1.0: (
         logits.new_empty(logits.shape[:-1], dtype=torch.float32), logits.new_empty(logits.shape)),
     "distill_loss_grad", _check_distill,
-)
+))
 
 
 def _distill_setup(ctx, inputs, output):

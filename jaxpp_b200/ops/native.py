@@ -437,11 +437,13 @@ def _gate_groups(gate) -> int:
 
 def residual_norm(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
     _here("residual_norm", x, y, w_post, gate, w_pre)
-    x, y, w_post, gate, w_pre = (_vectors(t) for t in (x, y, w_post, gate, w_pre))
-    stat = lambda w: torch.empty((0,) if w is None else x.shape[:-1], dtype=torch.float32, device=x.device)
-    r, rstd_post, rstd_pre = torch.empty_like(x), stat(w_post), stat(w_pre)
-    h = torch.empty_like(x) if w_pre is not None else torch.empty(0, dtype=x.dtype, device=x.device)
-    d = x.shape[-1]
+    x, y, w_post, gate, w_pre = _vectors(x), _vectors(y), _vectors(w_post), _vectors(gate), _vectors(w_pre)
+    shape, device = x.shape, x.device
+    d, rows = shape[-1], shape[:-1]
+    r = torch.empty_like(x)
+    h = torch.empty_like(x) if w_pre is not None else torch.empty(0, dtype=x.dtype, device=device)
+    rstd_post = torch.empty(0 if w_post is None else rows, dtype=torch.float32, device=device)
+    rstd_pre = torch.empty(0 if w_pre is None else rows, dtype=torch.float32, device=device)
     lib = load()
     if x.numel():
         _check(lib.jpb_residual_norm_fwd(_dt(x), x.data_ptr(), y.data_ptr(), _p(w_post), _p(gate), _p(w_pre), r.data_ptr(), h.data_ptr(),
@@ -632,14 +634,14 @@ def _here(what: str, *tensors) -> None:
     """The kernels are launched on the current stream of the current device: every operand has to be there."""
     current = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != current):
+        if t is not None and t.get_device() != current:
             raise NativeError(f"{what}: a tensor is on {t.device}, the current device is cuda:{current}")
 
 
 def _vectors(t: Optional[torch.Tensor]):
     """``t`` contiguous and on a 16-byte boundary (views may start anywhere)."""
-    if t is None:
-        return None
+    if t is None or (t.is_contiguous() and not (t.data_ptr() & 15)):
+        return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 

@@ -404,14 +404,16 @@ def _expert_order_impl(top_i: Tensor, n_experts: int):
     if not ops._use_native(top_i):
         return _expert_order_ref(top_i, n_experts)
     lib, native = _native()
+    native._here("expert_order", top_i)
     flat = top_i.contiguous()
     n = flat.numel()
     dest = torch.empty(n, dtype=torch.int64, device=flat.device)
     inv = torch.empty(n, dtype=torch.int32, device=flat.device)
     offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=flat.device)
-    scratch = torch.empty(lib.jpb_expert_order_scratch_elems(n, n_experts), dtype=torch.int32, device=flat.device)
-    native._check(lib.jpb_expert_order(flat.data_ptr(), dest.data_ptr(), inv.data_ptr(), offsets.data_ptr(), scratch.data_ptr(), n,
-                                       n_experts, native._stream()), "jpb_expert_order", 2)
+    elems = lib.jpb_expert_order_scratch_elems(n, n_experts)
+    scratch = torch.empty(elems, dtype=torch.int32, device=flat.device) if elems else None
+    native._check(lib.jpb_expert_order(flat.data_ptr(), dest.data_ptr(), inv.data_ptr(), offsets.data_ptr(), native._p(scratch), n,
+                                       n_experts, native._stream()), "jpb_expert_order", 2 if elems else 1)
     return dest, inv, offsets
 
 
@@ -432,7 +434,7 @@ def expert_order(top_i: Tensor, n_experts: int):
     ``dest`` [picks] int64 says where each pick goes, ``inv`` [picks] int32 which pick a place holds, and expert ``e`` has
     places ``offsets[e]`` to ``offsets[e + 1]`` (``offsets`` [n_experts + 1] int32).  No capacity: no pick is dropped.  A pick
     that names no expert has ``dest`` = picks, and the places left over at the end hold none (``inv`` -1)."""
-    return torch.ops.b200moe.expert_order(top_i, n_experts)
+    return _expert_order(top_i, n_experts)
 
 
 # ---- the same three steps as kernels, where the experts are on this device -------------------------------------------
@@ -611,3 +613,4 @@ def _register_direct_calls():
 
 
 _register_direct_calls()
+_expert_order = ops._Direct(torch.ops.b200moe.expert_order)

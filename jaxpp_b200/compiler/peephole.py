@@ -70,10 +70,16 @@ def widen_parameter_sums(graph: fx.Graph, keep=()) -> int:
 
     b = torch.ops.b200
     n_args = {b.colsum.default: 1, b.rmsnorm_bwd.default: 4, b.rmsnorm_bwd_add.default: 5, b.layernorm_bwd.default: 5,
-              b.layernorm_bwd_add.default: 6}
+              b.layernorm_bwd_add.default: 6, b.residual_norm_bwd.default: 10}
+    first_sum = {b.residual_norm_bwd.default: 2}     # the results in front of it are gradients of activations
     count = 0
     for n in list(graph.nodes):
-        if n.op != "call_function" or n.target not in n_args or len(n.args) != n_args[n.target] or n.kwargs:
+        if n.op != "call_function" or n.target not in n_args or n.kwargs:
+            continue
+        args = n.args
+        if n.target is b.residual_norm_bwd.default and len(args) == 9:
+            args = (*args, 1.0)     # a residual scale of one, the op's default, is not recorded
+        if len(args) != n_args[n.target]:
             continue
         if n.target is b.colsum.default:
             sums = [n]
@@ -81,19 +87,20 @@ def widen_parameter_sums(graph: fx.Graph, keep=()) -> int:
             items = [u for u in n.users if u.op == "call_function" and u.target is operator.getitem]
             if len(items) != len(n.users):
                 continue
-            sums = [u for u in items if u.args[1] >= 1]
+            # (a gate or norm that a residual connection does without has a sum that nobody takes)
+            sums = [u for u in items if u.args[1] >= first_sum.get(n.target, 1) and (u.users or n.target not in first_sum)]
         if not sums or any(_val(s) is None or _val(s).dtype != torch.bfloat16 or not s.users or not all(_casts_to_fp32(u) and u not in keep for u in s.users)
                            for s in sums) or n in keep or any(s in keep for s in sums):
             continue      # someone wants a sum in its own type
         with graph.inserting_before(n):
-            new = graph.call_function(n.target, (*n.args, torch.float32))
+            new = graph.call_function(n.target, (*args, torch.float32))
         new.meta = dict(n.meta)
         wide = lambda v: v.to(torch.float32)
         if n.target is b.colsum.default:
             new.meta["val"] = wide(_val(n))
             sums = [new]
         elif isinstance(_val(n), (tuple, list)):
-            new.meta["val"] = type(_val(n))([v if i == 0 else wide(v) for i, v in enumerate(_val(n))])
+            new.meta["val"] = type(_val(n))([v if i < first_sum.get(n.target, 1) else wide(v) for i, v in enumerate(_val(n))])
         n.replace_all_uses_with(new)
         graph.erase_node(n)
         for s in sums:

@@ -40,6 +40,10 @@ class Hyper:
     shard_optimizer: bool = False
     # clip the gradient to this global L2 norm (over every pipeline stage, tensor- / expert-parallel shard); None = off
     clip_grad_norm: float | None = None
+    # train against a teacher's top logits (``ops.distill_loss``): weight of the softened term (the rest is the labels' cross
+    # entropy), temperature.  The step then takes the teacher's tensors too (see ``make_train_step``); None = labels alone
+    distill_alpha: float | None = None
+    distill_temperature: float = 1.0
 
 
 def stage_of_layer(cfg: tf.ModelConfig, layer: int) -> int:
@@ -115,7 +119,8 @@ def make_train_step(cfg: tf.ModelConfig, schedule, hyper: Hyper = Hyper(), dp_ax
                     dp: int = 1) -> Callable:
     """``step(state, tokens, labels) -> (state, losses)`` with ``tokens``/``labels`` of shape
     [n_microbatches, microbatch, seq]; ``losses[i]`` is the mean token loss of microbatch ``i`` over this
-    device's tokens."""
+    device's tokens.  With ``hyper.distill_alpha`` the step is ``step(state, tokens, labels, teacher_ids, teacher_logits)`` or
+    ``step(..., teacher_lse)``: [n_microbatches, microbatch, seq, K] twice and [n_microbatches, microbatch, seq]."""
 
     if cfg.cp > 1:
         # chunks of a sequence over the context axis: parameters are replicas there, so their gradients are summed over
@@ -126,7 +131,10 @@ def make_train_step(cfg: tf.ModelConfig, schedule, hyper: Hyper = Hyper(), dp_ax
             raise NotImplementedError("context parallelism together with data parallelism needs a mesh axis of its own")
         dp_axis, dp = cfg.cp_axis, cfg.cp
 
-    def step(state, tokens, labels):
+    def step(state, tokens, labels, *teacher):
+        if (hyper.distill_alpha is None) != (not teacher) or len(teacher) not in (0, 2, 3):
+            raise ValueError("a step with hyper.distill_alpha takes teacher_ids and teacher_logits (and teacher_lse) behind the labels, "
+                             "one without takes none")
         params = state["params"]
         n_mb, mb, seq = tokens.shape
         tokens_per_mb_local = mb * seq // cfg.tp
@@ -134,9 +142,11 @@ def make_train_step(cfg: tf.ModelConfig, schedule, hyper: Hyper = Hyper(), dp_ax
         rope = tf.rope_tables(cfg, tokens.device) if cfg.family in ("llama", "mixtral") else None
 
         def body(batch):
-            tok, lab = batch
+            tok, lab, *top = batch
 
             def loss_fn(p):
+                if top:
+                    return tf.lm_loss(cfg, p, tok, lab, rope, top, hyper.distill_alpha, hyper.distill_temperature)
                 return tf.lm_loss(cfg, p, tok, lab, rope)
 
             prev = ops.WGRAD_DTYPE[0]
@@ -147,7 +157,7 @@ def make_train_step(cfg: tf.ModelConfig, schedule, hyper: Hyper = Hyper(), dp_ax
                 ops.WGRAD_DTYPE[0] = prev
             return loss / tokens_per_mb_local, grads
 
-        losses, grads = jp.treduce(body, (tokens, labels), schedule=schedule)
+        losses, grads = jp.treduce(body, (tokens, labels, *teacher), schedule=schedule)
         grads = tf.sync_replicated_grads(cfg, grads)
         sharded_update = hyper.shard_optimizer and dp_axis is not None and dp > 1
         if dp_axis is not None and dp > 1 and not sharded_update:

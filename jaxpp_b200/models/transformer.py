@@ -29,7 +29,7 @@ from ..pipelining import mark_stage_end
 
 
 # parameters of a block that its attention half uses; the others belong to the feed-forward half
-ATTN_HALF_KEYS = frozenset({"attn_norm", "wqkv", "wo", "b_qkv", "b_o", "ln1_w", "ln1_b"})
+ATTN_HALF_KEYS = frozenset({"attn_norm", "wqkv", "wo", "b_qkv", "b_o", "ln1_w", "ln1_b", "attn_post_norm", "attn_gate"})
 
 
 @dataclasses.dataclass(frozen=True)
@@ -74,8 +74,23 @@ class ModelConfig:
     # the rank that holds the last stage busier than the rest; ``balanced_stage_layers`` picks sizes that even out
     # the pipeline ranks' total work.
     stage_layers: tuple | None = None
+    # mixture of experts without a capacity: every token reaches all its experts, whose products take groups of any length
+    # (``moe.moe_ffn_dropless``; experts on this device)
+    dropless: bool = False
+    # RMSNorm families: the output of each half of a block is normalised too, before it joins the residual stream:
+    #   x <- residual_scale * x + gate * RMSNorm(half(RMSNorm(x)))
+    # ``residual_gate`` is the initial value of learned gates, one per channel and half (None: no gates)
+    sandwich_norm: bool = False
+    residual_scale: float = 1.0
+    residual_gate: float | None = None
 
     def __post_init__(self):
+        if self.dropless and (self.family != "mixtral" or self.ep > 1):
+            raise ValueError("dropless experts are those of the mixtral family with all experts on this device (ep = 1)")
+        if (self.sandwich_norm or self.residual_scale != 1.0 or self.residual_gate is not None) and self.family not in ("llama", "mixtral"):
+            raise ValueError("sandwich norms, residual scale and gates belong to the RMSNorm families (llama, mixtral)")
+        if not self.sandwich_norm and (self.residual_scale != 1.0 or self.residual_gate is not None):
+            raise ValueError("residual_scale and residual_gate go with sandwich_norm")
         if self.stage_layers is not None:
             sl = tuple(float(n) for n in self.stage_layers)
             if (len(sl) != self.n_stages or abs(sum(sl) - self.n_layers) > 1e-9 or min(sl) < 0.5
@@ -303,6 +318,10 @@ def init_layer(cfg: ModelConfig, layer: int, device="cpu", seed: int = 0, tp_ran
         p["b_qkv"] = zeros(qkv_rows)
         p["b_o"], p["b_down"] = zeros(), zeros()
         p["ln1_w"], p["ln1_b"], p["ln2_w"], p["ln2_b"] = ones(), zeros(), ones(), zeros()
+    if cfg.sandwich_norm:
+        p["attn_post_norm"], p["ffn_post_norm"] = ones(), ones()
+        if cfg.residual_gate is not None:
+            p["attn_gate"], p["ffn_gate"] = ones() * cfg.residual_gate, ones() * cfg.residual_gate
     return p
 
 
@@ -364,35 +383,65 @@ def _attention(cfg: ModelConfig, qkv: torch.Tensor, batch: int, rope) -> torch.T
 
 # Every block is two halves with the residual stream as their only link, so that a pipeline stage boundary can fall
 # between them: ``<family>_attn(cfg, p, x, batch, rope) -> x`` and ``<family>_ffn(cfg, p, x) -> x`` (mixtral: (x, aux)).
+def _llama_attn_out(cfg: ModelConfig, p: dict, h: torch.Tensor, batch: int, rope) -> torch.Tensor:
+    a = _attention(cfg, tpops.column_linear(h, p["wqkv"], None, cfg), batch, rope)
+    return tpops.row_linear(a, p["wo"], None, cfg)
+
+
+def _llama_ffn_out(cfg: ModelConfig, p: dict, h: torch.Tensor) -> torch.Tensor:
+    return tpops.row_linear(ops.swiglu(tpops.column_linear(h, p["w_up"], None, cfg)), p["w_down"], None, cfg)
+
+
+def _mixtral_ffn_out(cfg: ModelConfig, p: dict, h: torch.Tensor):
+    from ..parallel import moe
+
+    experts = {"router": p["router"], "w_up": p["e_up"], "w_down": p["e_down"]}
+    if cfg.dropless:
+        return moe.moe_ffn_dropless(h, experts, cfg.n_experts, cfg.top_k)
+    return moe.moe_ffn(h, experts, cfg.n_experts, cfg.top_k, cfg.capacity_factor, cfg.ep, cfg.ep_axis)
+
+
+def _join(cfg: ModelConfig, p: dict, half: str, x: torch.Tensor, y: torch.Tensor, w_pre=None):
+    """The residual connection behind one half of a block (``half``: "attn" or "ffn"); with ``w_pre`` also the norm in front of
+    the next half, in the same pass: returns (x, h)."""
+    x, h, _, _ = ops.residual_norm(x, y, p[f"{half}_post_norm"], p.get(f"{half}_gate"), w_pre, cfg.residual_scale, cfg.eps)
+    return (x, h) if w_pre is not None else x
+
+
 def llama_attn(cfg: ModelConfig, p: dict, x: torch.Tensor, batch: int, rope) -> torch.Tensor:
     h = ops.rmsnorm(x, p["attn_norm"], cfg.eps)[0]
-    qkv = tpops.column_linear(h, p["wqkv"], None, cfg)
-    a = _attention(cfg, qkv, batch, rope)
-    return x + tpops.row_linear(a, p["wo"], None, cfg)
+    y = _llama_attn_out(cfg, p, h, batch, rope)
+    return _join(cfg, p, "attn", x, y) if cfg.sandwich_norm else x + y
 
 
 def llama_ffn(cfg: ModelConfig, p: dict, x: torch.Tensor) -> torch.Tensor:
     h = ops.rmsnorm(x, p["ffn_norm"], cfg.eps)[0]
-    gu = tpops.column_linear(h, p["w_up"], None, cfg)
-    return x + tpops.row_linear(ops.swiglu(gu), p["w_down"], None, cfg)
+    y = _llama_ffn_out(cfg, p, h)
+    return _join(cfg, p, "ffn", x, y) if cfg.sandwich_norm else x + y
 
 
 def llama_block(cfg: ModelConfig, p: dict, x: torch.Tensor, batch: int, rope) -> torch.Tensor:
-    return llama_ffn(cfg, p, llama_attn(cfg, p, x, batch, rope))
+    if not cfg.sandwich_norm:
+        return llama_ffn(cfg, p, llama_attn(cfg, p, x, batch, rope))
+    y = _llama_attn_out(cfg, p, ops.rmsnorm(x, p["attn_norm"], cfg.eps)[0], batch, rope)
+    x, h = _join(cfg, p, "attn", x, y, p["ffn_norm"])
+    return _join(cfg, p, "ffn", x, _llama_ffn_out(cfg, p, h))
 
 
 def mixtral_ffn(cfg: ModelConfig, p: dict, x: torch.Tensor):
-    from ..parallel import moe
-
     h = ops.rmsnorm(x, p["ffn_norm"], cfg.eps)[0]
-    y, aux = moe.moe_ffn(h, {"router": p["router"], "w_up": p["e_up"], "w_down": p["e_down"]}, cfg.n_experts, cfg.top_k,
-                         cfg.capacity_factor, cfg.ep, cfg.ep_axis)
-    return x + y, aux
+    y, aux = _mixtral_ffn_out(cfg, p, h)
+    return (_join(cfg, p, "ffn", x, y) if cfg.sandwich_norm else x + y), aux
 
 
 def mixtral_block(cfg: ModelConfig, p: dict, x: torch.Tensor, batch: int, rope):
     """Llama attention + top-k mixture-of-experts SwiGLU FFN; returns (x, load-balancing loss of this block)."""
-    return mixtral_ffn(cfg, p, llama_attn(cfg, p, x, batch, rope))
+    if not cfg.sandwich_norm:
+        return mixtral_ffn(cfg, p, llama_attn(cfg, p, x, batch, rope))
+    y = _llama_attn_out(cfg, p, ops.rmsnorm(x, p["attn_norm"], cfg.eps)[0], batch, rope)
+    x, h = _join(cfg, p, "attn", x, y, p["ffn_norm"])
+    y, aux = _mixtral_ffn_out(cfg, p, h)
+    return _join(cfg, p, "ffn", x, y), aux
 
 
 def gpt2_attn(cfg: ModelConfig, p: dict, x: torch.Tensor, batch: int, rope) -> torch.Tensor:
@@ -532,17 +581,27 @@ def encoder_forward(cfg: ModelConfig, params: dict, hidden: torch.Tensor) -> tor
     return mark_stage_end(x).view_as(hidden)
 
 
-def lm_loss(cfg: ModelConfig, params: dict, tokens: torch.Tensor, labels: torch.Tensor, rope=None) -> torch.Tensor:
+def lm_loss(cfg: ModelConfig, params: dict, tokens: torch.Tensor, labels: torch.Tensor, rope=None, teacher=None,
+            distill_alpha: float = 1.0, distill_temperature: float = 1.0) -> torch.Tensor:
     """Sum over this device's tokens of the next-token cross entropy.  ``tokens``/``labels`` are
     [batch, seq] int64; with tensor parallelism each device embeds and scores its own slice of the tokens
-    (sequence parallel), so the returned value is a partial sum."""
+    (sequence parallel), so the returned value is a partial sum.
+
+    ``teacher`` (ids, logits[, log-sum-exp]), [batch, seq, K] twice and [batch, seq] float32: the loss is that of
+    ``ops.distill_loss`` with the given ``alpha`` and temperature instead."""
     b = tokens.shape[0]
     tp = cfg.tp
     if cfg.cp > 1 and cfg.family == "gpt2":
         raise NotImplementedError("context parallelism needs rotary positions (learned absolute positions are not split)")
     flat_tok, flat_lab = tokens.reshape(-1), labels.reshape(-1)
+    if teacher is not None:
+        if cfg.vocab_parallel and tp > 1:
+            raise NotImplementedError("distillation needs whole rows of logits (no vocabulary-parallel output projection)")
+        teacher = [t.reshape(-1) if i == 2 else t.reshape(-1, t.shape[-1]) for i, t in enumerate(teacher)]
     if tp > 1:
         flat_tok, flat_lab = tpops.local_token_slice(flat_tok, cfg), tpops.local_token_slice(flat_lab, cfg)
+        if teacher is not None:
+            teacher = [tpops.local_token_slice(t, cfg) for t in teacher]
     x = ops.embedding(flat_tok, params["embed"])
     if cfg.family == "gpt2":
         pos = params["pos"]
@@ -568,7 +627,11 @@ def lm_loss(cfg: ModelConfig, params: dict, tokens: torch.Tensor, labels: torch.
         loss = tpops.local_token_slice(every, cfg)
     else:
         logits = ops.linear(x, head, None)
-        loss, _ = ops.cross_entropy(logits, flat_lab)
+        if teacher is not None:
+            ids, top, *lse = teacher
+            loss = ops.distill_loss(logits, ids, top, lse[0] if lse else None, flat_lab, distill_temperature, distill_alpha)
+        else:
+            loss, _ = ops.cross_entropy(logits, flat_lab)
     total = loss.sum()
     if aux is not None:  # the load-balancing term is per token: scale it like the summed cross entropy
         total = total + cfg.aux_coef * aux * flat_lab.shape[0]
@@ -579,7 +642,8 @@ def sync_replicated_grads(cfg: ModelConfig, grads: dict) -> dict:
     """Sum over the tensor-parallel axis the gradients of parameters that are replicated across it."""
     if cfg.tp == 1:
         return grads
-    rep_layer = {"attn_norm", "ffn_norm", "ln1_w", "ln1_b", "ln2_w", "ln2_b", "b_o", "b_down", "router"}
+    rep_layer = {"attn_norm", "ffn_norm", "ln1_w", "ln1_b", "ln2_w", "ln2_b", "b_o", "b_down", "router", "attn_post_norm",
+                 "ffn_post_norm", "attn_gate", "ffn_gate"}
     out = dict(grads)
     out["layers"] = {
         name: {k: (tpops.all_reduce(g, cfg.tp_axis) if k in rep_layer else g) for k, g in layer.items()}

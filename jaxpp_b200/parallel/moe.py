@@ -1,7 +1,8 @@
 """Mixture-of-experts building blocks with expert parallelism (Mixtral-style top-k routing).
 
 The reference has no MoE support (only an ``"expert"`` axis name in a mesh test, tests/test_mpmd_mesh.py:71).
-Routing here is capacity based so that every shape in the captured step is static:
+Routing is capacity based, so that every expert has the same number of slots (``moe_ffn_dropless`` is the form without a
+capacity, for experts on one device; its shapes are static too, since the groups' sizes stay on the device):
 
     probs   = softmax(x W_r^T)                       [T, E]
     top-k   → expert ids, weights renormalised over the k picks; aux = E * Σ_e f_e · P_e (load balancing)
@@ -593,6 +594,22 @@ def moe_ffn(x: Tensor, p: dict, n_experts: int, top_k: int, capacity_factor: flo
     y = expert_ffn(buf, p["w_up"], p["w_down"], counts, capacity)
     out, _ = torch.ops.b200moe.combine_a2a(y, dest, weights.reshape(-1), n_experts, capacity, top_k, ep_axis, True)
     return out, aux
+
+
+def expert_ffn_ragged(rows: Tensor, w_up: Tensor, w_down: Tensor, offsets: Tensor) -> Tensor:
+    """:func:`expert_ffn` on rows sorted by expert (``expert_order``): rows [picks, d], expert ``e`` has ``offsets[e]`` to
+    ``offsets[e + 1]`` of them."""
+    return ops.linear_ragged(ops.swiglu(ops.linear_ragged(rows, w_up, offsets)), w_down, offsets)
+
+
+def moe_ffn_dropless(x: Tensor, p: dict, n_experts: int, top_k: int):
+    """:func:`moe_ffn` without a capacity, experts on this device: the picks are sorted by expert and every expert's products take
+    as many rows as it was picked for, so that no pick is dropped and no slot is empty.  Returns (y [T, d], aux loss)."""
+    top_i, weights, aux = route(x, p["router"], top_k)
+    dest, inv, offsets = expert_order(top_i, n_experts)
+    rows = torch.ops.b200moe.dispatch_rows(x, dest, inv, top_k)
+    y = expert_ffn_ragged(rows, p["w_up"], p["w_down"], offsets)
+    return torch.ops.b200moe.combine_rows(y, dest, inv, weights.reshape(-1), top_k), aux
 
 
 def _register_direct_calls():

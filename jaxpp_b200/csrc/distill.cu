@@ -557,7 +557,7 @@ static int distill_go(const DistillParams& p, const DistillShape& shape, int sms
   cfg.attrs = attr;
   cfg.numAttrs = shape.cluster > 1 ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
-  return e != cudaSuccess ? int(e) : int(cudaGetLastError());
+  return launch_result(e);
 }
 template <typename T, bool GRAD, int MODE>
 static int distill_threads(const DistillParams& p, const DistillShape& s, int sms, cudaStream_t stream) {

@@ -675,7 +675,7 @@ static int launch(SmemLimit& limit, Kernel kernel, int cg, int smem, int threads
   cfg.attrs = attr;
   cfg.numAttrs = cg > 1 ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  return e != cudaSuccess ? int(e) : int(cudaGetLastError());
+  return launch_result(e);
 }
 
 template <int CG, int BT>

@@ -15,6 +15,11 @@ inline int current_device() {
   cudaGetDevice(&dev);
   return dev >= 0 && dev < MAX_DEVICES ? dev : 0;
 }
+// The code of a launch, and no error left behind for the next question about one: the caller raises it.
+inline int launch_result(cudaError_t e) {
+  const cudaError_t last = cudaGetLastError();
+  return int(e != cudaSuccess ? e : last);
+}
 inline int sm_count_of_device() {
   static std::atomic<int> sms[MAX_DEVICES];
   const int dev = current_device();
@@ -25,15 +30,16 @@ inline int sm_count_of_device() {
   }
   return n;
 }
-// The largest dynamic shared memory that a kernel was allowed so far (one object per kernel).
+// The largest dynamic shared memory that a kernel was allowed so far (one object per kernel).  Without asking, a CTA has 48 KB of
+// both kinds together: 32 KB leave room for any kernel's static part.
 struct SmemLimit {
   std::atomic<int> bytes[MAX_DEVICES];
   template <typename Kernel>
   int allow(Kernel kernel, int want) {
     const int dev = current_device();
-    if (want <= 48 * 1024 || want <= bytes[dev].load(std::memory_order_relaxed)) return 0;
+    if (want <= 32 * 1024 || want <= bytes[dev].load(std::memory_order_relaxed)) return 0;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, want);
-    if (e != cudaSuccess) return int(e);
+    if (e != cudaSuccess) return launch_result(e);
     bytes[dev].store(want, std::memory_order_relaxed);   // (of two threads at once the smaller value may stay: it is asked again)
     return 0;
   }

@@ -75,7 +75,7 @@ def norm_exact(x, y, w_post, gate, w_pre, scale, eps):
 NORMS = [  # rows, d, gate rows (0: one vector; None: no gate), post, pre
     (1, 8, 0, True, True), (5, 8, None, True, True), (3, 264, 0, True, False), (4, 1024, None, False, True), (6, 40, 2, True, True),
     (7, 4096, 7, True, True), (130, 1600, 0, True, True), (64, 512, 4, False, True), (2, 8192, 0, True, True),
-    (9, 136, 3, True, False), (0, 64, 0, True, True), (300, 128, 0, False, False), (40, 16384, 2, True, True),
+    (9, 136, 3, True, False), (40, 2000, 0, True, True), (0, 64, 0, True, True), (300, 128, 0, False, False), (40, 16384, 2, True, True),
 ]
 
 
@@ -301,6 +301,7 @@ DISTILLS = [  # rows, V, K, tail, labels, temperature, alpha
     (3, 257, 64, False, True, 4.0, 0.5), (3, 1000, 16, True, True, 1.5, 0.9), (2, 4097, 100, True, False, 2.0, 1.0),
     (2, 32000, 64, True, True, 2.0, 0.5), (2, 50257, 100, False, False, 1.0, 1.0), (2, 333, 400, True, True, 1.0, 0.0),
     (0, 64, 4, True, True, 1.0, 0.5), (3, 40, 0, True, True, 1.0, 0.5), (2, 128256, 256, True, True, 0.5, 0.5), (300, 130, 5, True, True, 1.0, 0.5),
+    (300, 24000, 16, True, True, 1.0, 1.0), (300, 12000, 16, True, True, 1.0, 1.0),   # rows that take just under 48 KB
 ]
 
 

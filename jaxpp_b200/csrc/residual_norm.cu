@@ -53,19 +53,24 @@ struct RowRing {
 
   __device__ __forceinline__ uint32_t at_dr() const { return (1 + (x != nullptr) + (dh != nullptr)) * row_bytes; }
   __device__ __forceinline__ uint32_t at_gate() const { return at_dr() + (dr != nullptr) * row_bytes; }
-  __device__ __forceinline__ void one(uint8_t*& dst, const void* src, long long row, int s) const {
-    if (src == nullptr) return;
-    bulk_load(dst, static_cast<const uint8_t*>(src) + size_t(row) * row_bytes, row_bytes, &full[s]);
-    dst += row_bytes;
+  __device__ __forceinline__ int operands() const { return int(stage_bytes / row_bytes); }
+  // The k-th operand's row on its way to stage s (one thread; the barrier counts the operands).  The operands of a stage are
+  // asked for by different warps: asking takes 100 cycles each.
+  __device__ __forceinline__ void ask(int k, int s, long long row) const {
+    const void* src = k == 0 ? y : gate;
+    if (gate == nullptr || k + 1 < operands()) {
+      if (k == 1) src = x ? x : dr;
+      else if (k == 2) src = dh ? dh : dr;
+      else if (k == 3) src = dr;
+    }
+    if (gate != nullptr && k + 1 == operands()) row /= group_rows;
+    mbar_expect_tx(&full[s], row_bytes);
+    bulk_load(ring + size_t(s) * stage_bytes + k * row_bytes, static_cast<const uint8_t*>(src) + size_t(row) * row_bytes, row_bytes, &full[s]);
   }
-  __device__ __forceinline__ void issue(int s, long long row) const {   // one thread
-    mbar_expect_tx(&full[s], stage_bytes);
-    uint8_t* dst = ring + size_t(s) * stage_bytes;
-    one(dst, y, row, s);
-    one(dst, x, row, s);
-    one(dst, dh, row, s);
-    one(dst, dr, row, s);
-    if (gate != nullptr) one(dst, gate, row / group_rows, s);
+  __device__ __forceinline__ void ask_all(int s, long long row) const {   // every thread of the CTA
+    const int nwarps = blockDim.x >> 5, n = operands();
+    for (int k = threadIdx.x >> 5; k < n; k += nwarps)
+      if ((threadIdx.x & 31) == 0) ask(k, s, row);
   }
   // (a time-out is reported and the kernel goes on, over rows that nothing will use)
   __device__ __forceinline__ void wait(int s, uint32_t phase) const { mbar_wait_bounded(&full[s], phase, abort_flag, status); }
@@ -106,12 +111,10 @@ __device__ __forceinline__ float cta_sum(float v, float* scratch, int& slot, int
   for (int o = 1; o < span; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// Four sums at once: lanes trade values so that each ends up with one of the four (6 shuffles instead of 20), and after the
-// barrier the same way (parts as [warp][4]).
-__device__ __forceinline__ void cta_sum4(float (&v)[4], float* scratch, int& slot, int span) {
+// Four sums at once, in two halves with a barrier between them: lanes trade values so that each ends up with one of the four (6
+// shuffles instead of 20), and after the barrier the same way (parts as [warp][4]).
+__device__ __forceinline__ void sum4_begin(const float (&v)[4], float* s) {
   const int lane = threadIdx.x & 31;
-  float* s = scratch + slot * 128;
-  slot ^= 1;
   const bool b0 = lane & 1, b1 = lane & 2;
   float a = b0 ? v[2] : v[0], c = b0 ? v[3] : v[1];
   a += __shfl_xor_sync(0xffffffffu, b0 ? v[0] : v[2], 1);
@@ -122,8 +125,10 @@ __device__ __forceinline__ void cta_sum4(float (&v)[4], float* scratch, int& slo
   for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   // lane & 3 = 0, 1, 2, 3 has the sums of v[0], v[2], v[1], v[3]
   if (lane < 4) s[(threadIdx.x >> 5) * 4 + lane] = x;
-  __syncthreads();
-  x = 0.f;
+}
+__device__ __forceinline__ void sum4_end(float (&v)[4], const float* s, int span) {
+  const int lane = threadIdx.x & 31;
+  float x = 0.f;
   for (int i = lane; i < span * 4; i += 32) x += s[i];
   for (int o = 4; o < 32 && o < span * 4; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   v[0] = __shfl_sync(0xffffffffu, x, 0);
@@ -152,9 +157,8 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
                         p.stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
   if (tid == 0) {
     abort_flag = 0;
-    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], ring.operands());
     fence_barrier_init();
-    for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.issue(s, lo + s);
   }
   Vec<T> w_post[VECS], gate[VECS], w_pre[VECS];
 #pragma unroll
@@ -166,6 +170,8 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     if (p.w_pre) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
   }
   __syncthreads();
+  for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.ask_all(s, lo + s);
+  const uint32_t ring0 = smem_u32(ring.ring) + tid * 16, step = blockDim.x * 16;
   int slot = 0, s = 0;
   uint32_t phase = 0;
   long long gate_end = p.gate && !p.stream_gate ? lo : hi;   // row from which on another row of the gate counts
@@ -180,18 +186,19 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
       }
     }
     ring.wait(s, phase);
-    const uint8_t* stage = ring.ring + size_t(s) * ring.stage_bytes;
-    const T* sy = reinterpret_cast<const T*>(stage);
-    const T* sx = reinterpret_cast<const T*>(stage + row_bytes);
+    const uint32_t sy = ring0 + s * ring.stage_bytes, sx = sy + row_bytes;
     float y[VECS][VN], r[VECS][VN];
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
       if (v >= nvec) continue;
-      load_vec<T>(sy, size_t(v) * VN, y[i]);
-      load_vec<T>(sx, size_t(v) * VN, r[i]);
-      if (p.stream_gate) gate[i].load(reinterpret_cast<const T*>(stage + ring.at_gate()) + size_t(v) * VN);
+      Vec<T> raw;
+      lds_vec(raw, sy + i * step);
+      raw.to_float(y[i]);
+      lds_vec(raw, sx + i * step);
+      raw.to_float(r[i]);
+      if (p.stream_gate) lds_vec(gate[i], sy + ring.at_gate() + i * step);
 #pragma unroll
       for (int j = 0; j < VN; ++j) sum += y[i][j] * y[i][j];
     }
@@ -203,9 +210,10 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
       __syncthreads();
     }
     // the row is in registers by now, of every thread: its stage takes the next one
-    if (tid == 0 && row + p.stages < hi) ring.issue(s, row + p.stages);
+    if (row + p.stages < hi) ring.ask_all(s, row + p.stages);
     sum = 0.f;
-    const size_t base = size_t(row) * p.d;
+    T* const out_r = static_cast<T*>(p.r) + size_t(row) * p.d + size_t(tid) * VN;
+    T* const out_h = static_cast<T*>(p.h) + size_t(row) * p.d + size_t(tid) * VN;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
@@ -218,7 +226,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
         r[i][j] = p.scale * r[i][j] + g[j] * (y[i][j] * rstd1 * w[j]);
         sum += r[i][j] * r[i][j];
       }
-      store_vec<T>(p.r, base + size_t(v) * VN, r[i]);
+      store_vec<T>(out_r, i * step / int(sizeof(T)), r[i]);
     }
     if (p.w_pre) {
       const float rstd2 = rsqrtf(cta_sum(sum, scratch, slot, span) / p.d + p.eps);
@@ -231,7 +239,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
         w_pre[i].to_float(w);
 #pragma unroll
         for (int j = 0; j < VN; ++j) w[j] *= r[i][j] * rstd2;
-        store_vec<T>(p.h, base + size_t(v) * VN, w);
+        store_vec<T>(out_h, i * step / int(sizeof(T)), w);
       }
     }
     if (++s == p.stages) { s = 0; phase ^= 1; }
@@ -245,8 +253,8 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
 
 // Backward.  With c = gate * w_post * y (so that r = scale * x + rstd1 * c) the two means need one round of sums, and one
 // barrier, over the row:
-//   mean1 = mean(u * hat) = rstd2 * sum(u r) / d
-//   mean2 = mean(v * p)   = rstd1 * (sum(c dr) + rstd2 * (sum(c u) - rstd2 * mean1 * sum(c r))) / d
+//   dR = A - k1 * r  with  A = dr + rstd2 * u,  k1 = rstd2^2 * sum(rstd2 * u * r) / d
+//   mean(v * p) = rstd1 * (sum(c A) - k1 * sum(c r)) / d
 // and the sums over the rows of dR * p alone, S, give both dgate = w_post * S and dw_post = gate * S.  A CTA has consecutive
 // rows: a part of one group of rows that share a gate row, or whole groups.  The sums for the gate leave at the end of a group
 // (as the result, where the CTA has all of it), those for the weights when the CTA is done.
@@ -279,9 +287,8 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
                         p.stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
   if (tid == 0) {
     abort_flag = 0;
-    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], ring.operands());
     fence_barrier_init();
-    for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.issue(s, lo + s);
   }
   const F2 zero = f2(0.f);
   Vec<T> w_pre[VECS];
@@ -351,83 +358,92 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     first_group = false;
   };
   __syncthreads();
-  int slot = 0, s = 0;
-  uint32_t phase = 0;
-  long long left = 0;             // rows of the current group that are still to come
+  for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.ask_all(s, lo + s);
+  // A row's sums are finished while the next row's are made: one barrier per row, between the sums of row + 1 and the results of
+  // row + 1, with the results of row in front of it.  (At the end of a group the next row waits for its gate.)
   const float inv_d = 1.f / p.d;
   const F2 scale = f2(p.scale);
-  float next1 = lo < hi && p.w_post ? p.rstd_post[lo] : 1.f, next2 = lo < hi && pre ? p.rstd_pre[lo] : 0.f;
-  for (long long row = lo; row < hi; ++row) {
-    if (p.gate && left == 0) {
-      left = p.group_rows;        // (a part of a group ends with the CTA's rows)
-      if (!p.stream_gate) load_gate(static_cast<const T*>(p.gate) + size_t(group) * p.d);
+  struct Stats {
+    float rstd1, rstd2;
+  };
+  auto stats_of = [&](long long row) {
+    Stats t = {1.f, 0.f};
+    if (row < hi) {
+      if (p.w_post) t.rstd1 = p.rstd_post[row];
+      if (pre) t.rstd2 = p.rstd_pre[row];
     }
-    const float rstd1 = next1, rstd2 = next2;
-    if (row + 1 < hi) {
-      if (p.w_post) next1 = p.rstd_post[row + 1];
-      if (pre) next2 = p.rstd_pre[row + 1];
-    }
-    ring.wait(s, phase);
-    const uint8_t* stage = ring.ring + size_t(s) * ring.stage_bytes;
-    const T* sy = reinterpret_cast<const T*>(stage);
-    const T* sx = reinterpret_cast<const T*>(stage + row_bytes);          // read where there is a gradient of h
-    const T* sdh = reinterpret_cast<const T*>(stage + 2 * row_bytes);
-    const T* sdr = reinterpret_cast<const T*>(stage + ring.at_dr());
-    const T* sgate = p.stream_gate ? reinterpret_cast<const T*>(stage + ring.at_gate()) : nullptr;
-    if (sgate) load_gate(sgate);
-    const F2 r1 = f2(rstd1);
-    float sums[4];
-    {
-      F2 ur = zero, cd = zero, cu = zero, cr = zero;
+    return t;
+  };
+  // shared-memory address of this thread's first piece of operand k in stage s; the next ones are `step` bytes further
+  const uint32_t ring0 = smem_u32(ring.ring) + tid * 16, step = blockDim.x * 16;
+  auto operand = [&](int s, int k) { return ring0 + s * ring.stage_bytes + k * row_bytes; };
+  const int at_dr = pre ? 3 : 1, at_gate = operands - 1;
+  int slot = 0;
+  // this thread's part of sum(u r), sum(c A), sum(c r) with A = dr + rstd2 * u; adds to the sum for w_pre
+  auto row_sums = [&](int s, const Stats& t) {
+    const uint32_t sy = operand(s, 0), sx = operand(s, 1), sdh = operand(s, 2), sdr = operand(s, at_dr);
+    const F2 r1 = f2(t.rstd1), r2 = f2(t.rstd2);
+    F2 ur = zero, ca = zero, cr = zero;
 #pragma unroll
-      for (int i = 0; i < VECS; ++i) {
-        const int v = tid + i * blockDim.x;
-        if (v >= nvec) continue;
-        Vec<T> raw;
-        F2 y[NP], x[NP], u[NP], w[NP], dr[NP];
-        raw.load(sy + size_t(v) * VN);
-        to_pairs(raw, y);
+    for (int i = 0; i < VECS; ++i) {
+      const int v = tid + i * blockDim.x;
+      if (v >= nvec) continue;
+      Vec<T> raw;
+      F2 c[NP], A[NP];
+      lds_vec(raw, sy + i * step);
+      to_pairs(raw, c);
 #pragma unroll
-        for (int j = 0; j < NP; ++j) y[j] = y[j] * gw[i][j];               // c
-        if (p.dr) {
-          raw.load(sdr + size_t(v) * VN);
-          to_pairs(raw, dr);
+      for (int j = 0; j < NP; ++j) c[j] = c[j] * gw[i][j];
+      if (p.dr) {
+        lds_vec(raw, sdr + i * step);
+        to_pairs(raw, A);
+      } else {
 #pragma unroll
-          for (int j = 0; j < NP; ++j) cd = fma2(y[j], dr[j], cd);
-        }
-        if (pre) {
-          raw.load(sx + size_t(v) * VN);
-          to_pairs(raw, x);
-          raw.load(sdh + size_t(v) * VN);
-          to_pairs(raw, u);
-          to_pairs(w_pre[i], w);
+        for (int j = 0; j < NP; ++j) A[j] = zero;
+      }
+      if (pre) {
+        F2 x[NP], u[NP], w[NP];
+        lds_vec(raw, sx + i * step);
+        to_pairs(raw, x);
+        lds_vec(raw, sdh + i * step);
+        to_pairs(raw, u);
+        to_pairs(w_pre[i], w);
 #pragma unroll
-          for (int j = 0; j < NP; ++j) {
-            const F2 uw = u[j] * w[j], r = fma2(r1, y[j], scale * x[j]);
-            ur = fma2(uw, r, ur);
-            cu = fma2(y[j], uw, cu);
-            cr = fma2(y[j], r, cr);
-          }
+        for (int j = 0; j < NP; ++j) {
+          const F2 r = fma2(r1, c[j], scale * x[j]);
+          u[j] = u[j] * r2;
+          a_pre[i][j] = fma2(u[j], r, a_pre[i][j]);
+          u[j] = u[j] * w[j];
+          A[j] = A[j] + u[j];
+          ur = fma2(u[j], r, ur);
+          cr = fma2(c[j], r, cr);
         }
       }
-      sums[0] = ur.lo() + ur.hi(); sums[1] = cd.lo() + cd.hi(); sums[2] = cu.lo() + cu.hi(); sums[3] = cr.lo() + cr.hi();
+#pragma unroll
+      for (int j = 0; j < NP; ++j) ca = fma2(c[j], A[j], ca);
     }
-    cta_sum4(sums, scratch, slot, span);
-    // dR = dr + rstd2 * u - k1 * r,   dy = rstd1 * (gate * w_post * dR) - k2 * y
-    const float k1 = rstd2 * rstd2 * rstd2 * sums[0] * inv_d;
-    const float mean2 = p.w_post ? rstd1 * (sums[1] + (rstd2 * sums[2] - k1 * sums[3])) * inv_d : 0.f;
-    const F2 r2 = f2(rstd2), m1 = f2(-k1), m2 = f2(-mean2 * rstd1 * rstd1);
-    const size_t base = size_t(row) * p.d;
+    float sums[4] = {ur.lo() + ur.hi(), ca.lo() + ca.hi(), cr.lo() + cr.hi(), 0.f};
+    sum4_begin(sums, scratch + slot * 128);
+  };
+  // dx and dy of a row from its sums
+  auto row_results = [&](int s, long long row, const Stats& t, const float (&sums)[4]) {
+    const uint32_t sy = operand(s, 0), sx = operand(s, 1), sdh = operand(s, 2), sdr = operand(s, at_dr);
+    // dR = A - k1 * r = dr + rstd2 * u - k1 * rstd1 * c - k1 * scale * x;   dy = rstd1 * gate * w_post * dR - k2 * y
+    const float k1 = t.rstd2 * t.rstd2 * sums[0] * inv_d;
+    const float k2 = p.w_post ? t.rstd1 * t.rstd1 * t.rstd1 * (sums[1] - k1 * sums[2]) * inv_d : 0.f;
+    const F2 r1 = f2(t.rstd1), r2 = f2(t.rstd2), mc = f2(-k1 * t.rstd1), mx = f2(-k1 * p.scale), my = f2(-k2);
+    T* const dx = static_cast<T*>(p.dx) + size_t(row) * p.d + size_t(tid) * VN;
+    T* const dy = static_cast<T*>(p.dy) + size_t(row) * p.d + size_t(tid) * VN;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
       if (v >= nvec) continue;
       Vec<T> raw;
       F2 y[NP], dR[NP], o[NP];
-      raw.load(sy + size_t(v) * VN);
+      lds_vec(raw, sy + i * step);
       to_pairs(raw, y);
       if (p.dr) {
-        raw.load(sdr + size_t(v) * VN);
+        lds_vec(raw, sdr + i * step);
         to_pairs(raw, dR);
       } else {
 #pragma unroll
@@ -435,37 +451,78 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
       }
       if (pre) {
         F2 x[NP], u[NP], w[NP];
-        raw.load(sx + size_t(v) * VN);
+        lds_vec(raw, sx + i * step);
         to_pairs(raw, x);
-        raw.load(sdh + size_t(v) * VN);
+        lds_vec(raw, sdh + i * step);
         to_pairs(raw, u);
         to_pairs(w_pre[i], w);
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-          const F2 r = fma2(r1, y[j] * gw[i][j], scale * x[j]);
-          a_pre[i][j] = fma2(u[j], r * r2, a_pre[i][j]);
-          dR[j] = fma2(m1, r, fma2(r2, u[j] * w[j], dR[j]));
-        }
+        for (int j = 0; j < NP; ++j)
+          dR[j] = fma2(mx, x[j], fma2(mc, y[j] * gw[i][j], fma2(r2, u[j] * w[j], dR[j])));
       }
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
+        const F2 dRp = dR[j] * r1;
         o[j] = scale * dR[j];
-        const F2 pj = y[j] * r1;
-        S[i][j] = fma2(dR[j], pj, S[i][j]);
-        dR[j] = fma2(m2, y[j], r1 * (dR[j] * gw[i][j]));
+        S[i][j] = fma2(dRp, y[j], S[i][j]);
+        y[j] = fma2(dRp, gw[i][j], my * y[j]);
       }
       from_pairs(raw, o);
-      raw.store(static_cast<T*>(p.dx) + base + size_t(v) * VN);
-      from_pairs(raw, dR);
-      raw.store(static_cast<T*>(p.dy) + base + size_t(v) * VN);
+      raw.store(dx + i * step / int(sizeof(T)));
+      from_pairs(raw, y);
+      raw.store(dy + i * step / int(sizeof(T)));
     }
-    if (p.gate && (--left == 0 || row + 1 == hi)) {
-      flush(sgate ? sgate : static_cast<const T*>(p.gate) + size_t(group) * p.d);
+  };
+  auto gate_of = [&](int s) {
+    return p.stream_gate ? reinterpret_cast<const T*>(ring.ring + size_t(s) * ring.stage_bytes + at_gate * row_bytes)
+                         : static_cast<const T*>(p.gate) + size_t(group) * p.d;
+  };
+  int s = 0;
+  uint32_t phase = 0;             // of the stage of row + 1
+  long long left = p.gate ? p.group_rows : 0;        // rows of the current group from row on (a part of a group ends with the CTA's rows)
+  Stats now = stats_of(lo), next = stats_of(lo + 1);
+  if (lo < hi) {
+    ring.wait(0, 0);
+    if (p.gate) load_gate(gate_of(0));
+    row_sums(0, now);
+  }
+  __syncthreads();
+  int s_next = p.stages > 1 ? 1 : 0;
+  phase = p.stages > 1 ? 0 : 1;
+  for (long long row = lo; row < hi; ++row) {
+    float sums[4];
+    sum4_end(sums, scratch + slot * 128, span);
+    slot ^= 1;
+    const bool more = row + 1 < hi, group_end = p.gate && (left == 1 || !more);
+    const Stats after = stats_of(row + 2);
+    // (with one stage the next row comes only when this one is done with)
+    const bool early = more && !group_end && p.stages > 1;
+    if (early) {
+      ring.wait(s_next, phase);
+      row_sums(s_next, next);
+    }
+    row_results(s, row, now, sums);
+    if (group_end) {
+      flush(gate_of(s));
       ++group;
+      left = p.group_rows + 1;
     }
-    __syncthreads();              // every thread has read this stage
-    if (tid == 0 && row + p.stages < hi) ring.issue(s, row + p.stages);
-    if (++s == p.stages) { s = 0; phase ^= 1; }
+    --left;
+    if (more && !early) {
+      if (p.stages == 1) {
+        __syncthreads();
+        ring.ask_all(0, row + 1);
+      }
+      ring.wait(s_next, phase);
+      if (group_end) load_gate(gate_of(s_next));
+      row_sums(s_next, next);
+    }
+    __syncthreads();              // the sums of row + 1 are there, and the stage of this row is done with
+    if (p.stages > 1 && row + p.stages < hi) ring.ask_all(s, row + p.stages);
+    s = s_next;
+    if (++s_next >= p.stages) { s_next = 0; phase ^= 1; }
+    now = next;
+    next = after;
   }
   if (!p.gate) flush(nullptr);
 #pragma unroll
@@ -487,36 +544,39 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
 }
 
 // Sums of partial rows: blockIdx.y 0 and 1 the weights' (`parts` rows each), 2 + g the gate's group g (`chunks` rows).  A CTA
-// owns 32 columns, its warps every 8th row, four loads in flight each; the eight sums meet in shared memory.
-template <typename T>
-__global__ void __launch_bounds__(256) residual_norm_sums_kernel(const float* scratch, void* dw_post, void* dw_pre, void* dgate, int parts,
-                                                                 int chunks, int d, int wide) {
-  __shared__ float red[8][33];
-  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
+// owns 128 columns, four a lane; its warps (8, or 32 for many rows) take a row each in turn, up to six loads in flight, and meet in
+// shared memory.
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) residual_norm_sums_kernel(const float* __restrict__ scratch, void* dw_post, void* dw_pre, void* dgate,
+                                                                 int parts, int chunks, int d, int wide) {
+  __shared__ float4 red[WARPS][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 128 + lane * 4;
   const int which = blockIdx.y;
   void* out = which == 0 ? dw_post : which == 1 ? dw_pre : dgate;
   if (out == nullptr) return;      // the same for the whole CTA
   const int n = which < 2 ? parts : chunks;
   const size_t at = which < 2 ? size_t(which) * parts * d : (size_t(2) * parts + size_t(which - 2) * chunks) * d;
   const size_t out_at = which < 2 ? 0 : size_t(which - 2) * d;
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < d) {
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (c < d) {                     // (d is a multiple of 4)
     const float* s = scratch + at + c;
-    int i = ry;
-    for (; i + 24 < n; i += 32) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) a[k] += s[size_t(i + 8 * k) * d];
+#pragma unroll 6
+    for (int i = warp; i < n; i += WARPS) {
+      const float4 v = *reinterpret_cast<const float4*>(s + size_t(i) * d);
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
-    for (; i < n; i += 8) a[0] += s[size_t(i) * d];
   }
-  red[ry][cx] = (a[0] + a[1]) + (a[2] + a[3]);
+  red[warp][lane] = a;
   __syncthreads();
-  if (ry == 0 && c < d) {
-    float v = 0.f;
+  if (threadIdx.x < 128 && blockIdx.x * 128 + int(threadIdx.x) < d) {
+    const float* r = reinterpret_cast<const float*>(red) + threadIdx.x;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += red[k][cx];
-    if (wide) static_cast<float*>(out)[out_at + c] = v;
-    else static_cast<T*>(out)[out_at + c] = from_f<T>(v);
+    for (int k = 0; k < WARPS; ++k) v[k & 3] += r[k * 128];
+    const float sum = (v[0] + v[1]) + (v[2] + v[3]);
+    const size_t o = out_at + blockIdx.x * 128 + threadIdx.x;
+    if (wide) static_cast<float*>(out)[o] = sum;
+    else static_cast<T*>(out)[o] = from_f<T>(sum);
   }
 }
 
@@ -559,7 +619,7 @@ static int rn_launch(int grid, const RnShape& shape, const ResNormParams& p, cud
   auto kernel = BWD ? residual_norm_bwd_kernel<T, VECS> : residual_norm_fwd_kernel<T, VECS>;
   if (const int rc = limit.allow(kernel, shape.smem)) return rc;
   kernel<<<grid, shape.threads, shape.smem, stream>>>(p);
-  return int(cudaGetLastError());
+  return launch_result(cudaSuccess);
 }
 template <typename F>
 static int rn_dtype(int dt, F&& f) {
@@ -636,9 +696,15 @@ JPB_API int jpb_residual_norm_bwd(int dt, const void* dr, const void* dh, const 
                                    : rn_launch<T, 4, true>(plan.grid, shape, p, s);
     if (rc) return rc;
     const bool gate_sums = gate && plan.chunks > 1;
-    if (w_post || w_pre || gate_sums)
-      residual_norm_sums_kernel<T><<<dim3((d + 31) / 32, gate_sums ? 2 + groups : 2), 256, 0, s>>>(
-          scratch, w_post ? dw_post : nullptr, w_pre ? dw_pre : nullptr, gate_sums ? dgate : nullptr, plan.grid, plan.chunks, d, wide);
-    return int(cudaGetLastError());
+    if (w_post || w_pre || gate_sums) {
+      const dim3 sums((d + 127) / 128, gate_sums ? 2 + groups : 2);
+      auto run = [&](auto kernel, int threads) {
+        kernel<<<sums, threads, 0, s>>>(scratch, w_post ? dw_post : nullptr, w_pre ? dw_pre : nullptr, gate_sums ? dgate : nullptr,
+                                        plan.grid, plan.chunks, d, wide);
+      };
+      if (plan.grid > 64) run(residual_norm_sums_kernel<T, 32>, 1024);
+      else run(residual_norm_sums_kernel<T, 8>, 256);
+    }
+    return launch_result(cudaSuccess);
   });
 }

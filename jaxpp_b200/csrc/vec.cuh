@@ -61,6 +61,13 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
+// 16 bytes from shared memory by its 32-bit address: a pointer that went through a structure is loaded from as a generic one.
+__device__ __forceinline__ void lds_vec(Vec<float>& v, uint32_t addr) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.raw.x), "=f"(v.raw.y), "=f"(v.raw.z), "=f"(v.raw.w) : "r"(addr));
+}
+__device__ __forceinline__ void lds_vec(Vec<__nv_bfloat16>& v, uint32_t addr) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.raw.x), "=r"(v.raw.y), "=r"(v.raw.z), "=r"(v.raw.w) : "r"(addr));
+}
 // 16 bytes of T as pairs, and back.
 __device__ __forceinline__ void to_pairs(const Vec<float>& v, F2 (&f)[2]) {
   f[0] = f2(v.raw.x, v.raw.y);

@@ -95,7 +95,11 @@ class _Direct:
             return self.packet(*args, **kwargs)
         grad = torch.is_grad_enabled()
         for a in args:
-            if isinstance(a, Tensor) and ((type(a) is not Tensor and type(a) is not torch.nn.Parameter) or (grad and a.requires_grad)):
+            kind = type(a)
+            if kind is Tensor or kind is torch.nn.Parameter:
+                if grad and a.requires_grad:
+                    return self.packet(*args)
+            elif isinstance(a, Tensor):
                 return self.packet(*args)
         return self._impl(*args)
 

@@ -158,6 +158,17 @@ def _rows(t: torch.Tensor) -> int:
     return t.numel() // t.shape[-1]
 
 
+def _new(shape, dtype, device) -> torch.Tensor:
+    """``torch.empty`` by way of ``empty_strided``, which takes half its time (1.4 us instead of 3)."""
+    if len(shape) == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
+    strides, n = [], 1
+    for size in reversed(shape):
+        strides.append(n)
+        n *= size if size > 1 else 1
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
+
+
 # ---- GEMM ---------------------------------------------------------------------------------------------
 def _as_2d_bf16(t: torch.Tensor) -> torch.Tensor:
     # the common case first (a contiguous bfloat16 matrix whose rows start on 16-byte boundaries): this function runs
@@ -298,13 +309,13 @@ def _ragged_operands(what, offsets, *ts):
             raise NativeError(f"{what}: the tcgen05 GEMM takes bfloat16 operands, got {t.dtype}")
         if t.shape[-1] % 8 or t.shape[-2] % 8 and t.dim() == 3:
             raise NativeError(f"{what}: feature sizes have to be multiples of 8, got {tuple(t.shape)}")
-    return (offsets.contiguous(), *(_vectors(t) for t in ts))
+    return (offsets if offsets.is_contiguous() else offsets.contiguous(), *[_vectors(t) for t in ts])
 
 
 def _linear_ragged(what, rows, w, offsets, transposed):
     offsets, rows, w = _ragged_operands(what, offsets, rows, w)
     E, N, K = w.shape
-    out = torch.empty(rows.shape[0], K if transposed else N, dtype=torch.bfloat16, device=rows.device)
+    out = _new((rows.shape[0], K if transposed else N), torch.bfloat16, rows.device)
     _check(load().jpb_linear_ragged(rows.data_ptr(), w.data_ptr(), offsets.data_ptr(), out.data_ptr(), rows.shape[0], E, N, K,
                                     int(transposed), _stream()), what)
     return out
@@ -326,7 +337,7 @@ def linear_ragged_wgrad(dy, x, offsets, out_dtype=None, out=None, accumulate=Fal
         out_dtype = out_dtype or dy.dtype
         if out_dtype not in (torch.bfloat16, torch.float32):
             raise NativeError(f"linear_ragged_wgrad writes bfloat16 or float32, not {out_dtype}")
-        out = torch.empty(E, N, K, dtype=out_dtype, device=dy.device)
+        out = _new((E, N, K), out_dtype, dy.device)
     _check(load().jpb_linear_ragged_wgrad(dy.data_ptr(), x.data_ptr(), offsets.data_ptr(), out.data_ptr(), dy.shape[0], E, N, K,
                                           int(out.dtype == torch.float32), int(accumulate), _stream()), "linear_ragged_wgrad")
     return out
@@ -441,9 +452,9 @@ def residual_norm(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
     shape, device = x.shape, x.device
     d, rows = shape[-1], shape[:-1]
     r = torch.empty_like(x)
-    h = torch.empty_like(x) if w_pre is not None else torch.empty(0, dtype=x.dtype, device=device)
-    rstd_post = torch.empty(0 if w_post is None else rows, dtype=torch.float32, device=device)
-    rstd_pre = torch.empty(0 if w_pre is None else rows, dtype=torch.float32, device=device)
+    h = torch.empty_like(x) if w_pre is not None else _new((0,), x.dtype, device)
+    rstd_post = _new((0,) if w_post is None else rows, torch.float32, device)
+    rstd_pre = _new((0,) if w_pre is None else rows, torch.float32, device)
     lib = load()
     if x.numel():
         _check(lib.jpb_residual_norm_fwd(_dt(x), x.data_ptr(), y.data_ptr(), _p(w_post), _p(gate), _p(w_pre), r.data_ptr(), h.data_ptr(),
@@ -454,17 +465,17 @@ def residual_norm(x, y, w_post, gate, w_pre, scale=1.0, eps=1e-5):
 
 def residual_norm_bwd(dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre, scale=1.0, sum_dtype=None):
     _here("residual_norm_bwd", dr, dh, x, y, w_post, gate, w_pre, rstd_post, rstd_pre)
-    dr, dh, x, y, w_post, gate, w_pre = (_vectors(t) for t in (dr, dh, x, y, w_post, gate, w_pre))
+    dr, dh, x, y, w_post, gate, w_pre = [_vectors(t) for t in (dr, dh, x, y, w_post, gate, w_pre)]
     rstd_post, rstd_pre = rstd_post.contiguous(), rstd_pre.contiguous()
     wide, sums = _wide(sum_dtype, x), sum_dtype or x.dtype
-    like = lambda w: torch.empty(0, dtype=x.dtype, device=x.device) if w is None else torch.empty(w.shape, dtype=sums, device=x.device)
+    like = lambda w: _new((0,), x.dtype, x.device) if w is None else _new(w.shape, sums, x.device)
     dx, dy, dw_post, dgate, dw_pre = torch.empty_like(x), torch.empty_like(x), like(w_post), like(gate), like(w_pre)
     d = x.shape[-1]
     if d == 0:
         return dx, dy, dw_post, dgate, dw_pre
     rows, groups = x.numel() // d, _gate_groups(gate)
     lib = load()
-    scratch = torch.empty(lib.jpb_residual_norm_bwd_scratch_elems(_dt(x), rows, d, groups), dtype=torch.float32, device=x.device)
+    scratch = _new((lib.jpb_residual_norm_bwd_scratch_elems(_dt(x), rows, d, groups),), torch.float32, x.device)
     _check(lib.jpb_residual_norm_bwd(_dt(x), _p(dr), _p(dh), x.data_ptr(), y.data_ptr(), _p(w_post), _p(gate), _p(w_pre),
                                      rstd_post.data_ptr(), rstd_pre.data_ptr(), dx.data_ptr(), dy.data_ptr(), dw_post.data_ptr(),
                                      dgate.data_ptr(), dw_pre.data_ptr(), scratch.data_ptr(), rows, d, groups, float(scale), wide,
@@ -653,9 +664,10 @@ def _distill(dloss, logits, ids, top, lse, labels, temperature, alpha):
     dt = _dt(logits)
     logits = _vectors(logits)
     ids, top = ids.contiguous(), top.contiguous()
-    lse, labels = (None if t is None else t.contiguous() for t in (lse, labels))
+    lse = lse if lse is None else lse.contiguous()
+    labels = labels if labels is None else labels.contiguous()
     V, K = logits.shape[-1], ids.shape[-1]
-    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    loss = _new(logits.shape[:-1], torch.float32, logits.device)
     out = None
     if dloss is not None:
         dloss = dloss.float().contiguous()

@@ -408,11 +408,12 @@ def _expert_order_impl(top_i: Tensor, n_experts: int):
     native._here("expert_order", top_i)
     flat = top_i.contiguous()
     n = flat.numel()
-    dest = torch.empty(n, dtype=torch.int64, device=flat.device)
-    inv = torch.empty(n, dtype=torch.int32, device=flat.device)
-    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=flat.device)
+    device = flat.device
+    dest = native._new((n,), torch.int64, device)
+    inv = native._new((n,), torch.int32, device)
+    offsets = native._new((n_experts + 1,), torch.int32, device)
     elems = lib.jpb_expert_order_scratch_elems(n, n_experts)
-    scratch = torch.empty(elems, dtype=torch.int32, device=flat.device) if elems else None
+    scratch = native._new((elems,), torch.int32, device) if elems else None
     native._check(lib.jpb_expert_order(flat.data_ptr(), dest.data_ptr(), inv.data_ptr(), offsets.data_ptr(), native._p(scratch), n,
                                        n_experts, native._stream()), "jpb_expert_order", 2 if elems else 1)
     return dest, inv, offsets

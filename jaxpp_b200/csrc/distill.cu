@@ -149,9 +149,7 @@ __device__ __forceinline__ float plain_exp(float e, float f, float m1) {   // ex
   if (MODE == 2) { const float s = e * e; return s * s; }
   return exp2_fast(fmaf(f, LOG2E, -m1));
 }
-// The same for pairs; k = log2(e) / t, -m / t and -m in units of log 2.
 __device__ __forceinline__ F2 exp2_pair(F2 x) { return f2(exp2_fast(x.lo()), exp2_fast(x.hi())); }
-
 template <typename T, bool GRAD, int MODE, int THREADS>
 __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const __grid_constant__ DistillParams p) {
   constexpr int VN = Vec<T>::N, ES = sizeof(T);
@@ -167,7 +165,6 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
   const long long row_bytes = (long long)V * ES, step_bytes = row_step * row_bytes;
   const float it = 1.f / p.temperature, it2 = it * LOG2E;
   CtaReduce<THREADS / 32> reduce{scratch, 0};
-  const T ninf = from_f<T>(-INFINITY);
 
   // This CTA's part of the row that begins at byte `begin`: 16-byte pieces lo .. of the whole tensor, and the byte of the row's
   // first element from lo on.
@@ -197,6 +194,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
   // a conversion would wait for the load.
   struct Ahead {
     uint32_t id_lo, id_hi, top, z, z_label;
+    uint32_t edge;         // an element of the pieces at the ends of the part (16 threads have one each)
     float lse, g;
     long long label;
   };
@@ -213,8 +211,17 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
   auto id_of = [&](const Ahead& h) { return p.ids64 ? (long long)(uint64_t(h.id_hi) << 32 | h.id_lo) : (long long)int(h.id_lo); };
   auto raw_logit = [&](long long r, long long v) { return uint32_t(static_cast<const Bits*>(p.logits)[size_t(r) * V + v]); };
   auto logit_of = [&](uint32_t raw) { return __uint_as_float(ES == 2 ? raw << 16 : raw); };
-  auto ahead_ids = [&](long long r) {
+  // Element of the part that thread i has of the pieces at its ends (the others are copied whole), or -1.
+  auto edge_of = [&](const Part& q, int i) {
+    const int a = first_whole(q) * VN, b = max(a, last_whole(q) * VN);
+    return i < a ? i : b + i - a < q.pieces * VN ? b + i - a : -1;
+  };
+  auto ahead_ids = [&](long long r, long long begin) {
     Ahead h;
+    const Part q = part_of(begin);
+    const int v = edge_of(q, tid) - q.lead / ES;       // of the row
+    h.edge = 0;
+    if (tid < 2 * VN && edge_of(q, tid) >= 0 && v >= 0 && v < V) h.edge = raw_logit(r, v);
     h.id_lo = h.id_hi = 0xffffffffu;        // no entry
     h.top = h.z = h.z_label = 0;
     if (tid < K) raw_entry(r, tid, h);
@@ -241,7 +248,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
   }
   Ahead next;
   if (row0 < p.rows) {
-    next = ahead_ids(row0);
+    next = ahead_ids(row0, begin);
     ahead_logits(row0, next);
   }
   __syncthreads();
@@ -268,7 +275,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
     const float z_own = logit_of(now.z_label);
     float z_label = z_own;
     const bool more = row + row_step < p.rows;
-    if (more) next = ahead_ids(row + row_step);
+    if (more) next = ahead_ids(row + row_step, begin + step_bytes);
     // the largest of the teacher's values, and of the row's logits at the same places
     float top_max = -INFINITY, ref = -INFINITY;
     for (int j = tid; j < K; j += THREADS) {
@@ -287,13 +294,9 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       s_id[j] = !valid ? -2 : e >= v_lo && e < v_hi ? int(e) : -1;
       s_q[j] = top;
     }
-    {
-      // pieces at the ends of the row: its elements, and -inf around them
-      const int a = first_whole(q) * VN, b = max(a, last_whole(q) * VN);
-      for (int i = tid; i < a + n - b; i += THREADS) {
-        const int v = i < a ? i : b + i - a;
-        elem[v] = v >= v_lo && v < v_hi ? z[v - lead] : ninf;
-      }
+    if (tid < 2 * VN) {      // pieces at the ends of the part: the row's elements, and -inf around them
+      const int v = edge_of(q, tid);
+      if (v >= 0) reinterpret_cast<Bits*>(buf)[v] = v >= v_lo && v < v_hi ? Bits(now.edge) : ES == 2 ? Bits(0xff80u) : Bits(0xff800000u);
     }
     reduce.max2(top_max, ref);
     const bool some = top_max != -INFINITY;
@@ -403,27 +406,27 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       if (tid == 0) *mine = {m, out_t, out_1, in_t, in_1, cross, mass_in, label_here ? z_own : -INFINITY};
       __syncwarp();
       cluster_sync();
-      auto read = [&](int c) {
-        uint32_t at;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(c));
-        PartSums o;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.m), "=f"(o.out_t), "=f"(o.out_1), "=f"(o.in_t) : "r"(at) : "memory");
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.in_1), "=f"(o.cross), "=f"(o.mass), "=f"(o.label) : "r"(at + 16) : "memory");
-        return o;
-      };
-      out_t = out_1 = in_t = in_1 = cross = mass_in = 0.f;
-      M = z_label = -INFINITY;
-      for (int c = 0; c < C; ++c) M = fmaxf(M, read(c).m);
-      for (int c = 0; c < C; ++c) {
-        const PartSums o = read(c);
-        const float et = exp2_fast((o.m - M) * it2), e1 = exp2_fast((o.m - M) * LOG2E);
-        out_t += o.out_t * et;
-        out_1 += o.out_1 * e1;
-        in_t += o.in_t * et;
-        in_1 += o.in_1 * e1;
-        cross += o.cross;
-        mass_in += o.mass;
-        z_label = fmaxf(z_label, o.label);
+      // lane c reads part c (lanes go round), and the parts are added up across lanes: one trip to the other SMs
+      uint32_t at;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(tid & (C - 1)));
+      PartSums o;
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.m), "=f"(o.out_t), "=f"(o.out_1), "=f"(o.in_t) : "r"(at) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.in_1), "=f"(o.cross), "=f"(o.mass), "=f"(o.label) : "r"(at + 16) : "memory");
+      M = o.m;
+      for (int x = 1; x < C; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+      const float et = exp2_fast((o.m - M) * it2), e1 = exp2_fast((o.m - M) * LOG2E);
+      out_t = o.out_t * et; out_1 = o.out_1 * e1; in_t = o.in_t * et; in_1 = o.in_1 * e1;
+      cross = o.cross; mass_in = o.mass; z_label = o.label;
+      for (int x = 1; x < C; x <<= 1) {
+        out_t += __shfl_xor_sync(0xffffffffu, out_t, x);
+        in_t += __shfl_xor_sync(0xffffffffu, in_t, x);
+        if (MODE != 0) {
+          out_1 += __shfl_xor_sync(0xffffffffu, out_1, x);
+          in_1 += __shfl_xor_sync(0xffffffffu, in_1, x);
+        }
+        cross += __shfl_xor_sync(0xffffffffu, cross, x);
+        mass_in += __shfl_xor_sync(0xffffffffu, mass_in, x);
+        z_label = fmaxf(z_label, __shfl_xor_sync(0xffffffffu, z_label, x));
       }
     }
     const float s_t = out_t + in_t, s_1 = MODE == 0 ? s_t : out_1 + in_1, p_o = out_t / s_t;
@@ -494,8 +497,10 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
         }
       }
     }
-    if (tid < 32 && rank == 0) {  // the loss: its logarithms in four lanes
-      const float l4 = log_exact(tid == 1 ? q_sum : tid == 2 ? (rest ? ratio : 1.f) : tid == 3 ? s_1 : s_t);
+    // the loss: its logarithms in four lanes of a warp that has neither the first entries nor the next row to see to
+    if (tid >> 5 == THREADS / 32 - 2 && rank == 0) {
+      const int lane = tid & 31;
+      const float l4 = log_exact(lane == 1 ? q_sum : lane == 2 ? (rest ? ratio : 1.f) : lane == 3 ? s_1 : s_t);
       const float log_t = __shfl_sync(0xffffffffu, l4, 0), log_q = __shfl_sync(0xffffffffu, l4, 1), log_r = __shfl_sync(0xffffffffu, l4, 2),
                   log_1 = __shfl_sync(0xffffffffu, l4, 3);
       float l = 0.f;
@@ -505,7 +510,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
         l = p.alpha * p.temperature * p.temperature * soft;
       }
       if (hard) l += (1.f - p.alpha) * (log_1 - (z_label - M));
-      if (tid == 0) p.loss[row] = l;
+      if (lane == 0) p.loss[row] = l;
     }
   }
   __syncwarp();

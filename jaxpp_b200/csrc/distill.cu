@@ -246,6 +246,10 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
     if (row0 < p.rows) fetch(begin, 0);
     if (buffers == 2 && row0 + row_step < p.rows) fetch(begin + step_bytes, 1);
   }
+  // The exponentials relative to m are 2^(z * it2 - fl(m * it2)): all of them too large by 2^off, off being what the rounding of
+  // m * it2 leaves (and likewise for the plain ones).  Ratios do not see it; the logarithm of a sum takes it off.
+  auto off_t = [&](float m) { return fmaf(m, it2, -(m * it2)); };
+  auto off_1 = [&](float m) { return MODE == 1 ? 2.f * off_t(m) : MODE == 2 ? 4.f * off_t(m) : MODE == 3 ? fmaf(m, LOG2E, -(m * LOG2E)) : off_t(m); };
   Ahead next;
   if (row0 < p.rows) {
     next = ahead_ids(row0, begin);
@@ -414,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.in_1), "=f"(o.cross), "=f"(o.mass), "=f"(o.label) : "r"(at + 16) : "memory");
       M = o.m;
       for (int x = 1; x < C; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-      const float et = exp2_fast((o.m - M) * it2), e1 = exp2_fast((o.m - M) * LOG2E);
+      const float et = exp2_fast((o.m - M) * it2 + (off_t(M) - off_t(o.m))), e1 = exp2_fast((o.m - M) * LOG2E + (off_1(M) - off_1(o.m)));
       out_t = o.out_t * et; out_1 = o.out_1 * e1; in_t = o.in_t * et; in_1 = o.in_1 * e1;
       cross = o.cross; mass_in = o.mass; z_label = o.label;
       for (int x = 1; x < C; x <<= 1) {
@@ -501,8 +505,9 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
     if (tid >> 5 == THREADS / 32 - 2 && rank == 0) {
       const int lane = tid & 31;
       const float l4 = log_exact(lane == 1 ? q_sum : lane == 2 ? (rest ? ratio : 1.f) : lane == 3 ? s_1 : s_t);
-      const float log_t = __shfl_sync(0xffffffffu, l4, 0), log_q = __shfl_sync(0xffffffffu, l4, 1), log_r = __shfl_sync(0xffffffffu, l4, 2),
-                  log_1 = __shfl_sync(0xffffffffu, l4, 3);
+      constexpr float LN2 = 0.6931471805599453f;
+      const float log_t = __shfl_sync(0xffffffffu, l4, 0) - off_t(M) * LN2, log_1 = __shfl_sync(0xffffffffu, l4, 3) - off_1(M) * LN2;
+      const float log_q = __shfl_sync(0xffffffffu, l4, 1), log_r = __shfl_sync(0xffffffffu, l4, 2);
       float l = 0.f;
       if (some && p.alpha > 0.f) {
         float soft = cross + q_o * log_r;
@@ -572,7 +577,7 @@ template <typename T, bool GRAD>
 static int distill_mode(DistillParams p, cudaStream_t stream) {
   const int sms = sm_count_of_device();
   const DistillShape s = distill_shape(p.rows, p.V, p.K, sizeof(T), sms);
-  if (s.smem > 220 * 1024) return -JPB_ERR_BAD_ARGUMENT;
+  if (s.smem > 220 * 1024) return -JPB_ERR_BAD_ARGUMENT;     // a row of more than 8 x (220 KB - 24 K)
   p.log_cluster = s.cluster == 8 ? 3 : s.cluster == 4 ? 2 : s.cluster == 2;
   p.buffer = s.buffer;
   p.buffers = s.buffers;
@@ -588,13 +593,14 @@ static int distill_mode(DistillParams p, cudaStream_t stream) {
 
 // logits [rows, V] of dtype 0 = fp32 or 1 = bf16, contiguous, on a 16-byte boundary; ids [rows, K] int64 (ids64) or int32; top
 // [rows, K] fp32 (top_fp32) or bf16; lse [rows] or null; labels [rows] or null; loss [rows].  With dlogits (like logits) the
-// gradient for the row weights dloss is written too.  K <= 1024; a row of logits takes at most 1.6 MB.
+// gradient for the row weights dloss is written too.  K <= 1024; a row of logits takes at most
+// 8 times 220 KB less 24 bytes an entry.
 JPB_API int jpb_distill(int dt, const float* dloss, const void* logits, const void* ids, int ids64, const void* top, int top_fp32,
                         const float* lse, const long long* labels, float temperature, float alpha, float* loss, void* dlogits,
                         long long rows, int V, int K, void* stream) {
   using namespace jpb;
   if (rows <= 0) return 0;
-  if (V <= 0 || K < 0 || K > DISTILL_MAX_K || V > (8 * 200 * 1024) / (dt == 0 ? 4 : 2) || (dlogits && !dloss) ||
+  if (V <= 0 || K < 0 || K > DISTILL_MAX_K || V > (8 * 220 * 1024) / (dt == 0 ? 4 : 2) || (dlogits && !dloss) ||
       ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) & 15))
     return -JPB_ERR_BAD_ARGUMENT;
   DistillParams p = {logits, ids, top, lse, labels, dloss, loss, dlogits, rows, V, K, ids64, top_fp32, temperature, alpha, 0, 0, 1, nullptr};

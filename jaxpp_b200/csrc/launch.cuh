@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <mutex>
 
 namespace jpb {
 
@@ -32,15 +33,20 @@ inline int sm_count_of_device() {
 }
 // The largest dynamic shared memory that a kernel was allowed so far (one object per kernel).  Without asking, a CTA has 48 KB of
 // both kinds together: 32 KB leave room for any kernel's static part.
+// Asked for under a lock, and only ever raised: a second thread must not set a smaller limit between the first one's question and
+// its launch.
 struct SmemLimit {
   std::atomic<int> bytes[MAX_DEVICES];
+  std::mutex lock;
   template <typename Kernel>
   int allow(Kernel kernel, int want) {
     const int dev = current_device();
-    if (want <= 32 * 1024 || want <= bytes[dev].load(std::memory_order_relaxed)) return 0;
+    if (want <= 32 * 1024 || want <= bytes[dev].load(std::memory_order_acquire)) return 0;
+    std::lock_guard<std::mutex> held(lock);
+    if (want <= bytes[dev].load(std::memory_order_relaxed)) return 0;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, want);
     if (e != cudaSuccess) return launch_result(e);
-    bytes[dev].store(want, std::memory_order_relaxed);   // (of two threads at once the smaller value may stay: it is asked again)
+    bytes[dev].store(want, std::memory_order_release);
     return 0;
   }
 };

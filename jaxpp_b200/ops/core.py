@@ -271,6 +271,8 @@ def _check_ragged(rows, w, offsets, width, what):
 def _check_offsets(rows, offsets, groups, what):
     if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.shape[0] < 2 or (groups is not None and offsets.shape[0] != groups + 1):
         raise ValueError(f"{what}: offsets are [groups + 1] int32, got {tuple(offsets.shape)} {offsets.dtype}")
+    if rows.shape[0] >= 2 ** 31:
+        raise ValueError(f"{what}: fewer than 2^31 rows, got {rows.shape[0]}")
     if offsets.device != rows.device:
         raise ValueError(f"{what}: offsets are on {offsets.device}, the rows on {rows.device}")
 
@@ -964,6 +966,7 @@ _autograd("cross_entropy", _ce_autograd, _ce_setup)
 #   teacher_lse None:  q = softmax(teacher_logits / temperature) over the row's entries
 #   teacher_lse [..]:  the log-sum-exp of ALL the teacher's logits over the temperature; q = exp(teacher_logits / temperature -
 #                      teacher_lse), and what q leaves is held against what p leaves outside of the entries, as one more class
+#                      (unless p leaves less than 2^-126 there, the smallest normal number: then it has no such class)
 # An id that a row lists twice has the sum of both probabilities as far as p is concerned: each entry is a term of its own.
 # Rows without an entry have no first term, rows with a label outside of 0 .. V-1 no second one (labels None: no row has it).
 # ``distill_loss_grad`` gives the losses together with the gradient of the logits for row weights ``dloss`` that are known
@@ -1010,7 +1013,7 @@ def _distill_ref(dloss, logits, ids, top, lse, labels, temperature, alpha):
         q_rest = (1.0 - q.sum(-1, dtype=torch.float64)).clamp(min=0).float()
         inside = torch.zeros_like(z).scatter_add(-1, ids, valid.float()) > 0
         p_rest = p.masked_fill(inside, 0.0).sum(-1)
-        rest = (q_rest > 0) & (p_rest > 0)
+        rest = (q_rest > 0) & (p_rest >= 2.0 ** -126)
         one = torch.ones_like(p_rest)
         ratio = torch.where(rest, q_rest / torch.where(rest, p_rest, one), torch.zeros_like(one))
         soft = soft + torch.where(rest, q_rest * torch.where(rest, ratio, one).log(), torch.zeros_like(one))

@@ -242,7 +242,7 @@ def distill_exact(dloss, logits, ids, top, lse, labels, t, alpha):
             inside[where] = True
             if lse is not None:
                 q_o, p_o = max(0.0, 1.0 - mass), float(p[~inside].sum())
-                if q_o > 0 and p_o > 0:
+                if q_o > 0 and p_o >= 2.0 ** -126:
                     ratio = q_o / p_o
                     kl += q_o * math.log(ratio)
                     mass += q_o
@@ -302,6 +302,7 @@ DISTILLS = [  # rows, V, K, tail, labels, temperature, alpha
     (2, 32000, 64, True, True, 2.0, 0.5), (2, 50257, 100, False, False, 1.0, 1.0), (2, 333, 400, True, True, 1.0, 0.0),
     (0, 64, 4, True, True, 1.0, 0.5), (3, 40, 0, True, True, 1.0, 0.5), (2, 128256, 256, True, True, 0.5, 0.5), (300, 130, 5, True, True, 1.0, 0.5),
     (300, 24000, 16, True, True, 1.0, 1.0), (300, 12000, 16, True, True, 1.0, 1.0),   # rows that take just under 48 KB
+    (2, 500001, 64, True, True, 2.0, 0.5), (150, 32000, 64, True, True, 1.0, 0.5), (5, 70000, 1024, True, True, 4.0, 0.5),
 ]
 
 
@@ -309,6 +310,8 @@ DISTILLS = [  # rows, V, K, tail, labels, temperature, alpha
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,V,K,tail,labels,t,alpha", DISTILLS)
 def test_distill(device, dtype, rows, V, K, tail, labels, t, alpha):
+    if device == "cuda" and V * dtype.itemsize > 8 * (220 * 1024 - 24 * K):
+        pytest.skip("rows of at most 8 * (220 KB - 24 bytes an entry)")
     args = distill_inputs(rows, V, K, device, dtype, tail, labels, t, torch.int64 if K % 2 else torch.int32)
     check_distill(device, *args, t, alpha)
 
@@ -397,6 +400,23 @@ def test_distill_shapes_and_views(device):
         check(ops.distill_loss(z, ids.view(*sh, 7), top.view(*sh, 7), lse.view(sh), labels.view(sh), 1.0, 0.5).reshape(-1), want[0], twice)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_distill_far_apart(device):
+    """Logits far from the entries': sums that leave fp32's range relative to an entry, large offsets common to a row, small and
+    large temperatures, a row of equal logits."""
+    for t in (2.0, 0.25, 8.0):
+        logits, ids, top, lse, labels = distill_inputs(6, 900, 4, device, torch.float32, True, True, t, torch.int64)
+        ids[:, :] = torch.arange(4, device=device)
+        logits[0, 500:] += 300.0                # the row's maximum is e^300 above the entries
+        logits[1] += 10000.0
+        logits[2] -= 5000.0
+        logits[3] = 7.25
+        logits[4, 4:] = -400.0                  # the entries hold everything
+        ids[5], labels[5] = -1, 3
+        logits[5, :] -= 200.0                   # no entries, a label far below zero
+        check_distill(device, logits, ids, top, lse, labels, t, 0.5)
+
+
 def test_distill_refusals():
     logits, ids, top, lse, labels = distill_inputs(4, 30, 5, "cpu")
     bad = [(logits, ids[:3], top, lse, labels, 1.0, 1.0), (logits, ids.float(), top, lse, labels, 1.0, 1.0),
@@ -459,3 +479,85 @@ def test_expert_order_refusals():
                            (torch.zeros(4, 2, dtype=torch.int64), 257)):
         with pytest.raises((ValueError, RuntimeError)):
             moe.expert_order(picks, experts)
+
+
+# ---- streams and graphs -----------------------------------------------------------------------------------------------------
+def _calls():
+    """(name, call on fresh operands): what a program would capture."""
+    x, y, w_post, gate, w_pre = norm_inputs(48, 1024, 4, True, True, torch.bfloat16, "cuda")
+    _, _, a, b = ops.residual_norm(x, y, w_post, gate, w_pre, 0.9, 1e-5)
+    logits, ids, top, lse, labels = distill_inputs(60, 3001, 17, "cuda", torch.bfloat16, True, True, 2.0)
+    picks = torch.randint(0, 8, (700, 2), generator=torch.Generator().manual_seed(1)).cuda()
+    many = torch.randint(0, 64, (9000, 2), generator=torch.Generator().manual_seed(2)).cuda()
+    offsets = moe.expert_order(picks, 8)[2]
+    rows, w, dy = rnd(3, 1400, 256, dtype=torch.bfloat16, device="cuda"), rnd(4, 8, 192, 256, dtype=torch.bfloat16, device="cuda"), rnd(
+        5, 1400, 192, dtype=torch.bfloat16, device="cuda")
+    g = torch.ones(60, device="cuda")
+    return {
+        "residual_norm": (lambda: ops.residual_norm(x, y, w_post, gate, w_pre, 0.9, 1e-5), x),
+        "residual_norm_bwd": (lambda: ops.residual_norm_bwd(y, x, x, y, w_post, gate, w_pre, a, b, 0.9), y),
+        "distill_loss": (lambda: (ops.distill_loss(logits, ids, top, lse, labels, 2.0, 0.5),), logits),
+        "distill_loss_grad": (lambda: ops.distill_loss_grad(g, logits, ids, top, lse, labels, 2.0, 0.5), logits),
+        "expert_order": (lambda: moe.expert_order(picks, 8), picks),
+        "expert_order, many": (lambda: moe.expert_order(many, 64), many),
+        "linear_ragged": (lambda: (ops.linear_ragged(rows, w, offsets),), rows),
+        "linear_ragged_dgrad": (lambda: (ops.linear_ragged_dgrad(dy, w, offsets),), dy),
+        "linear_ragged_wgrad": (lambda: (ops.linear_ragged_wgrad(dy, rows, offsets),), rows),
+    }
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed_with_other_values():
+    """Every op in a graph of its own, replayed after its input has changed, and two graphs replayed at once on two streams."""
+    graphs = []
+    for name, (call, first) in _calls().items():
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((name, call, first, graph, out))
+    for name, call, first, graph, out in graphs:
+        first.copy_(first.flip(0))
+        want = [t.clone() for t in call()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(out, want):
+            assert torch.equal(p, q), name
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    wants = [[t.clone() for t in call()] for _, call, _, _, _ in graphs]
+    torch.cuda.synchronize()
+    for round_ in range(3):
+        for i, (_, _, _, graph, _) in enumerate(graphs):
+            with torch.cuda.stream(streams[(i + round_) % 3]):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (name, _, _, _, out), want in zip(graphs, wants):
+            assert all(torch.equal(p, q) for p, q in zip(out, want)), name
+
+
+@pytest.mark.gpu
+def test_several_streams_and_threads_at_once():
+    """The same calls from three threads on streams of their own give what one call alone gives."""
+    import threading
+
+    calls = _calls()
+    want = {name: [t.clone() for t in call()] for name, (call, _) in calls.items()}
+    torch.cuda.synchronize()
+    bad = []
+
+    def run():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                for name, (call, _) in calls.items():
+                    got = call()
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(p, q) for p, q in zip(got, want[name])):
+                        bad.append(name)
+
+    threads = [threading.Thread(target=run) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -527,8 +527,11 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
   }
 }
 
-// How many CTAs share a row, and their size.  A CTA's part is what fits three or more times into an SM's shared memory, so that
-// some CTAs copy while others compute; fewer rows than SMs are cut further, down to 4 KB.
+// How many CTAs share a row, and their size.  A CTA's part is what fits twice or more into an SM's shared memory, so that some CTAs
+// copy while others compute; fewer rows than half the SMs are cut further, down to 8 KB.  A cluster waits for its slowest part:
+// rows of 100 KB (1024 x 50257 bf16) whole, two to an SM, take 39 us for the loss and 55 with the gradient, halved 49 and 55.
+// 256 threads for parts of 16 KB and more, three CTAs to an SM; 128 below (of 80 registers: with 512 threads of 64 the gradient
+// of those rows takes 61 us).  Two rows are held where that costs no CTA.
 struct DistillShape {
   int cluster, buffer, buffers, smem, threads, per_sm;
 };
@@ -536,7 +539,7 @@ static DistillShape distill_shape(long long rows, int V, int K, int es, int sms)
   DistillShape s;
   const long long bytes = (long long)V * es + 32;
   s.cluster = 1;
-  while (s.cluster < 8 && (bytes / s.cluster > 70 * 1024 || (rows * s.cluster * 2 <= sms && bytes / s.cluster > 8 * 1024))) s.cluster *= 2;
+  while (s.cluster < 8 && (bytes / s.cluster > 104 * 1024 || (rows * s.cluster * 2 <= sms && bytes / s.cluster > 8 * 1024))) s.cluster *= 2;
   s.buffer = int((bytes / s.cluster + 32 + 127) / 128 * 128);
   s.threads = s.buffer > 16 * 1024 ? 256 : 128;
   const int by_threads = 768 / s.threads;              // (registers for 768 threads)

@@ -760,10 +760,18 @@ JPB_API int jpb_linear_ragged(const void* tokens, const void* w, const int* offs
   p.offsets = offsets; p.groups = groups; p.rows = rows; p.M = transposed ? K : N; p.K = transposed ? N : K;
   p.w_blocked = transposed && p.M % 64 == 0; p.D = static_cast<__nv_bfloat16*>(out); p.status = jpb_status_device_ptr();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // Which blocks (the host knows the mean of the groups' rows, not the rows).  Measured with ragged groups, us, as 1 x 32 rows /
+  // 1 x 128 / a pair's 256, L2 flushed:
+  //   8 x 14336 x 4096    mean 1: 115 / 141 / 115    24: 170 / 180 / 182    32: 195 / 182 / 182    96: - / 186 / 186   128: - / 209 / 190
+  //   64 x 1408 x 2048    mean 1: 55 / 55 / 61       24: 86 / 82 / 86       48: 100 / 82 / 88      96: - / 88 / 90     192: - / 115 / 94
+  // Small products are short of tiles, or of steps in a tile to hide its start and its store behind:
+  //   8 x 2048 x 512      mean 250: - / 18 / 20      512 (8.6 GFLOP): - / 23 / 27      1024 (17 GFLOP): - / 35 / 33
+  //   8 x 1024 x 4096     mean 128 (8.6 GFLOP): - / 33 / 35    192 (13 GFLOP): - / 33 / 37    250 (17 GFLOP): - / 49 / 39
   const int mean = (rows + groups - 1) / groups;
-  if (mean <= 32) return launch_rows<1, 32>(w, tokens, p, transposed, s);
+  if (mean <= 24) return launch_rows<1, 32>(w, tokens, p, transposed, s);
   const long long pairs = ((long long)rows / 256 + groups) * ((p.M + 255) / 256);
-  if (mean <= 128 || pairs < sm_count_of_device() / 4) return launch_rows<1, 128>(w, tokens, p, transposed, s);
+  const bool small = pairs < sm_count_of_device() / 4 || 2.0 * rows * p.M * p.K < 14e9;
+  if (mean <= 96 || small) return launch_rows<1, 128>(w, tokens, p, transposed, s);
   return launch_rows<2, 256>(w, tokens, p, transposed, s);
 }
 
@@ -781,6 +789,9 @@ JPB_API int jpb_linear_ragged_wgrad(const void* dy, const void* x, const int* of
   WgradParams p = {};
   p.offsets = offsets; p.groups = groups; p.rows = rows; p.N = N; p.K = K; p.dy_blocked = N % 64 == 0; p.x_blocked = K % 64 == 0;
   p.out_fp32 = out_fp32; p.accumulate = accumulate; p.status = jpb_status_device_ptr();
+  // Tiles of 128 x 128 where pairs' 256 x 256 would leave most SMs without one.  Measured, us, single / pairs: 8 x 512 x 512 (32
+  // pairs) 8.2 / 10.2 with 16 rows a group, 16.4 / 18.4 with 1024, 32.8 / 36.9 with 4096; 4 x 1024 x 1024 (64 pairs) 10.2 / 10.2,
+  // 20.5 / 18.4, 53.2 / 34.8.
   const long long pairs = (long long)groups * ((N + 255) / 256) * ((K + 255) / 256);
   if (pairs < sm_count_of_device() / 3) return launch_wgrad<1, 128>(dy, x, dw, p, s);
   return launch_wgrad<2, 256>(dy, x, dw, p, s);

@@ -339,9 +339,10 @@ __global__ void __launch_bounds__(1024) order_place_kernel(const long long* __re
   }
   for (int i = placed + int(blockIdx.x) * 1024 + tid; i < n; i += int(gridDim.x) * 1024) inv[i] = -1;
 }
-// Picks of a CTA: whole steps of 1024, at most 128 CTAs.  Up to 4096 picks one CTA does both steps.
+// Picks of a CTA: whole steps of 1024, at most 128 CTAs.  Up to 2048 picks one CTA does both steps (2048 picks: 10.2 us against
+// 12.3 in two launches; 3000: 14.3 against 12.3; 8192: 24.6 against 12.3).
 static int order_run(int n) {
-  if (n <= 4096) return 4096;
+  if (n <= 2048) return 2048;
   const long long steps = ((long long)n + 1023) / 1024;
   return int((steps + 127) / 128) * 1024;
 }

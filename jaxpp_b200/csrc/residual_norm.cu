@@ -51,8 +51,6 @@ struct RowRing {
   volatile int* abort_flag;
   int* status;
 
-  __device__ __forceinline__ uint32_t at_dr() const { return (1 + (x != nullptr) + (dh != nullptr)) * row_bytes; }
-  __device__ __forceinline__ uint32_t at_gate() const { return at_dr() + (dr != nullptr) * row_bytes; }
   __device__ __forceinline__ int operands() const { return int(stage_bytes / row_bytes); }
   // The k-th operand's row on its way to stage s (one thread; the barrier counts the operands).  The operands of a stage are
   // asked for by different warps: asking takes 100 cycles each.
@@ -77,18 +75,6 @@ struct RowRing {
 };
 
 template <typename T>
-__device__ __forceinline__ void load_vec(const void* base, size_t at, float (&f)[Vec<T>::N]) {
-  Vec<T> v;
-  v.load(static_cast<const T*>(base) + at);
-  v.to_float(f);
-}
-template <typename T>
-__device__ __forceinline__ void store_vec(void* base, size_t at, const float (&f)[Vec<T>::N]) {
-  Vec<T> v;
-  v.from_float(f);
-  v.store(static_cast<T*>(base) + at);
-}
-template <typename T>
 __device__ __forceinline__ Vec<T> ones() {
   Vec<T> v;
   float f[Vec<T>::N];
@@ -98,21 +84,29 @@ __device__ __forceinline__ Vec<T> ones() {
   return v;
 }
 
-// Sums over a CTA with one barrier: `slot` alternates between two halves of the scratch.  Shuffles are what a sum costs (an SM
-// does one a cycle, for all its warps): after the barrier a lane picks up one warp's part and as many steps follow as there are
-// warps, not as there are lanes; `span` is the number of warps rounded up to a power of two, the parts behind it are zeros.
-__device__ __forceinline__ float cta_sum(float v, float* scratch, int& slot, int span) {
+// Sums over a CTA with one barrier.  Shuffles are what a sum costs (an SM does one a cycle, for all its warps): lanes trade values
+// so that each ends up with one of the sums, and after the barrier a lane picks up one warp's part and as many steps follow as
+// there are warps, not as there are lanes; `span` is the number of warps rounded up to a power of two, the parts behind it are
+// zeros.  `slot` alternates between two halves of the scratch.
+// Two sums (parts as [warp][2]):
+__device__ __forceinline__ void cta_sum2(float& a, float& b, float* scratch, int& slot, int span) {
   float* s = scratch + slot * 32;
   slot ^= 1;
-  v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  const int lane = threadIdx.x & 31;
+  const bool odd = lane & 1;
+  float x = odd ? b : a;
+  x += __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+#pragma unroll
+  for (int o = 2; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if (lane < 2) s[(threadIdx.x >> 5) * 2 + lane] = x;
   __syncthreads();
-  v = s[threadIdx.x & (span - 1)];
-  for (int o = 1; o < span; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  x = s[lane & (2 * span - 1)];
+  for (int o = 2; o < 2 * span; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  const float other = __shfl_xor_sync(0xffffffffu, x, 1);
+  a = odd ? other : x;
+  b = odd ? x : other;
 }
-// Four sums at once, in two halves with a barrier between them: lanes trade values so that each ends up with one of the four (6
-// shuffles instead of 20), and after the barrier the same way (parts as [warp][4]).
+// Four (parts as [warp][4]), in two halves with the caller's barrier between them:
 __device__ __forceinline__ void sum4_begin(const float (&v)[4], float* s) {
   const int lane = threadIdx.x & 31;
   const bool b0 = lane & 1, b1 = lane & 2;
@@ -142,9 +136,28 @@ __device__ __forceinline__ int warps_span() {
   return n;
 }
 
+// gate * w_post, either of which may be null, at this thread's places.
+template <typename T, int VECS>
+__device__ __forceinline__ void gate_weights(F2 (&gw)[VECS][Vec<T>::N / 2], const void* w_post, const T* gate, int nvec) {
+  constexpr int VN = Vec<T>::N, NP = VN / 2;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v >= nvec) continue;
+    Vec<T> w = ones<T>(), g = ones<T>();
+    if (w_post) w.load(static_cast<const T*>(w_post) + size_t(v) * VN);
+    if (gate) g.load(gate + size_t(v) * VN);
+    F2 f[NP];
+    to_pairs(w, f);
+    to_pairs(g, gw[i]);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) gw[i][j] = gw[i][j] * f[j];
+  }
+}
+
 template <typename T, int VECS>
 __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const __grid_constant__ ResNormParams p) {
-  constexpr int VN = Vec<T>::N;
+  constexpr int VN = Vec<T>::N, NP = VN / 2;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int abort_flag;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);
@@ -160,89 +173,113 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], ring.operands());
     fence_barrier_init();
   }
-  Vec<T> w_post[VECS], gate[VECS], w_pre[VECS];
+  __syncthreads();
+  for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.ask_all(s, lo + s);
+  // (while the first rows come)
+  Vec<T> w_pre[VECS];
+  F2 gw[VECS][NP];      // gate * w_post
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
-    w_post[i] = gate[i] = w_pre[i] = ones<T>();
-    if (v >= nvec) continue;
-    if (p.w_post) w_post[i].load(static_cast<const T*>(p.w_post) + size_t(v) * VN);
-    if (p.w_pre) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
+    w_pre[i] = ones<T>();
+    if (v < nvec && p.w_pre) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
   }
-  __syncthreads();
-  for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.ask_all(s, lo + s);
+  const T* const gate = static_cast<const T*>(p.gate);
+  const bool now_and_then = p.gate && !p.stream_gate;
+  long long gate_end = hi;             // row from which on another row of the gate counts
+  if (now_and_then) gate_end = (lo / p.group_rows + 1) * p.group_rows;
+  else if (p.gate) gate_end = lo;
+  if (!p.stream_gate && lo < hi) gate_weights<T, VECS>(gw, p.w_post, now_and_then ? gate + size_t(lo / p.group_rows) * p.d : nullptr, nvec);
   const uint32_t ring0 = smem_u32(ring.ring) + tid * 16, step = blockDim.x * 16;
-  int slot = 0, s = 0;
-  uint32_t phase = 0;
-  long long gate_end = p.gate && !p.stream_gate ? lo : hi;   // row from which on another row of the gate counts
+  const float inv_d = 1.f / p.d;
+  const F2 scale = f2(p.scale);
+  // this thread's part of the sum of y^2 over the row in stage s
+  auto squares = [&](int s) {
+    F2 sum = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      if (tid + i * blockDim.x >= nvec) continue;
+      Vec<T> raw;
+      F2 y[NP];
+      lds_vec(raw, ring0 + s * ring.stage_bytes + i * step);
+      to_pairs(raw, y);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) sum = fma2(y[j], y[j], sum);
+    }
+    return sum.lo() + sum.hi();
+  };
+  int slot = 0, s = 0, s_next = 1;
+  uint32_t phase = 0;                                // of the stage of row + 1
+  float rstd1 = 1.f;
+  auto post = [&](float sum, long long row) {
+    if (!p.w_post) return;
+    rstd1 = rsqrtf(sum * inv_d + p.eps);
+    if (tid == 0) p.rstd_post[row] = rstd1;
+  };
+  if (lo < hi) {
+    ring.wait(0, 0);
+    float sum = squares(0), none = 0.f;
+    cta_sum2(none, sum, scratch, slot, span);
+    post(sum, lo);
+  }
+  // One barrier a row: the second norm's sum goes with the first norm's of the next row.
   for (long long row = lo; row < hi; ++row) {
+    const uint32_t sy = ring0 + s * ring.stage_bytes, sx = sy + row_bytes;
     if (row == gate_end) {
       const long long g = row / p.group_rows;
       gate_end = (g + 1) * p.group_rows;
-#pragma unroll
-      for (int i = 0; i < VECS; ++i) {
-        const int v = tid + i * blockDim.x;
-        if (v < nvec) gate[i].load(static_cast<const T*>(p.gate) + size_t(g) * p.d + size_t(v) * VN);
-      }
+      gate_weights<T, VECS>(gw, p.w_post, p.stream_gate ? reinterpret_cast<const T*>(ring.ring + size_t(s) * ring.stage_bytes + 2 * row_bytes)
+                                                        : gate + size_t(g) * p.d, nvec);
     }
-    ring.wait(s, phase);
-    const uint32_t sy = ring0 + s * ring.stage_bytes, sx = sy + row_bytes;
-    float y[VECS][VN], r[VECS][VN];
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int v = tid + i * blockDim.x;
-      if (v >= nvec) continue;
-      Vec<T> raw;
-      lds_vec(raw, sy + i * step);
-      raw.to_float(y[i]);
-      lds_vec(raw, sx + i * step);
-      raw.to_float(r[i]);
-      if (p.stream_gate) lds_vec(gate[i], sy + ring.at_gate() + i * step);
-#pragma unroll
-      for (int j = 0; j < VN; ++j) sum += y[i][j] * y[i][j];
-    }
-    float rstd1 = 1.f;
-    if (p.w_post) {
-      rstd1 = rsqrtf(cta_sum(sum, scratch, slot, span) / p.d + p.eps);
-      if (tid == 0) p.rstd_post[row] = rstd1;
-    } else {
-      __syncthreads();
-    }
-    // the row is in registers by now, of every thread: its stage takes the next one
-    if (row + p.stages < hi) ring.ask_all(s, row + p.stages);
-    sum = 0.f;
+    F2 r[VECS][NP], squares_r = f2(0.f);
+    const F2 r1 = f2(rstd1);
     T* const out_r = static_cast<T*>(p.r) + size_t(row) * p.d + size_t(tid) * VN;
-    T* const out_h = static_cast<T*>(p.h) + size_t(row) * p.d + size_t(tid) * VN;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      const int v = tid + i * blockDim.x;
-      if (v >= nvec) continue;
-      float w[VN], g[VN];
-      w_post[i].to_float(w);
-      gate[i].to_float(g);
+      if (tid + i * blockDim.x >= nvec) continue;
+      Vec<T> raw;
+      F2 y[NP];
+      lds_vec(raw, sy + i * step);
+      to_pairs(raw, y);
+      lds_vec(raw, sx + i * step);
+      to_pairs(raw, r[i]);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) {
-        r[i][j] = p.scale * r[i][j] + g[j] * (y[i][j] * rstd1 * w[j]);
-        sum += r[i][j] * r[i][j];
+      for (int j = 0; j < NP; ++j) {
+        r[i][j] = fma2(r1, y[j] * gw[i][j], scale * r[i][j]);
+        squares_r = fma2(r[i][j], r[i][j], squares_r);
       }
-      store_vec<T>(out_r, i * step / int(sizeof(T)), r[i]);
+      from_pairs(raw, r[i]);
+      raw.store(out_r + i * step / int(sizeof(T)));
     }
+    const bool more = row + 1 < hi;
+    float sum = squares_r.lo() + squares_r.hi(), sum_next = 0.f;
+    if (more) {
+      ring.wait(s_next, phase);
+      sum_next = squares(s_next);
+    }
+    cta_sum2(sum, sum_next, scratch, slot, span);
+    // every thread is done with the row's stage: it takes another row
+    if (row + p.stages < hi) ring.ask_all(s, row + p.stages);
+    if (more) post(sum_next, row + 1);
     if (p.w_pre) {
-      const float rstd2 = rsqrtf(cta_sum(sum, scratch, slot, span) / p.d + p.eps);
+      const float rstd2 = rsqrtf(sum * inv_d + p.eps);
       if (tid == 0) p.rstd_pre[row] = rstd2;
+      const F2 r2 = f2(rstd2);
+      T* const out_h = static_cast<T*>(p.h) + size_t(row) * p.d + size_t(tid) * VN;
 #pragma unroll
       for (int i = 0; i < VECS; ++i) {
-        const int v = tid + i * blockDim.x;
-        if (v >= nvec) continue;
-        float w[VN];
-        w_pre[i].to_float(w);
+        if (tid + i * blockDim.x >= nvec) continue;
+        F2 w[NP];
+        to_pairs(w_pre[i], w);
 #pragma unroll
-        for (int j = 0; j < VN; ++j) w[j] *= r[i][j] * rstd2;
-        store_vec<T>(out_h, i * step / int(sizeof(T)), w);
+        for (int j = 0; j < NP; ++j) w[j] = w[j] * (r[i][j] * r2);
+        Vec<T> raw;
+        from_pairs(raw, w);
+        raw.store(out_h + i * step / int(sizeof(T)));
       }
     }
-    if (++s == p.stages) { s = 0; phase ^= 1; }
+    s = s_next;
+    if (++s_next >= p.stages) { s_next = 0; phase ^= 1; }
   }
   if (abort_flag) {     // copies may still be in flight: many times their time
     const uint64_t begin = globaltimer_ns();
@@ -290,24 +327,12 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], ring.operands());
     fence_barrier_init();
   }
+  __syncthreads();
+  for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.ask_all(s, lo + s);
   const F2 zero = f2(0.f);
   Vec<T> w_pre[VECS];
   F2 gw[VECS][NP], S[VECS][NP], a_pre[VECS][NP];    // gate * w_post; sums of dR * p (of the group) and dh * hat
-  auto load_gate = [&](const T* gate) {                      // gate: this row's, or null
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int v = tid + i * blockDim.x;
-      if (v >= nvec) continue;
-      Vec<T> w = ones<T>(), g = ones<T>();
-      if (p.w_post) w.load(static_cast<const T*>(p.w_post) + size_t(v) * VN);
-      if (gate) g.load(gate + size_t(v) * VN);
-      F2 f[NP];
-      to_pairs(w, f);
-      to_pairs(g, gw[i]);
-#pragma unroll
-      for (int j = 0; j < NP; ++j) gw[i][j] = gw[i][j] * f[j];
-    }
-  };
+  auto load_gate = [&](const T* gate) { gate_weights<T, VECS>(gw, p.w_post, gate, nvec); };   // gate: this row's, or null
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
@@ -316,7 +341,6 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     w_pre[i] = ones<T>();
     if (v < nvec && p.w_pre) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
   }
-  if (!p.gate) load_gate(nullptr);
   long long group = lo < hi ? lo / p.group_rows : 0;
   bool first_group = true;
   // end of a group: S goes to dgate (or its partial sum) and, times the gate, to the partial sum of dw_post
@@ -357,8 +381,6 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     }
     first_group = false;
   };
-  __syncthreads();
-  for (int s = 0; s < p.stages && lo + s < hi; ++s) ring.ask_all(s, lo + s);
   // A row's sums are finished while the next row's are made: one barrier per row, between the sums of row + 1 and the results of
   // row + 1, with the results of row in front of it.  (At the end of a group the next row waits for its gate.)
   const float inv_d = 1.f / p.d;
@@ -482,8 +504,10 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
   long long left = p.gate ? p.group_rows : 0;        // rows of the current group from row on (a part of a group ends with the CTA's rows)
   Stats now = stats_of(lo), next = stats_of(lo + 1);
   if (lo < hi) {
+    if (!p.gate) load_gate(nullptr);
+    else if (!p.stream_gate) load_gate(gate_of(0));
     ring.wait(0, 0);
-    if (p.gate) load_gate(gate_of(0));
+    if (p.stream_gate) load_gate(gate_of(0));
     row_sums(0, now);
   }
   __syncthreads();
@@ -609,10 +633,13 @@ static RnPlan rn_bwd_plan(long long rows, int groups, int per_sm) {
   const long long units = groups * chunks;
   return {int(units < want ? units : want), int(chunks)};
 }
-// A gate whose rows change after a few rows of x comes with them through the ring; one that changes seldom is loaded then.
-static int rn_stream_gate(const void* gate, long long rows, int groups) { return gate && groups > 1 && rows / groups < 16; }
+// A gate whose rows change after one to three rows of x comes with them through the ring; one that changes seldomer is loaded
+// then.  Backward of 8192 x 4096 bf16, streamed / loaded, us: 168 / 199 with a gate of its own for every row, 145 / 152 for every
+// two, 135 / 131 for every four, 137 / 121 for every 32.
+static bool rn_short_groups(long long rows, int groups) { return groups > 1 && rows / groups < 4; }
+static int rn_stream_gate(const void* gate, long long rows, int groups) { return gate && rn_short_groups(rows, groups); }
 // (as many operands as the backward can have: the plan must not depend on which are absent, since the scratch goes by it)
-static int rn_bwd_operands(long long rows, int groups) { return 4 + (groups > 1 && rows / groups < 16); }
+static int rn_bwd_operands(long long rows, int groups) { return 4 + rn_short_groups(rows, groups); }
 template <typename T, int VECS, bool BWD>
 static int rn_launch(int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t stream) {
   static SmemLimit limit;

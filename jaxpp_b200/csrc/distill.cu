@@ -14,7 +14,10 @@
 // are written last.
 // What bounds it: HBM (a row read, and one written), then the exponentials, of which an SM does 16 a cycle: one per element for
 // the sums and one for the gradient.  With both temperatures in play the plain exponential is a power of the softened one where
-// t is 2 or 4, else it is taken too.
+// t is 2 or 4, else it is taken too.  4096 x 32000 bf16, 64 entries: the loss 61 us (4.3 TB/s), with the gradient 104 us (5.0 TB/s;
+// a copy would take 80): both exponentials alone keep an SM for 58 us, the rest are the barriers between a row's phases, which the
+// two or three other CTAs of the SM do not quite cover.  Many entries cost their scattered reads and writes: 512 of them 98 and
+// 198 us.
 #include "launch.cuh"
 #include "vec.cuh"
 
@@ -35,7 +38,7 @@ struct DistillParams {
   int ids64, top_fp32;
   float temperature, alpha;
   int log_cluster;             // CTAs of a row: 1, 2, 4 or 8
-  int buffer, buffers;         // bytes of a CTA's part of a row, and how many rows a CTA holds (1 or 2)
+  int buffer;                  // bytes of a CTA's part of a row
   int* status;
 };
 
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float scratch[2 * THREADS / 32 * 8];
   __shared__ __align__(16) PartSums parts[2];
-  __shared__ uint64_t full[2];
+  __shared__ uint64_t full;
   __shared__ int abort_flag, repeated[2];
   const int tid = threadIdx.x, V = p.V, K = p.K;
   const int rank = p.log_cluster ? int(cluster_ctarank()) : 0, C = 1 << p.log_cluster;
@@ -179,14 +182,14 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
   // pieces that are wholly in the row: copied at once; the one or two others hold elements of the next rows
   auto first_whole = [&](const Part& q) { return q.lead > 0 ? 1 : 0; };
   auto last_whole = [&](const Part& q) { return min(q.pieces, (q.lead + int(row_bytes)) >> 4); };
-  auto fetch = [&](long long begin, int which) {     // one thread
+  auto fetch = [&](long long begin) {                // one thread
     const Part q = part_of(begin);
     const int a = first_whole(q), b = last_whole(q);
     if (b > a) {
-      mbar_expect_tx(&full[which], uint32_t(b - a) * 16);
-      bulk_load(smem + which * p.buffer + a * 16, static_cast<const uint8_t*>(p.logits) + (q.lo + a) * 16, uint32_t(b - a) * 16, &full[which]);
+      mbar_expect_tx(&full, uint32_t(b - a) * 16);
+      bulk_load(smem + a * 16, static_cast<const uint8_t*>(p.logits) + (q.lo + a) * 16, uint32_t(b - a) * 16, &full);
     } else {
-      mbar_arrive(&full[which]);
+      mbar_arrive(&full);
     }
   };
   // What a row needs beside its logits is asked for a row ahead: first the entries (one a thread; further ones when their turn
@@ -236,15 +239,12 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
     if (h.label >= 0 && h.label < V) h.z_label = raw_logit(r, h.label);
   };
   long long begin = row0 * row_bytes;
-  const int buffers = p.buffers;
   if (tid == 0) {
     abort_flag = 0;
     repeated[0] = repeated[1] = 0;
-    mbar_init(&full[0], 1);
-    mbar_init(&full[1], 1);
+    mbar_init(&full, 1);
     fence_barrier_init();
-    if (row0 < p.rows) fetch(begin, 0);
-    if (buffers == 2 && row0 + row_step < p.rows) fetch(begin + step_bytes, 1);
+    if (row0 < p.rows) fetch(begin);
   }
   // The exponentials relative to m are 2^(z * it2 - fl(m * it2)): all of them too large by 2^off, off being what the rounding of
   // m * it2 leaves (and likewise for the plain ones).  Ratios do not see it; the logarithm of a sum takes it off.
@@ -256,14 +256,13 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
     ahead_logits(row0, next);
   }
   __syncthreads();
-  uint32_t phase = 0;             // bit of each buffer
-  int which = 0, turn = 0;
-  for (long long row = row0; row < p.rows; row += row_step, begin += step_bytes, turn ^= 1, which = buffers == 2 ? which ^ 1 : 0) {
+  int turn = 0;
+  for (long long row = row0; row < p.rows; row += row_step, begin += step_bytes, turn ^= 1) {
     const Part q = part_of(begin);
-    uint8_t* buf = smem + which * p.buffer;          // this CTA's part of the row
+    uint8_t* buf = smem;                             // this CTA's part of the row
     // [K] elements of the part where the entries' ids are (-2: no entry, -1: in another part), their logits and probabilities;
     // two sets take turns, so that the last gradients of a row need not be waited for
-    int* s_id = reinterpret_cast<int*>(smem + buffers * p.buffer) + turn * 3 * K;
+    int* s_id = reinterpret_cast<int*>(smem + p.buffer) + turn * 3 * K;
     float* s_q = reinterpret_cast<float*>(s_id + K);
     float* s_z = s_q + K;
     T* elem = reinterpret_cast<T*>(buf);
@@ -330,8 +329,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       }
     }
     // ---- the row ----
-    mbar_wait_bounded(&full[which], (phase >> which) & 1, &abort_flag, p.status);
-    phase ^= 1u << which;
+    mbar_wait_bounded(&full, turn, &abort_flag, p.status);
     // S is taken out of the row: every entry leaves its number in its place, and the one whose number is found there stands for
     // the id and leaves -inf (whose bits are no entry's number)
     volatile Bits* place = reinterpret_cast<volatile Bits*>(buf);
@@ -402,7 +400,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       if (mx == -INFINITY) break;       // nothing here but -inf: sums of zero, relative to anything
       m = mx;
     }
-    if (!GRAD && tid == THREADS - 32 && row + row_step * buffers < p.rows) fetch(begin + step_bytes * buffers, which);   // (all have read it)
+    if (!GRAD && tid == THREADS - 32 && more) fetch(begin + step_bytes);   // (all have read it)
     // ---- together with the other parts ----
     float M = m;
     if (C > 1) {
@@ -481,7 +479,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       }
       fence_proxy_async();
       __syncthreads();            // the row is done with; the elements of S and the label's are written again
-      if (tid == THREADS - 32 && row + row_step * buffers < p.rows) fetch(begin + step_bytes * buffers, which);
+      if (tid == THREADS - 32 && more) fetch(begin + step_bytes);
       if (!zero) {
         for (int j = tid, i = 0; j < K; j += THREADS, ++i) {
           if (!(owner >> i & 1)) continue;
@@ -528,26 +526,27 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
 }
 
 // How many CTAs share a row, and their size.  A CTA's part is what fits twice or more into an SM's shared memory, so that some CTAs
-// copy while others compute; fewer rows than half the SMs are cut further, down to 8 KB.  A cluster waits for its slowest part:
-// rows of 100 KB (1024 x 50257 bf16) whole, two to an SM, take 39 us for the loss and 55 with the gradient, halved 49 and 55.
-// 256 threads for parts of 16 KB and more, three CTAs to an SM; 128 below (of 80 registers: with 512 threads of 64 the gradient
-// of those rows takes 61 us).  Two rows are held where that costs no CTA.
+// copy while others compute; a cluster waits for its slowest part.  Rows of 100 KB (1024 x 50257 bf16) whole, two to an SM: 30 us
+// for the loss, 53 with the gradient; halved 37 and 54.  Of 200 KB (2048 x 100000) halved: 119 and 181 us; in four parts 218 and
+// 296.  (A CTA that held two rows, the next one on its way, was slower wherever that cost an SM a CTA, and nowhere faster.)
+// Gradients of fewer rows than half the SMs are cut further, down to 8 KB: 1 x 32000 7.6 -> 6.6 us, 36 x 32000 7.8 -> 7.4.  The
+// loss alone is not (5.3 us against 5.7): there the trade costs what the shorter pass saves.
+// 128 threads where four such CTAs fit into an SM, else 256, which two or three CTAs have the registers for: 4096 x 16000 (six
+// CTAs) 58 us with 128 threads and 69 with 256, x 24000 (four) 83 and 85, x 28000 (three) 111 and 95.
 struct DistillShape {
-  int cluster, buffer, buffers, smem, threads, per_sm;
+  int cluster, buffer, smem, threads, per_sm;
 };
-static DistillShape distill_shape(long long rows, int V, int K, int es, int sms) {
+static DistillShape distill_shape(long long rows, int V, int K, int es, bool grad, int sms) {
   DistillShape s;
   const long long bytes = (long long)V * es + 32;
   s.cluster = 1;
-  while (s.cluster < 8 && (bytes / s.cluster > 104 * 1024 || (rows * s.cluster * 2 <= sms && bytes / s.cluster > 8 * 1024))) s.cluster *= 2;
+  while (s.cluster < 8 && (bytes / s.cluster > 104 * 1024 || (grad && rows * s.cluster * 2 <= sms && bytes / s.cluster > 8 * 1024))) s.cluster *= 2;
   s.buffer = int((bytes / s.cluster + 32 + 127) / 128 * 128);
-  s.threads = s.buffer > 16 * 1024 ? 256 : 128;
-  const int by_threads = 768 / s.threads;              // (registers for 768 threads)
-  auto by_smem = [&](int buffers) { return 226 * 1024 / (buffers * s.buffer + 24 * K + 2560); };
-  s.buffers = by_smem(2) >= by_threads ? 2 : 1;
-  s.smem = s.buffers * s.buffer + 24 * K;
-  s.per_sm = by_smem(s.buffers) < by_threads ? by_smem(s.buffers) : by_threads;
-  if (s.per_sm < 1) s.per_sm = 1;
+  s.smem = s.buffer + 24 * K;
+  const int fit = 226 * 1024 / (s.smem + 2560);
+  s.threads = fit >= 4 ? 128 : 256;
+  const int most = 768 / s.threads;              // (registers for 768 threads)
+  s.per_sm = fit > most ? most : fit > 1 ? fit : 1;
   return s;
 }
 
@@ -579,11 +578,10 @@ static int distill_threads(const DistillParams& p, const DistillShape& s, int sm
 template <typename T, bool GRAD>
 static int distill_mode(DistillParams p, cudaStream_t stream) {
   const int sms = sm_count_of_device();
-  const DistillShape s = distill_shape(p.rows, p.V, p.K, sizeof(T), sms);
+  const DistillShape s = distill_shape(p.rows, p.V, p.K, sizeof(T), GRAD, sms);
   if (s.smem > 220 * 1024) return -JPB_ERR_BAD_ARGUMENT;     // a row of more than 8 x (220 KB - 24 K)
   p.log_cluster = s.cluster == 8 ? 3 : s.cluster == 4 ? 2 : s.cluster == 2;
   p.buffer = s.buffer;
-  p.buffers = s.buffers;
   p.status = jpb_status_device_ptr();
   if (p.alpha == 0.f) p.temperature = 1.f;          // the cross entropy alone
   if (p.labels == nullptr || p.alpha == 1.f || p.temperature == 1.f) return distill_threads<T, GRAD, 0>(p, s, sms, stream);
@@ -606,7 +604,7 @@ JPB_API int jpb_distill(int dt, const float* dloss, const void* logits, const vo
   if (V <= 0 || K < 0 || K > DISTILL_MAX_K || V > (8 * 220 * 1024) / (dt == 0 ? 4 : 2) || (dlogits && !dloss) ||
       ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) & 15))
     return -JPB_ERR_BAD_ARGUMENT;
-  DistillParams p = {logits, ids, top, lse, labels, dloss, loss, dlogits, rows, V, K, ids64, top_fp32, temperature, alpha, 0, 0, 1, nullptr};
+  DistillParams p = {logits, ids, top, lse, labels, dloss, loss, dlogits, rows, V, K, ids64, top_fp32, temperature, alpha, 0, 0, nullptr};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dt == 0) return dlogits ? distill_mode<float, true>(p, s) : distill_mode<float, false>(p, s);
   if (dt == 1) return dlogits ? distill_mode<__nv_bfloat16, true>(p, s) : distill_mode<__nv_bfloat16, false>(p, s);

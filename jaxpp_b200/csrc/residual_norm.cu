@@ -9,11 +9,11 @@
 // All arithmetic is fp32; r is kept unrounded between the two norms, and the backward computes it again from x and y, so that
 // its gradients are those of the forward's function and not of the rounded stream.
 //
-// What bounds it: HBM, four rows moved per row forward (x, y, r, h) and six backward (dr, dh, x, y, dx, dy).  The forward keeps up:
-// 8192 x 4096 bf16 takes 50 us (5.3 TB/s), a launch and the first row's way through included, which are 8 of them (4096 x 4096: 29
-// us).  The backward does not quite: 4096 x 8192 with a gate for each of four sequences takes 101 us and 7 for the sums of the
-// partial rows (3.7 TB/s in all; the same copies without arithmetic 67 us): every operand is widened from bf16 twice, for the sums
-// and for the results, since there is no room in the registers for a row and the three running sums of its columns.
+// What bounds it: HBM, four rows moved per row forward (x, y, r, h) and six backward (dr, dh, x, y, dx, dy).  8192 x 4096 bf16 forward
+// takes 51 us (5.3 TB/s), a launch and the first row's way through included, which are 5 of them.  Backward of 8192 x 8192 with a gate
+// for each of four sequences 153 us (5.3 TB/s), of 4096 rows 88: 78 and 7 for the sums of the partial rows (the copies without
+// arithmetic take 67): every operand is widened from bf16 twice, for the sums and for the results, since there is no room in the
+// registers for a row and the three running sums of its columns.
 #include "launch.cuh"
 #include "vec.cuh"
 
@@ -141,13 +141,13 @@ __device__ __forceinline__ int warps_span() {
 }
 
 // gate * w_post, either of which may be null, at this thread's places.
-template <typename T, int VECS>
+template <typename T, int VECS, bool FULL>
 __device__ __forceinline__ void gate_weights(F2 (&gw)[VECS][Vec<T>::N / 2], const void* w_post, const T* gate, int nvec) {
   constexpr int VN = Vec<T>::N, NP = VN / 2;
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    if (v >= nvec) continue;
+    if (!FULL && v >= nvec) continue;
     Vec<T> w = ones<T>(), g = ones<T>();
     if (w_post) w.load(static_cast<const T*>(w_post) + size_t(v) * VN);
     if (gate) g.load(gate + size_t(v) * VN);
@@ -159,9 +159,13 @@ __device__ __forceinline__ void gate_weights(F2 (&gw)[VECS][Vec<T>::N / 2], cons
   }
 }
 
-template <typename T, int VECS>
+// FULL (of both kernels): both norms and, backward, both gradients are there, rows are VECS pieces for every thread, and the gate does
+// not come through the ring, so that nothing in the loop depends on what there is.  A third of the backward's instructions were tests
+// and the moves around them: 4096 x 8192 88 us instead of 108, 16384 x 1024 55 instead of 69; forward of 4096 x 4096 26 instead of 29.
+template <typename T, int VECS, bool FULL>
 __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const __grid_constant__ ResNormParams p) {
   constexpr int VN = Vec<T>::N, NP = VN / 2;
+  const bool stream_gate = !FULL && p.stream_gate;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int abort_flag;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);
@@ -170,8 +174,8 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
   for (int i = tid; i < 64; i += blockDim.x) scratch[i] = 0.f;
   const long long lo = p.rows * blockIdx.x / gridDim.x, hi = p.rows * (blockIdx.x + 1) / gridDim.x;
   const uint32_t row_bytes = uint32_t(p.d) * sizeof(T);
-  const RowRing ring = {full, smem + RN_HEAD, row_bytes, row_bytes * (p.stream_gate ? 3 : 2), p.y, p.x, nullptr, nullptr,
-                        p.stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
+  const RowRing ring = {full, smem + RN_HEAD, row_bytes, row_bytes * (stream_gate ? 3 : 2), p.y, p.x, nullptr, nullptr,
+                        stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
   if (tid == 0) {
     abort_flag = 0;
     for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], ring.operands());
@@ -186,14 +190,14 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
     w_pre[i] = ones<T>();
-    if (v < nvec && p.w_pre) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
+    if (FULL || (v < nvec && p.w_pre)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
   }
   const T* const gate = static_cast<const T*>(p.gate);
-  const bool now_and_then = p.gate && !p.stream_gate;
+  const bool now_and_then = p.gate && !stream_gate;
   long long gate_end = hi;             // row from which on another row of the gate counts
   if (now_and_then) gate_end = (lo / p.group_rows + 1) * p.group_rows;
   else if (p.gate) gate_end = lo;
-  if (!p.stream_gate && lo < hi) gate_weights<T, VECS>(gw, p.w_post, now_and_then ? gate + size_t(lo / p.group_rows) * p.d : nullptr, nvec);
+  if (!stream_gate && lo < hi) gate_weights<T, VECS, FULL>(gw, p.w_post, now_and_then ? gate + size_t(lo / p.group_rows) * p.d : nullptr, nvec);
   const uint32_t ring0 = smem_u32(ring.ring) + tid * 16, step = blockDim.x * 16;
   const float inv_d = 1.f / p.d;
   const F2 scale = f2(p.scale);
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     F2 sum = f2(0.f);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      if (tid + i * blockDim.x >= nvec) continue;
+      if (!FULL && tid + i * blockDim.x >= nvec) continue;
       Vec<T> raw;
       F2 y[NP];
       lds_vec(raw, ring0 + s * ring.stage_bytes + i * step);
@@ -216,7 +220,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
   uint32_t phase = 0;                                // of the stage of row + 1
   float rstd1 = 1.f;
   auto post = [&](float sum, long long row) {
-    if (!p.w_post) return;
+    if (!FULL && !p.w_post) return;
     rstd1 = rsqrtf(sum * inv_d + p.eps);
     if (tid == 0) p.rstd_post[row] = rstd1;
   };
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     if (row == gate_end) {
       const long long g = row / p.group_rows;
       gate_end = (g + 1) * p.group_rows;
-      gate_weights<T, VECS>(gw, p.w_post, p.stream_gate ? reinterpret_cast<const T*>(ring.ring + size_t(s) * ring.stage_bytes + 2 * row_bytes)
+      gate_weights<T, VECS, FULL>(gw, p.w_post, stream_gate ? reinterpret_cast<const T*>(ring.ring + size_t(s) * ring.stage_bytes + 2 * row_bytes)
                                                         : gate + size_t(g) * p.d, nvec);
     }
     F2 r[VECS][NP], squares_r = f2(0.f);
@@ -240,7 +244,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     T* const out_r = static_cast<T*>(p.r) + size_t(row) * p.d + size_t(tid) * VN;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      if (tid + i * blockDim.x >= nvec) continue;
+      if (!FULL && tid + i * blockDim.x >= nvec) continue;
       Vec<T> raw;
       F2 y[NP];
       lds_vec(raw, sy + i * step);
@@ -265,14 +269,14 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     // every thread is done with the row's stage: it takes another row
     if (row + p.stages < hi) ring.ask_all(s, row + p.stages);
     if (more) post(sum_next, row + 1);
-    if (p.w_pre) {
+    if (FULL || p.w_pre) {
       const float rstd2 = rsqrtf(sum * inv_d + p.eps);
       if (tid == 0) p.rstd_pre[row] = rstd2;
       const F2 r2 = f2(rstd2);
       T* const out_h = static_cast<T*>(p.h) + size_t(row) * p.d + size_t(tid) * VN;
 #pragma unroll
       for (int i = 0; i < VECS; ++i) {
-        if (tid + i * blockDim.x >= nvec) continue;
+        if (!FULL && tid + i * blockDim.x >= nvec) continue;
         F2 w[NP];
         to_pairs(w_pre[i], w);
 #pragma unroll
@@ -299,18 +303,19 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
 // and the sums over the rows of dR * p alone, S, give both dgate = w_post * S and dw_post = gate * S.  A CTA has consecutive
 // rows: a part of one group of rows that share a gate row, or whole groups.  The sums for the gate leave at the end of a group
 // (as the result, where the CTA has all of it), those for the weights when the CTA is done.
-// (Two rounds of sums and scalar arithmetic took three times as long; the operands kept in registers from the sums on, 161 us
-// instead of 101 for 4096 x 8192, for the spills.)
-template <typename T, int VECS>
+// (Two rounds of sums and scalar arithmetic took three times as long; with the operands kept in registers from the sums on, their
+// spills made it 161 us for 4096 x 8192.)
+template <typename T, int VECS, bool FULL>
 __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const __grid_constant__ ResNormParams p) {
   constexpr int VN = Vec<T>::N, NP = VN / 2;
+  const bool stream_gate = !FULL && p.stream_gate;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int abort_flag;
   __shared__ __align__(16) float scratch[2 * 32 * 4];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);
   const int tid = threadIdx.x, nvec = p.d / VN, span = warps_span();
   for (int i = tid; i < 2 * 32 * 4; i += blockDim.x) scratch[i] = 0.f;
-  const bool pre = p.w_pre && p.dh;
+  const bool pre = FULL || (p.w_pre && p.dh), has_dr = FULL || p.dr;
   float* part_post = p.scratch + size_t(blockIdx.x) * p.d;
   float* part_pre = p.scratch + size_t(gridDim.x + blockIdx.x) * p.d;
   float* part_gate = p.scratch + size_t(2 * gridDim.x + blockIdx.x) * p.d;
@@ -324,9 +329,9 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     hi = (long long)p.groups * (blockIdx.x + 1) / gridDim.x * p.group_rows;
   }
   const uint32_t row_bytes = uint32_t(p.d) * sizeof(T);
-  const int operands = 1 + 2 * pre + (p.dr != nullptr) + p.stream_gate;
+  const int operands = FULL ? 4 : 1 + 2 * pre + has_dr + stream_gate;
   const RowRing ring = {full, smem + RN_HEAD, row_bytes, row_bytes * operands, p.y, pre ? p.x : nullptr, pre ? p.dh : nullptr, p.dr,
-                        p.stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
+                        stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
   if (tid == 0) {
     abort_flag = 0;
     for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], ring.operands());
@@ -337,14 +342,14 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
   const F2 zero = f2(0.f);
   Vec<T> w_pre[VECS];
   F2 gw[VECS][NP], S[VECS][NP], a_pre[VECS][NP];    // gate * w_post; sums of dR * p (of the group) and dh * hat
-  auto load_gate = [&](const T* gate) { gate_weights<T, VECS>(gw, p.w_post, gate, nvec); };   // gate: this row's, or null
+  auto load_gate = [&](const T* gate) { gate_weights<T, VECS, FULL>(gw, p.w_post, gate, nvec); };   // gate: this row's, or null
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
 #pragma unroll
     for (int j = 0; j < NP; ++j) S[i][j] = a_pre[i][j] = gw[i][j] = zero;
     w_pre[i] = ones<T>();
-    if (v < nvec && p.w_pre) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
+    if (FULL || (v < nvec && p.w_pre)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
   }
   long long group = lo < hi ? lo / p.group_rows : 0;
   bool first_group = true;
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
-      if (v >= nvec) continue;
+      if (!FULL && v >= nvec) continue;
       Vec<T> w = ones<T>(), g = ones<T>();
       if (p.w_post) w.load(static_cast<const T*>(p.w_post) + size_t(v) * VN);
       if (gate) g.load(gate + size_t(v) * VN);
@@ -396,7 +401,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
   auto stats_of = [&](long long row) {
     Stats t = {1.f, 0.f};
     if (row < hi) {
-      if (p.w_post) t.rstd1 = p.rstd_post[row];
+      if (FULL || p.w_post) t.rstd1 = p.rstd_post[row];
       if (pre) t.rstd2 = p.rstd_pre[row];
     }
     return t;
@@ -414,14 +419,14 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
-      if (v >= nvec) continue;
+      if (!FULL && v >= nvec) continue;
       Vec<T> raw;
       F2 c[NP], A[NP];
       lds_vec(raw, sy + i * step);
       to_pairs(raw, c);
 #pragma unroll
       for (int j = 0; j < NP; ++j) c[j] = c[j] * gw[i][j];
-      if (p.dr) {
+      if (has_dr) {
         lds_vec(raw, sdr + i * step);
         to_pairs(raw, A);
       } else {
@@ -457,19 +462,19 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     const uint32_t sy = operand(s, 0), sx = operand(s, 1), sdh = operand(s, 2), sdr = operand(s, at_dr);
     // dR = A - k1 * r = dr + rstd2 * u - k1 * rstd1 * c - k1 * scale * x;   dy = rstd1 * gate * w_post * dR - k2 * y
     const float k1 = t.rstd2 * t.rstd2 * sums[0] * inv_d;
-    const float k2 = p.w_post ? t.rstd1 * t.rstd1 * t.rstd1 * (sums[1] - k1 * sums[2]) * inv_d : 0.f;
+    const float k2 = FULL || p.w_post ? t.rstd1 * t.rstd1 * t.rstd1 * (sums[1] - k1 * sums[2]) * inv_d : 0.f;
     const F2 r1 = f2(t.rstd1), r2 = f2(t.rstd2), mc = f2(-k1 * t.rstd1), mx = f2(-k1 * p.scale), my = f2(-k2);
     T* const dx = static_cast<T*>(p.dx) + size_t(row) * p.d + size_t(tid) * VN;
     T* const dy = static_cast<T*>(p.dy) + size_t(row) * p.d + size_t(tid) * VN;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
-      if (v >= nvec) continue;
+      if (!FULL && v >= nvec) continue;
       Vec<T> raw;
       F2 y[NP], dR[NP], o[NP];
       lds_vec(raw, sy + i * step);
       to_pairs(raw, y);
-      if (p.dr) {
+      if (has_dr) {
         lds_vec(raw, sdr + i * step);
         to_pairs(raw, dR);
       } else {
@@ -501,7 +506,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     }
   };
   auto gate_of = [&](int s) {
-    return p.stream_gate ? reinterpret_cast<const T*>(ring.ring + size_t(s) * ring.stage_bytes + at_gate * row_bytes)
+    return stream_gate ? reinterpret_cast<const T*>(ring.ring + size_t(s) * ring.stage_bytes + at_gate * row_bytes)
                          : static_cast<const T*>(p.gate) + size_t(group) * p.d;
   };
   int s = 0;
@@ -510,9 +515,9 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
   Stats now = stats_of(lo), next = stats_of(lo + 1);
   if (lo < hi) {
     if (!p.gate) load_gate(nullptr);
-    else if (!p.stream_gate) load_gate(gate_of(0));
+    else if (!stream_gate) load_gate(gate_of(0));
     ring.wait(0, 0);
-    if (p.stream_gate) load_gate(gate_of(0));
+    if (stream_gate) load_gate(gate_of(0));
     row_sums(0, now);
   }
   __syncthreads();
@@ -557,11 +562,11 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
-    if (v >= nvec) continue;
+    if (!FULL && v >= nvec) continue;
     float2* to = reinterpret_cast<float2*>(part_pre) + v * NP;
 #pragma unroll
     for (int j = 0; j < NP; ++j)
-      if (p.w_pre) to[j] = make_float2(a_pre[i][j].lo(), a_pre[i][j].hi());
+      if (FULL || p.w_pre) to[j] = make_float2(a_pre[i][j].lo(), a_pre[i][j].hi());
   }
   if (p.gate && lo >= hi && p.w_post)     // a CTA without rows (none at all, or a gate of more groups than rows)
     for (int c = tid; c < p.d; c += blockDim.x) part_post[c] = 0.f;
@@ -610,8 +615,8 @@ __global__ void __launch_bounds__(32 * WARPS) residual_norm_sums_kernel(const fl
 }
 
 // Threads of a CTA, 16-byte pieces of a row per thread, CTAs per SM, stages of the ring and bytes of shared memory.  Two pieces a
-// thread, four where 512 threads need them (rows of more than 16 KB): four would take 183 us instead of 112 for the backward of
-// 8192 x 4096 and 59 instead of 55 forward.  The forward needs two stages and has them: three operands of 32 KB are its most.
+// thread, four where 512 threads need them (rows of more than 16 KB): with tests in the loops, four took 183 us instead of 112 for
+// the backward of 8192 x 4096 and 59 instead of 55 forward.  The forward needs two stages and has them: three operands of 32 KB are its most.
 struct RnShape {
   int threads, vecs, per_sm, stages, smem;
 };
@@ -647,13 +652,19 @@ static bool rn_short_groups(long long rows, int groups) { return groups > 1 && r
 static int rn_stream_gate(const void* gate, long long rows, int groups) { return gate && rn_short_groups(rows, groups); }
 // (as many operands as the backward can have: the plan must not depend on which are absent, since the scratch goes by it)
 static int rn_bwd_operands(long long rows, int groups) { return 4 + rn_short_groups(rows, groups); }
-template <typename T, int VECS, bool BWD>
-static int rn_launch(int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t stream) {
+template <typename T, int VECS, bool BWD, bool FULL>
+static int rn_launch_as(int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t stream) {
   static SmemLimit limit;
-  auto kernel = BWD ? residual_norm_bwd_kernel<T, VECS> : residual_norm_fwd_kernel<T, VECS>;
+  auto kernel = BWD ? residual_norm_bwd_kernel<T, VECS, FULL> : residual_norm_fwd_kernel<T, VECS, FULL>;
   if (const int rc = limit.allow(kernel, shape.smem)) return rc;
   kernel<<<grid, shape.threads, shape.smem, stream>>>(p);
   return launch_result(cudaSuccess);
+}
+template <typename T, bool BWD>
+static int rn_launch(int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t s) {
+  const bool full = p.d == shape.vecs * shape.threads * Vec<T>::N && p.w_post && p.w_pre && !p.stream_gate && (!BWD || (p.dr && p.dh));
+  if (shape.vecs == 2) return full ? rn_launch_as<T, 2, BWD, true>(grid, shape, p, s) : rn_launch_as<T, 2, BWD, false>(grid, shape, p, s);
+  return full ? rn_launch_as<T, 4, BWD, true>(grid, shape, p, s) : rn_launch_as<T, 4, BWD, false>(grid, shape, p, s);
 }
 template <typename F>
 static int rn_dtype(int dt, F&& f) {
@@ -692,8 +703,7 @@ JPB_API int jpb_residual_norm_fwd(int dt, const void* x, const void* y, const vo
     const long long most = (long long)sm_count_of_device() * shape.per_sm;
     const int grid = int(rows < most ? rows : most);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return shape.vecs == 2 ? rn_launch<T, 2, false>(grid, shape, p, s)
-                           : rn_launch<T, 4, false>(grid, shape, p, s);
+    return rn_launch<T, false>(grid, shape, p, s);
   });
 }
 
@@ -726,8 +736,7 @@ JPB_API int jpb_residual_norm_bwd(int dt, const void* dr, const void* dh, const 
     p.groups = groups; p.chunks = plan.chunks; p.dgate = dgate; p.wide = wide; p.scale = scale;
     p.stages = shape.stages; p.stream_gate = rn_stream_gate(gate, rows, groups); p.status = jpb_status_device_ptr();
     if (rows == 0 && gate) cudaMemsetAsync(dgate, 0, size_t(groups) * d * (wide ? 4 : sizeof(T)), s);
-    const int rc = shape.vecs == 2 ? rn_launch<T, 2, true>(plan.grid, shape, p, s)
-                                   : rn_launch<T, 4, true>(plan.grid, shape, p, s);
+    const int rc = rn_launch<T, true>(plan.grid, shape, p, s);
     if (rc) return rc;
     const bool gate_sums = gate && plan.chunks > 1;
     if (w_post || w_pre || gate_sums) {

@@ -76,6 +76,7 @@ NORMS = [  # rows, d, gate rows (0: one vector; None: no gate), post, pre
     (1, 8, 0, True, True), (5, 8, None, True, True), (3, 264, 0, True, False), (4, 1024, None, False, True), (6, 40, 2, True, True),
     (7, 4096, 7, True, True), (130, 1600, 0, True, True), (64, 512, 4, False, True), (2, 8192, 0, True, True),
     (9, 136, 3, True, False), (40, 2000, 0, True, True), (0, 64, 0, True, True), (300, 128, 0, False, False), (40, 16384, 2, True, True),
+    (300, 1024, 4, True, True), (160, 2048, 40, True, True), (97, 512, 0, True, True), (320, 5120, None, True, True), (64, 256, 64, True, True),
 ]
 
 

@@ -62,7 +62,9 @@ def _define(schema: str, ref_impl, fake_impl, native_name: str | None = None, ch
         def impl(*args, __ref=ref_impl, __nn=native_name, __check=check):
             if __check is not None:
                 __check(*args)
-            first = next(a for a in args if isinstance(a, Tensor))
+            for first in args:
+                if isinstance(first, Tensor):
+                    break
             if _use_native(first):
                 return getattr(_native(), __nn)(*args)
             return __ref(*args)

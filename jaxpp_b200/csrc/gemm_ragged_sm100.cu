@@ -101,11 +101,11 @@ struct RowsTile {
   int group, m_blk, t0, n;   // rows t0 .. t0 + n of the tokens
 };
 template <int BT, int GRAIN>
-__device__ __forceinline__ RowsTile rows_tile(const RowsParams& p, const int* off, const int* first, int tile, int& e) {
-  while (tile >= first[e + 1]) ++e;
+__device__ __forceinline__ RowsTile rows_tile(int tiles_m, const int* off, const int* first, int tile, int& e) {   // first: in blocks
+  while (tile >= first[e + 1] * tiles_m) ++e;
   const int n = off[e + 1] - off[e], blocks = blocks_of<BT>(n), grains = (n + GRAIN - 1) / GRAIN;
   constexpr int GB = GROUP_BLOCKS / BT;
-  const int i = tile - first[e], per = GB * p.tiles_m, g = i / per, in = i - g * per;
+  const int i = tile - first[e] * tiles_m, per = GB * tiles_m, g = i / per, in = i - g * per;
   const int gb = min(GB, blocks - g * GB);
   const int m_blk = in / gb, b = g * GB + in - m_blk * gb;
   const int lo = int((long long)grains * b / blocks) * GRAIN, hi = int((long long)grains * (b + 1) / blocks) * GRAIN;
@@ -153,13 +153,28 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     tmem_relinquish_cg<CG>();
   }
   if (warp == 2)
-    make_table(p.offsets, p.groups, p.rows, off, first, [&](int n) { return n > 0 ? blocks_of<BT>(n) * p.tiles_m : 0; });
+    make_table(p.offsets, p.groups, p.rows, off, first, [&](int n) { return n > 0 ? blocks_of<BT>(n) : 0; });
   tc_fence_before();
   __syncthreads();
   if (CG == 2) cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int num_tiles = first[p.groups];
+  const int blocks = first[p.groups];
+  // Weight rows of a tile.  Blocks of few tokens are a pass over the weights, at 6.8 TB/s while all SMs read and 70 GB/s of an SM
+  // alone: a last round of a few tiles takes as long as a quarter of a round does otherwise.  Lower tiles, whose copies overlap (in
+  // L2), give that round more of them.  One token of two experts of 28672 x 4096, 448 tiles of 128 rows on 148 SMs: 86 us with
+  // these, 83 with the 552 of 104 that this finds; a token of each of eight 280 and 268 (7.0 TB/s).  (Tiles of 32 rows in that round
+  // alone took 90: an SM's rate falls with the size of its copies.)
+  int height = 128 * CG, tiles_m = p.tiles_m;
+  if constexpr (BT == 32 && !W_MN) {
+    long long best = 0x7fffffffffffffffll;
+    for (int h = 128; h >= 96; h -= 8) {
+      const int per = (p.M + h - 1) / h, tiles = blocks * per, last = tiles % tile_step;
+      const long long cost = (long long)(tiles - last) * h + (last ? max(last * h, 128 * 96) : 0);     // rows at the common rate
+      if (cost < best) { best = cost; height = h; tiles_m = per; }
+    }
+  }
+  const int num_tiles = blocks * tiles_m;
 
   if (warp == 0) {
     // ------------------------------- TMA producer --------------------------------------------
@@ -167,9 +182,9 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     bool ok = true;
     int e = 0;
     for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-      const RowsTile t = rows_tile<BT, GRAIN>(p, off, first, tile, e);
+      const RowsTile t = rows_tile<BT, GRAIN>(tiles_m, off, first, tile, e);
       const int n_mma = (t.n + GRAIN - 1) / GRAIN * GRAIN;
-      const int m0 = (t.m_blk * CG + rank) * 128, t_rows = n_mma / CG, t0 = t.t0 + rank * t_rows;
+      const int m0 = t.m_blk * height + rank * 128, t_rows = n_mma / CG, t0 = t.t0 + rank * t_rows;
       const uint32_t bytes = W_BYTES + (t_rows + C::BOX - 1) / C::BOX * (C::BOX * BK * 2);
       for (int kb = 0; kb < k_blocks; ++kb) {
         const int s = it % STAGES;
@@ -236,7 +251,7 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       bool ok = true;
       int e = 0;
       for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++tile_i) {
-        const RowsTile t = rows_tile<BT, GRAIN>(p, off, first, tile, e);
+        const RowsTile t = rows_tile<BT, GRAIN>(tiles_m, off, first, tile, e);
         const uint32_t idesc = idesc0 | (uint32_t((t.n + GRAIN - 1) / GRAIN * GRAIN >> 3) << 17);
         const uint32_t acc = tile_i & 1, acc_ph = (tile_i >> 1) & 1;
         if (!mbar_wait_bounded_warp(&acc_empty[acc], acc_ph ^ 1, abort_flag, p.status)) { ok = false; break; }
@@ -277,15 +292,15 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     bool ok = true;
     int e = 0;
     for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++tile_i) {
-      const RowsTile t = rows_tile<BT, GRAIN>(p, off, first, tile, e);
+      const RowsTile t = rows_tile<BT, GRAIN>(tiles_m, off, first, tile, e);
       const uint32_t acc = tile_i & 1, acc_ph = (tile_i >> 1) & 1;
       if (!mbar_wait_bounded_warp(&acc_full[acc], acc_ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
       const uint32_t t_acc = tmem_base + (uint32_t(quarter * 32) << 16) + acc * BT;
       // A thread holds one column of the result, the tokens one after the other.  Neighbours trade every second value, so
       // that a lane has two columns of one token: 4 bytes a lane, two rows of 64 bytes a warp and store.
-      const int col = (t.m_blk * CG + rank) * 128 + quarter * 32 + (lane & ~1);
-      const bool odd = lane & 1, in = col < p.M;
+      const int at = rank * 128 + quarter * 32 + (lane & ~1), col = t.m_blk * height + at;
+      const bool odd = lane & 1, in = at < height && col < p.M;
       __nv_bfloat16* d = p.D + size_t(t.t0) * p.M + col;
 #pragma unroll 1
       for (int c = 0; c < t.n; c += 32) {
@@ -703,7 +718,7 @@ static int launch_rows(const void* w, const void* tokens, RowsParams& p, int w_m
   const uint32_t box[2] = {BK, uint32_t(C::BOX)};
   if ((rc = jpb_make_tensor_map(&mt, tokens, 2, 2, dims, strides, box, 1))) return rc;
   p.tiles_m = (p.M + 128 * CG - 1) / (128 * CG);
-  const long long tiles = ((long long)(p.rows + BT - 1) / BT + p.groups) * p.tiles_m;
+  const long long tiles = ((long long)(p.rows + BT - 1) / BT + p.groups) * (p.M / (96 * CG) + 1);      // at most
   if (tiles > 0x7fffffffll) return -JPB_ERR_BAD_ARGUMENT;
   static SmemLimit limit[2];
   if (w_mn) return launch(limit[1], ragged_rows_kernel<CG, BT, true>, CG, C::SMEM_BYTES, 192, tiles, stream, mw, mt, p);

@@ -66,7 +66,13 @@ int* jpb_status_device_ptr() {
   std::lock_guard<std::mutex> lock(g_status_mutex);
   if (!g_status_dev[dev]) {
     int* h = nullptr;
-    if (cudaHostAlloc(reinterpret_cast<void**>(&h), 64, cudaHostAllocMapped) != cudaSuccess) return nullptr;
+    // (the first call of a process may come while its stream is captured: the allocation is not part of the graph, which this mode
+    // lets this thread say)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&h), 64, cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return nullptr;
     for (int i = 0; i < 16; ++i) h[i] = 0;
     int* d = nullptr;
     cudaHostGetDevicePointer(reinterpret_cast<void**>(&d), h, 0);

@@ -4,6 +4,9 @@ reference implementations of the ops) and on the GPU (the kernels).
 Tolerances: a result is rounded once to its type, which is half a step (``finfo.eps / 2`` of its value), and comes from fp32
 arithmetic, whose part is derived beside each test as a number of roundings of 2^-24 of the size of the terms."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -562,3 +565,35 @@ def test_several_streams_and_threads_at_once():
     for t in threads:
         t.join()
     assert not bad
+
+
+FIRST_CALLS = """
+import torch
+from jaxpp_b200.ops import core as ops
+from jaxpp_b200.parallel import moe
+
+x = torch.randn(64, 4096, device="cuda").bfloat16()
+w, y = torch.randn(2, 512, 4096, device="cuda").bfloat16(), torch.ones(4096, device="cuda", dtype=torch.bfloat16)
+offsets = torch.tensor([0, 30, 64], dtype=torch.int32, device="cuda")
+ids, top = torch.randint(0, 4096, (64, 8), device="cuda"), torch.randn(64, 8, device="cuda")
+
+def calls():
+    return (*ops.residual_norm(x, x, y, None, y), ops.linear_ragged(x, w, offsets), ops.linear_ragged_wgrad(x[:, :512], x, offsets),
+            ops.distill_loss(x, ids, top, None, None, 2.0, 1.0), *moe.expert_order(ids, 200))
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_captured():
+    """Nothing that a first call sets up (the status word, shared-memory limits, tensor maps) breaks a capture under way."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]

@@ -18,6 +18,7 @@
 #include "vec.cuh"
 
 #include <initializer_list>
+#include <type_traits>
 
 namespace jpb {
 
@@ -159,12 +160,18 @@ __device__ __forceinline__ void gate_weights(F2 (&gw)[VECS][Vec<T>::N / 2], cons
   }
 }
 
-// FULL (of both kernels): both norms and, backward, both gradients are there, rows are VECS pieces for every thread, and the gate does
-// not come through the ring, so that nothing in the loop depends on what there is.  A third of the backward's instructions were tests
-// and the moves around them: 4096 x 8192 88 us instead of 108, 16384 x 1024 55 instead of 69; forward of 4096 x 4096 26 instead of 29.
-template <typename T, int VECS, bool FULL>
+// KIND, of both kernels: what there is, so that nothing in the loop depends on it.  Unless it is RN_ANY, rows are VECS pieces for every
+// thread, the gate does not come through the ring, and the backward has dr and, with the second norm, dh.  A third of the backward's
+// instructions were tests and the moves around them: 4096 x 8192 88 us instead of 108, 16384 x 1024 55 instead of 69; forward of 4096 x
+// 4096 26 instead of 29; without the second norm, 8192 x 4096, 38 and 59 us instead of 46 and 87; without the first, 75 backward instead
+// of 105.
+enum RnKind { RN_ANY, RN_BOTH, RN_POST, RN_PRE };
+template <typename T, int VECS, int KIND>
 __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const __grid_constant__ ResNormParams p) {
   constexpr int VN = Vec<T>::N, NP = VN / 2;
+  constexpr bool FULL = KIND != RN_ANY;
+  const bool post = FULL ? KIND != RN_PRE : p.w_post != nullptr;
+  const bool pre = FULL ? KIND != RN_POST : p.w_pre != nullptr;
   const bool stream_gate = !FULL && p.stream_gate;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int abort_flag;
@@ -190,7 +197,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
     w_pre[i] = ones<T>();
-    if (FULL || (v < nvec && p.w_pre)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
+    if (pre && (FULL || v < nvec)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
   }
   const T* const gate = static_cast<const T*>(p.gate);
   const bool now_and_then = p.gate && !stream_gate;
@@ -219,8 +226,8 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
   int slot = 0, s = 0, s_next = 1;
   uint32_t phase = 0;                                // of the stage of row + 1
   float rstd1 = 1.f;
-  auto post = [&](float sum, long long row) {
-    if (!FULL && !p.w_post) return;
+  auto post_stat = [&](float sum, long long row) {
+    if (!post) return;
     rstd1 = rsqrtf(sum * inv_d + p.eps);
     if (tid == 0) p.rstd_post[row] = rstd1;
   };
@@ -228,7 +235,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     ring.wait(0, 0);
     float sum = squares(0), none = 0.f;
     cta_sum2(none, sum, scratch, slot, span);
-    post(sum, lo);
+    post_stat(sum, lo);
   }
   // One barrier a row: the second norm's sum goes with the first norm's of the next row.
   for (long long row = lo; row < hi; ++row) {
@@ -254,7 +261,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         r[i][j] = fma2(r1, y[j] * gw[i][j], scale * r[i][j]);
-        squares_r = fma2(r[i][j], r[i][j], squares_r);
+        if (pre) squares_r = fma2(r[i][j], r[i][j], squares_r);
       }
       from_pairs(raw, r[i]);
       raw.store(out_r + i * step / int(sizeof(T)));
@@ -263,13 +270,13 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     float sum = squares_r.lo() + squares_r.hi(), sum_next = 0.f;
     if (more) {
       ring.wait(s_next, phase);
-      sum_next = squares(s_next);
+      if (post) sum_next = squares(s_next);
     }
     cta_sum2(sum, sum_next, scratch, slot, span);
     // every thread is done with the row's stage: it takes another row
     if (row + p.stages < hi) ring.ask_all(s, row + p.stages);
-    if (more) post(sum_next, row + 1);
-    if (FULL || p.w_pre) {
+    if (more) post_stat(sum_next, row + 1);
+    if (pre) {
       const float rstd2 = rsqrtf(sum * inv_d + p.eps);
       if (tid == 0) p.rstd_pre[row] = rstd2;
       const F2 r2 = f2(rstd2);
@@ -305,9 +312,11 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
 // (as the result, where the CTA has all of it), those for the weights when the CTA is done.
 // (Two rounds of sums and scalar arithmetic took three times as long; with the operands kept in registers from the sums on, their
 // spills made it 161 us for 4096 x 8192.)
-template <typename T, int VECS, bool FULL>
+template <typename T, int VECS, int KIND>
 __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const __grid_constant__ ResNormParams p) {
   constexpr int VN = Vec<T>::N, NP = VN / 2;
+  constexpr bool FULL = KIND != RN_ANY;
+  const bool post = FULL ? KIND != RN_PRE : p.w_post != nullptr;
   const bool stream_gate = !FULL && p.stream_gate;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int abort_flag;
@@ -315,7 +324,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);
   const int tid = threadIdx.x, nvec = p.d / VN, span = warps_span();
   for (int i = tid; i < 2 * 32 * 4; i += blockDim.x) scratch[i] = 0.f;
-  const bool pre = FULL || (p.w_pre && p.dh), has_dr = FULL || p.dr;
+  const bool pre = FULL ? KIND != RN_POST : p.w_pre && p.dh, has_dr = FULL || p.dr;
   float* part_post = p.scratch + size_t(blockIdx.x) * p.d;
   float* part_pre = p.scratch + size_t(gridDim.x + blockIdx.x) * p.d;
   float* part_gate = p.scratch + size_t(2 * gridDim.x + blockIdx.x) * p.d;
@@ -329,7 +338,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     hi = (long long)p.groups * (blockIdx.x + 1) / gridDim.x * p.group_rows;
   }
   const uint32_t row_bytes = uint32_t(p.d) * sizeof(T);
-  const int operands = FULL ? 4 : 1 + 2 * pre + has_dr + stream_gate;
+  const int operands = FULL ? (pre ? 4 : 2) : 1 + 2 * pre + has_dr + stream_gate;
   const RowRing ring = {full, smem + RN_HEAD, row_bytes, row_bytes * operands, p.y, pre ? p.x : nullptr, pre ? p.dh : nullptr, p.dr,
                         stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
   if (tid == 0) {
@@ -349,7 +358,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
 #pragma unroll
     for (int j = 0; j < NP; ++j) S[i][j] = a_pre[i][j] = gw[i][j] = zero;
     w_pre[i] = ones<T>();
-    if (FULL || (v < nvec && p.w_pre)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
+    if (pre && (FULL || v < nvec)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
   }
   long long group = lo < hi ? lo / p.group_rows : 0;
   bool first_group = true;
@@ -401,7 +410,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
   auto stats_of = [&](long long row) {
     Stats t = {1.f, 0.f};
     if (row < hi) {
-      if (FULL || p.w_post) t.rstd1 = p.rstd_post[row];
+      if (post) t.rstd1 = p.rstd_post[row];
       if (pre) t.rstd2 = p.rstd_pre[row];
     }
     return t;
@@ -448,11 +457,12 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
           u[j] = u[j] * w[j];
           A[j] = A[j] + u[j];
           ur = fma2(u[j], r, ur);
-          cr = fma2(c[j], r, cr);
+          if (post) cr = fma2(c[j], r, cr);
         }
       }
 #pragma unroll
-      for (int j = 0; j < NP; ++j) ca = fma2(c[j], A[j], ca);
+      for (int j = 0; j < NP; ++j)
+        if (post) ca = fma2(c[j], A[j], ca);
     }
     float sums[4] = {ur.lo() + ur.hi(), ca.lo() + ca.hi(), cr.lo() + cr.hi(), 0.f};
     sum4_begin(sums, scratch + slot * 128);
@@ -462,7 +472,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     const uint32_t sy = operand(s, 0), sx = operand(s, 1), sdh = operand(s, 2), sdr = operand(s, at_dr);
     // dR = A - k1 * r = dr + rstd2 * u - k1 * rstd1 * c - k1 * scale * x;   dy = rstd1 * gate * w_post * dR - k2 * y
     const float k1 = t.rstd2 * t.rstd2 * sums[0] * inv_d;
-    const float k2 = FULL || p.w_post ? t.rstd1 * t.rstd1 * t.rstd1 * (sums[1] - k1 * sums[2]) * inv_d : 0.f;
+    const float k2 = post ? t.rstd1 * t.rstd1 * t.rstd1 * (sums[1] - k1 * sums[2]) * inv_d : 0.f;
     const F2 r1 = f2(t.rstd1), r2 = f2(t.rstd2), mc = f2(-k1 * t.rstd1), mx = f2(-k1 * p.scale), my = f2(-k2);
     T* const dx = static_cast<T*>(p.dx) + size_t(row) * p.d + size_t(tid) * VN;
     T* const dy = static_cast<T*>(p.dy) + size_t(row) * p.d + size_t(tid) * VN;
@@ -566,7 +576,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     float2* to = reinterpret_cast<float2*>(part_pre) + v * NP;
 #pragma unroll
     for (int j = 0; j < NP; ++j)
-      if (FULL || p.w_pre) to[j] = make_float2(a_pre[i][j].lo(), a_pre[i][j].hi());
+      if (p.w_pre) to[j] = make_float2(a_pre[i][j].lo(), a_pre[i][j].hi());
   }
   if (p.gate && lo >= hi && p.w_post)     // a CTA without rows (none at all, or a gate of more groups than rows)
     for (int c = tid; c < p.d; c += blockDim.x) part_post[c] = 0.f;
@@ -652,19 +662,29 @@ static bool rn_short_groups(long long rows, int groups) { return groups > 1 && r
 static int rn_stream_gate(const void* gate, long long rows, int groups) { return gate && rn_short_groups(rows, groups); }
 // (as many operands as the backward can have: the plan must not depend on which are absent, since the scratch goes by it)
 static int rn_bwd_operands(long long rows, int groups) { return 4 + rn_short_groups(rows, groups); }
-template <typename T, int VECS, bool BWD, bool FULL>
+template <typename T, int VECS, bool BWD, int KIND>
 static int rn_launch_as(int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t stream) {
   static SmemLimit limit;
-  auto kernel = BWD ? residual_norm_bwd_kernel<T, VECS, FULL> : residual_norm_fwd_kernel<T, VECS, FULL>;
+  auto kernel = BWD ? residual_norm_bwd_kernel<T, VECS, KIND> : residual_norm_fwd_kernel<T, VECS, KIND>;
   if (const int rc = limit.allow(kernel, shape.smem)) return rc;
   kernel<<<grid, shape.threads, shape.smem, stream>>>(p);
   return launch_result(cudaSuccess);
 }
 template <typename T, bool BWD>
 static int rn_launch(int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t s) {
-  const bool full = p.d == shape.vecs * shape.threads * Vec<T>::N && p.w_post && p.w_pre && !p.stream_gate && (!BWD || (p.dr && p.dh));
-  if (shape.vecs == 2) return full ? rn_launch_as<T, 2, BWD, true>(grid, shape, p, s) : rn_launch_as<T, 2, BWD, false>(grid, shape, p, s);
-  return full ? rn_launch_as<T, 4, BWD, true>(grid, shape, p, s) : rn_launch_as<T, 4, BWD, false>(grid, shape, p, s);
+  int kind = RN_ANY;
+  if (p.d == shape.vecs * shape.threads * Vec<T>::N && !p.stream_gate && (!BWD || (p.dr && (p.dh || !p.w_pre))))
+    kind = p.w_post && p.w_pre ? RN_BOTH : p.w_post ? RN_POST : p.w_pre ? RN_PRE : RN_ANY;
+  auto with = [&](auto vecs) {
+    constexpr int VECS = decltype(vecs)::value;
+    switch (kind) {
+      case RN_BOTH: return rn_launch_as<T, VECS, BWD, RN_BOTH>(grid, shape, p, s);
+      case RN_POST: return rn_launch_as<T, VECS, BWD, RN_POST>(grid, shape, p, s);
+      case RN_PRE: return rn_launch_as<T, VECS, BWD, RN_PRE>(grid, shape, p, s);
+    }
+    return rn_launch_as<T, VECS, BWD, RN_ANY>(grid, shape, p, s);
+  };
+  return shape.vecs == 2 ? with(std::integral_constant<int, 2>()) : with(std::integral_constant<int, 4>());
 }
 template <typename F>
 static int rn_dtype(int dt, F&& f) {

@@ -80,6 +80,7 @@ NORMS = [  # rows, d, gate rows (0: one vector; None: no gate), post, pre
     (7, 4096, 7, True, True), (130, 1600, 0, True, True), (64, 512, 4, False, True), (2, 8192, 0, True, True),
     (9, 136, 3, True, False), (40, 2000, 0, True, True), (0, 64, 0, True, True), (300, 128, 0, False, False), (40, 16384, 2, True, True),
     (300, 1024, 4, True, True), (160, 2048, 40, True, True), (97, 512, 0, True, True), (320, 5120, None, True, True), (64, 256, 64, True, True),
+    (300, 1024, 4, True, False), (160, 2048, None, False, True), (97, 512, 0, False, True), (65, 8192, 0, True, False), (8, 16384, 4, False, True),
 ]
 
 

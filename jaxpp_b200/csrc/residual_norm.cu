@@ -142,13 +142,13 @@ __device__ __forceinline__ int warps_span() {
 }
 
 // gate * w_post, either of which may be null, at this thread's places.
-template <typename T, int VECS, bool FULL>
+template <typename T, int VECS, bool EXACT>
 __device__ __forceinline__ void gate_weights(F2 (&gw)[VECS][Vec<T>::N / 2], const void* w_post, const T* gate, int nvec) {
   constexpr int VN = Vec<T>::N, NP = VN / 2;
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    if (!FULL && v >= nvec) continue;
+    if (!EXACT && v >= nvec) continue;
     Vec<T> w = ones<T>(), g = ones<T>();
     if (w_post) w.load(static_cast<const T*>(w_post) + size_t(v) * VN);
     if (gate) g.load(gate + size_t(v) * VN);
@@ -160,19 +160,19 @@ __device__ __forceinline__ void gate_weights(F2 (&gw)[VECS][Vec<T>::N / 2], cons
   }
 }
 
-// KIND, of both kernels: what there is, so that nothing in the loop depends on it.  Unless it is RN_ANY, rows are VECS pieces for every
-// thread, the gate does not come through the ring, and the backward has dr and, with the second norm, dh.  A third of the backward's
-// instructions were tests and the moves around them: 4096 x 8192 88 us instead of 108, 16384 x 1024 55 instead of 69; forward of 4096 x
-// 4096 26 instead of 29; without the second norm, 8192 x 4096, 38 and 59 us instead of 46 and 87; without the first, 75 backward instead
-// of 105.
+// KIND and EXACT, of both kernels: which norms there are (and then the gate does not come through the ring, and the backward has dr
+// and, with the second norm, dh), and whether rows are VECS pieces for every thread, so that the loop does not ask.  A third of the
+// backward's instructions were such tests and the moves around them: 4096 x 8192 88 us instead of 108, 16384 x 1024 55 instead of 69,
+// 15804 x 744 (not exact) 50 instead of 66; forward of 4096 x 4096 26 instead of 29; without the second norm, 8192 x 4096, 38 and 59 us
+// instead of 46 and 87; without the first, 75 backward instead of 105.
 enum RnKind { RN_ANY, RN_BOTH, RN_POST, RN_PRE };
-template <typename T, int VECS, int KIND>
+template <typename T, int VECS, int KIND, bool EXACT>
 __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const __grid_constant__ ResNormParams p) {
   constexpr int VN = Vec<T>::N, NP = VN / 2;
-  constexpr bool FULL = KIND != RN_ANY;
-  const bool post = FULL ? KIND != RN_PRE : p.w_post != nullptr;
-  const bool pre = FULL ? KIND != RN_POST : p.w_pre != nullptr;
-  const bool stream_gate = !FULL && p.stream_gate;
+  constexpr bool KNOWN = KIND != RN_ANY;
+  const bool post = KNOWN ? KIND != RN_PRE : p.w_post != nullptr;
+  const bool pre = KNOWN ? KIND != RN_POST : p.w_pre != nullptr;
+  const bool stream_gate = !KNOWN && p.stream_gate;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int abort_flag;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);
@@ -197,14 +197,14 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
     w_pre[i] = ones<T>();
-    if (pre && (FULL || v < nvec)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
+    if (pre && (EXACT || v < nvec)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
   }
   const T* const gate = static_cast<const T*>(p.gate);
   const bool now_and_then = p.gate && !stream_gate;
   long long gate_end = hi;             // row from which on another row of the gate counts
   if (now_and_then) gate_end = (lo / p.group_rows + 1) * p.group_rows;
   else if (p.gate) gate_end = lo;
-  if (!stream_gate && lo < hi) gate_weights<T, VECS, FULL>(gw, p.w_post, now_and_then ? gate + size_t(lo / p.group_rows) * p.d : nullptr, nvec);
+  if (!stream_gate && lo < hi) gate_weights<T, VECS, EXACT>(gw, p.w_post, now_and_then ? gate + size_t(lo / p.group_rows) * p.d : nullptr, nvec);
   const uint32_t ring0 = smem_u32(ring.ring) + tid * 16, step = blockDim.x * 16;
   const float inv_d = 1.f / p.d;
   const F2 scale = f2(p.scale);
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     F2 sum = f2(0.f);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      if (!FULL && tid + i * blockDim.x >= nvec) continue;
+      if (!EXACT && tid + i * blockDim.x >= nvec) continue;
       Vec<T> raw;
       F2 y[NP];
       lds_vec(raw, ring0 + s * ring.stage_bytes + i * step);
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     if (row == gate_end) {
       const long long g = row / p.group_rows;
       gate_end = (g + 1) * p.group_rows;
-      gate_weights<T, VECS, FULL>(gw, p.w_post, stream_gate ? reinterpret_cast<const T*>(ring.ring + size_t(s) * ring.stage_bytes + 2 * row_bytes)
+      gate_weights<T, VECS, EXACT>(gw, p.w_post, stream_gate ? reinterpret_cast<const T*>(ring.ring + size_t(s) * ring.stage_bytes + 2 * row_bytes)
                                                         : gate + size_t(g) * p.d, nvec);
     }
     F2 r[VECS][NP], squares_r = f2(0.f);
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
     T* const out_r = static_cast<T*>(p.r) + size_t(row) * p.d + size_t(tid) * VN;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      if (!FULL && tid + i * blockDim.x >= nvec) continue;
+      if (!EXACT && tid + i * blockDim.x >= nvec) continue;
       Vec<T> raw;
       F2 y[NP];
       lds_vec(raw, sy + i * step);
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
       T* const out_h = static_cast<T*>(p.h) + size_t(row) * p.d + size_t(tid) * VN;
 #pragma unroll
       for (int i = 0; i < VECS; ++i) {
-        if (!FULL && tid + i * blockDim.x >= nvec) continue;
+        if (!EXACT && tid + i * blockDim.x >= nvec) continue;
         F2 w[NP];
         to_pairs(w_pre[i], w);
 #pragma unroll
@@ -312,19 +312,19 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_fwd_kernel(const 
 // (as the result, where the CTA has all of it), those for the weights when the CTA is done.
 // (Two rounds of sums and scalar arithmetic took three times as long; with the operands kept in registers from the sums on, their
 // spills made it 161 us for 4096 x 8192.)
-template <typename T, int VECS, int KIND>
+template <typename T, int VECS, int KIND, bool EXACT>
 __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const __grid_constant__ ResNormParams p) {
   constexpr int VN = Vec<T>::N, NP = VN / 2;
-  constexpr bool FULL = KIND != RN_ANY;
-  const bool post = FULL ? KIND != RN_PRE : p.w_post != nullptr;
-  const bool stream_gate = !FULL && p.stream_gate;
+  constexpr bool KNOWN = KIND != RN_ANY;
+  const bool post = KNOWN ? KIND != RN_PRE : p.w_post != nullptr;
+  const bool stream_gate = !KNOWN && p.stream_gate;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int abort_flag;
   __shared__ __align__(16) float scratch[2 * 32 * 4];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);
   const int tid = threadIdx.x, nvec = p.d / VN, span = warps_span();
   for (int i = tid; i < 2 * 32 * 4; i += blockDim.x) scratch[i] = 0.f;
-  const bool pre = FULL ? KIND != RN_POST : p.w_pre && p.dh, has_dr = FULL || p.dr;
+  const bool pre = KNOWN ? KIND != RN_POST : p.w_pre && p.dh, has_dr = KNOWN || p.dr;
   float* part_post = p.scratch + size_t(blockIdx.x) * p.d;
   float* part_pre = p.scratch + size_t(gridDim.x + blockIdx.x) * p.d;
   float* part_gate = p.scratch + size_t(2 * gridDim.x + blockIdx.x) * p.d;
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     hi = (long long)p.groups * (blockIdx.x + 1) / gridDim.x * p.group_rows;
   }
   const uint32_t row_bytes = uint32_t(p.d) * sizeof(T);
-  const int operands = FULL ? (pre ? 4 : 2) : 1 + 2 * pre + has_dr + stream_gate;
+  const int operands = KNOWN ? (pre ? 4 : 2) : 1 + 2 * pre + has_dr + stream_gate;
   const RowRing ring = {full, smem + RN_HEAD, row_bytes, row_bytes * operands, p.y, pre ? p.x : nullptr, pre ? p.dh : nullptr, p.dr,
                         stream_gate ? p.gate : nullptr, p.group_rows, &abort_flag, p.status};
   if (tid == 0) {
@@ -351,14 +351,14 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
   const F2 zero = f2(0.f);
   Vec<T> w_pre[VECS];
   F2 gw[VECS][NP], S[VECS][NP], a_pre[VECS][NP];    // gate * w_post; sums of dR * p (of the group) and dh * hat
-  auto load_gate = [&](const T* gate) { gate_weights<T, VECS, FULL>(gw, p.w_post, gate, nvec); };   // gate: this row's, or null
+  auto load_gate = [&](const T* gate) { gate_weights<T, VECS, EXACT>(gw, p.w_post, gate, nvec); };   // gate: this row's, or null
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
 #pragma unroll
     for (int j = 0; j < NP; ++j) S[i][j] = a_pre[i][j] = gw[i][j] = zero;
     w_pre[i] = ones<T>();
-    if (pre && (FULL || v < nvec)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
+    if (pre && (EXACT || v < nvec)) w_pre[i].load(static_cast<const T*>(p.w_pre) + size_t(v) * VN);
   }
   long long group = lo < hi ? lo / p.group_rows : 0;
   bool first_group = true;
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
-      if (!FULL && v >= nvec) continue;
+      if (!EXACT && v >= nvec) continue;
       Vec<T> w = ones<T>(), g = ones<T>();
       if (p.w_post) w.load(static_cast<const T*>(p.w_post) + size_t(v) * VN);
       if (gate) g.load(gate + size_t(v) * VN);
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
-      if (!FULL && v >= nvec) continue;
+      if (!EXACT && v >= nvec) continue;
       Vec<T> raw;
       F2 c[NP], A[NP];
       lds_vec(raw, sy + i * step);
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
-      if (!FULL && v >= nvec) continue;
+      if (!EXACT && v >= nvec) continue;
       Vec<T> raw;
       F2 y[NP], dR[NP], o[NP];
       lds_vec(raw, sy + i * step);
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
-    if (!FULL && v >= nvec) continue;
+    if (!EXACT && v >= nvec) continue;
     float2* to = reinterpret_cast<float2*>(part_pre) + v * NP;
 #pragma unroll
     for (int j = 0; j < NP; ++j)
@@ -635,7 +635,7 @@ static RnShape rn_shape(int d, int elem, int operands) {
   const int nvec = d * elem / 16;
   s.vecs = nvec > 1024 ? 4 : 2;
   s.threads = ((nvec + s.vecs - 1) / s.vecs + 31) / 32 * 32;
-  s.per_sm = RN_THREADS / s.threads < 8 ? RN_THREADS / s.threads : 8;
+  s.per_sm = RN_THREADS / s.threads;
   const int stage = operands * d * elem;
   s.stages = (226 * 1024 / s.per_sm - 2560 - RN_HEAD) / stage;   // (2560: static and reserved shared memory of a CTA)
   if (s.stages > RN_MAX_STAGES) s.stages = RN_MAX_STAGES;
@@ -662,10 +662,10 @@ static bool rn_short_groups(long long rows, int groups) { return groups > 1 && r
 static int rn_stream_gate(const void* gate, long long rows, int groups) { return gate && rn_short_groups(rows, groups); }
 // (as many operands as the backward can have: the plan must not depend on which are absent, since the scratch goes by it)
 static int rn_bwd_operands(long long rows, int groups) { return 4 + rn_short_groups(rows, groups); }
-template <typename T, int VECS, bool BWD, int KIND>
+template <typename T, int VECS, bool BWD, int KIND, bool EXACT>
 static int rn_launch_as(int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t stream) {
   static SmemLimit limit;
-  auto kernel = BWD ? residual_norm_bwd_kernel<T, VECS, KIND> : residual_norm_fwd_kernel<T, VECS, KIND>;
+  auto kernel = BWD ? residual_norm_bwd_kernel<T, VECS, KIND, EXACT> : residual_norm_fwd_kernel<T, VECS, KIND, EXACT>;
   if (const int rc = limit.allow(kernel, shape.smem)) return rc;
   kernel<<<grid, shape.threads, shape.smem, stream>>>(p);
   return launch_result(cudaSuccess);
@@ -673,18 +673,23 @@ static int rn_launch_as(int grid, const RnShape& shape, const ResNormParams& p, 
 template <typename T, bool BWD>
 static int rn_launch(int grid, const RnShape& shape, const ResNormParams& p, cudaStream_t s) {
   int kind = RN_ANY;
-  if (p.d == shape.vecs * shape.threads * Vec<T>::N && !p.stream_gate && (!BWD || (p.dr && (p.dh || !p.w_pre))))
+  if (!p.stream_gate && (!BWD || (p.dr && (p.dh || !p.w_pre))))
     kind = p.w_post && p.w_pre ? RN_BOTH : p.w_post ? RN_POST : p.w_pre ? RN_PRE : RN_ANY;
-  auto with = [&](auto vecs) {
+  const bool exact = p.d == shape.vecs * shape.threads * Vec<T>::N;
+  auto with = [&](auto vecs, auto whole) {
     constexpr int VECS = decltype(vecs)::value;
+    constexpr bool EXACT = decltype(whole)::value;
     switch (kind) {
-      case RN_BOTH: return rn_launch_as<T, VECS, BWD, RN_BOTH>(grid, shape, p, s);
-      case RN_POST: return rn_launch_as<T, VECS, BWD, RN_POST>(grid, shape, p, s);
-      case RN_PRE: return rn_launch_as<T, VECS, BWD, RN_PRE>(grid, shape, p, s);
+      case RN_BOTH: return rn_launch_as<T, VECS, BWD, RN_BOTH, EXACT>(grid, shape, p, s);
+      case RN_POST: return rn_launch_as<T, VECS, BWD, RN_POST, EXACT>(grid, shape, p, s);
+      case RN_PRE: return rn_launch_as<T, VECS, BWD, RN_PRE, EXACT>(grid, shape, p, s);
     }
-    return rn_launch_as<T, VECS, BWD, RN_ANY>(grid, shape, p, s);
+    return rn_launch_as<T, VECS, BWD, RN_ANY, false>(grid, shape, p, s);
   };
-  return shape.vecs == 2 ? with(std::integral_constant<int, 2>()) : with(std::integral_constant<int, 4>());
+  const std::integral_constant<int, 2> two;
+  const std::integral_constant<int, 4> four;
+  if (exact) return shape.vecs == 2 ? with(two, std::true_type()) : with(four, std::true_type());
+  return shape.vecs == 2 ? with(two, std::false_type()) : with(four, std::false_type());
 }
 template <typename F>
 static int rn_dtype(int dt, F&& f) {

@@ -89,8 +89,12 @@ struct RowsParams {
   int w_blocked;         // MN-major weights through a 4-D map {64, K, M / 64, groups}: one copy per stage
   int tiles_m;
   __nv_bfloat16* D;      // [rows, M]
+  int* head;             // blocks of up to 32 rows, or null: number of parts of the reduction, first row of a group, end of the last
+  float* parts;          // [parts][rows, M]
   int* status;
 };
+// Parts of a long reduction where its tiles are fewer than half the SMs (SPLIT_MIN blocks of 64 at least in each).
+constexpr int SPLIT_MAX = 8, SPLIT_MIN = 8;
 
 // A group of n rows is cut into blocks of at most BT rows, as even as the grain allows: a stage of the ring carries 128 rows of
 // weights whatever the block's size, so that a short block costs at least half of a whole one.
@@ -174,19 +178,32 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       if (cost < best) { best = cost; height = h; tiles_m = per; }
     }
   }
-  const int num_tiles = blocks * tiles_m;
+  // few tiles: their reductions in parts, which a second kernel adds up
+  int splits = 1;
+  if constexpr (BT == 32)
+    if (p.parts) splits = max(1, min(min(SPLIT_MAX, k_blocks / SPLIT_MIN), tile_step / max(1, blocks * tiles_m)));
+  const int num_items = blocks * tiles_m * splits;
+  auto k_from = [&](int item) { return BT == 32 ? k_blocks * (item % splits) / splits : 0; };
+  auto k_to = [&](int item) { return BT == 32 ? k_blocks * (item % splits + 1) / splits : k_blocks; };
+  auto tile_of = [&](int item) { return BT == 32 ? item / splits : item; };
+  if (BT == 32 && p.parts && blockIdx.x == 0 && threadIdx.x == 64) {
+    p.head[0] = splits;
+    p.head[1] = off[0];
+    p.head[2] = off[p.groups];
+  }
 
   if (warp == 0) {
     // ------------------------------- TMA producer --------------------------------------------
     uint32_t it = 0, armed = 0, armed_phase = 0;
     bool ok = true;
     int e = 0;
-    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-      const RowsTile t = rows_tile<BT, GRAIN>(tiles_m, off, first, tile, e);
+    for (int item = first_tile; item < num_items && ok; item += tile_step) {
+      const RowsTile t = rows_tile<BT, GRAIN>(tiles_m, off, first, tile_of(item), e);
+      const int kb1 = k_to(item);
       const int n_mma = (t.n + GRAIN - 1) / GRAIN * GRAIN;
       const int m0 = t.m_blk * height + rank * 128, t_rows = n_mma / CG, t0 = t.t0 + rank * t_rows;
       const uint32_t bytes = W_BYTES + (t_rows + C::BOX - 1) / C::BOX * (C::BOX * BK * 2);
-      for (int kb = 0; kb < k_blocks; ++kb) {
+      for (int kb = k_from(item); kb < kb1; ++kb) {
         const int s = it % STAGES;
         const uint32_t ph = (it / STAGES) & 1;
         if (!mbar_wait_bounded_warp(&empty[s], ph ^ 1, abort_flag, p.status)) { ok = false; break; }
@@ -250,14 +267,15 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       uint32_t it = 0, tile_i = 0;
       bool ok = true;
       int e = 0;
-      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++tile_i) {
-        const RowsTile t = rows_tile<BT, GRAIN>(tiles_m, off, first, tile, e);
+      for (int item = first_tile; item < num_items && ok; item += tile_step, ++tile_i) {
+        const RowsTile t = rows_tile<BT, GRAIN>(tiles_m, off, first, tile_of(item), e);
+        const int kb0 = k_from(item), kb1 = k_to(item);
         const uint32_t idesc = idesc0 | (uint32_t((t.n + GRAIN - 1) / GRAIN * GRAIN >> 3) << 17);
         const uint32_t acc = tile_i & 1, acc_ph = (tile_i >> 1) & 1;
         if (!mbar_wait_bounded_warp(&acc_empty[acc], acc_ph ^ 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BT;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!mbar_wait_bounded_warp(&full[s], ph, abort_flag, p.status)) { ok = false; break; }
@@ -267,7 +285,7 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
             for (int k = 0; k < BK / UMMA_K; ++k)
               umma_bf16_ss2_cg<CG>(d_tmem, w_desc.lo + at + k * W_STEP, w_desc.hi, t_desc.lo + at + k * T_STEP, t_desc.hi, idesc,
-                                   kb > 0 || k > 0);
+                                   kb > kb0 || k > 0);
             umma_commit_cg<CG>(&empty[s], 3);
           }
           __syncwarp();
@@ -291,8 +309,8 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     uint32_t tile_i = 0;
     bool ok = true;
     int e = 0;
-    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++tile_i) {
-      const RowsTile t = rows_tile<BT, GRAIN>(tiles_m, off, first, tile, e);
+    for (int item = first_tile; item < num_items && ok; item += tile_step, ++tile_i) {
+      const RowsTile t = rows_tile<BT, GRAIN>(tiles_m, off, first, tile_of(item), e);
       const uint32_t acc = tile_i & 1, acc_ph = (tile_i >> 1) & 1;
       if (!mbar_wait_bounded_warp(&acc_full[acc], acc_ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
@@ -307,6 +325,14 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         uint32_t v[32];
         tmem_ld_32x32(t_acc + c, v);
         tc_wait_ld();
+        if (BT == 32 && splits > 1) {
+          const int own = at + odd;
+          float* to = p.parts + (size_t(item % splits) * p.rows + t.t0) * p.M + t.m_blk * height + own;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (in && j < t.n) to[size_t(j) * p.M] = __uint_as_float(v[j]);
+          continue;
+        }
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
           const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
@@ -331,6 +357,25 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_cg<CG>(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// The parts of a reduction added up, eight columns a thread; rows of no group have their zeros.
+__global__ void __launch_bounds__(256) ragged_parts_kernel(const int* __restrict__ head, const float* __restrict__ parts,
+                                                           __nv_bfloat16* __restrict__ D, int rows, int M) {
+  const int splits = head[0], lo = head[1], hi = head[2], pieces = M >> 3;
+  if (splits < 2) return;
+  const long long n = (long long)(hi - lo) * pieces;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const size_t at = size_t(lo) * M + i * 8;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    for (int k = 0; k < splits; ++k) {
+      const float4* q = reinterpret_cast<const float4*>(parts + size_t(k) * rows * M + at);
+      const float4 u = __ldcg(q), v = __ldcg(q + 1);
+      a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+      b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+    }
+    *reinterpret_cast<uint4*>(D + at) = make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
   }
 }
 
@@ -718,7 +763,7 @@ static int launch_rows(const void* w, const void* tokens, RowsParams& p, int w_m
   const uint32_t box[2] = {BK, uint32_t(C::BOX)};
   if ((rc = jpb_make_tensor_map(&mt, tokens, 2, 2, dims, strides, box, 1))) return rc;
   p.tiles_m = (p.M + 128 * CG - 1) / (128 * CG);
-  const long long tiles = ((long long)(p.rows + BT - 1) / BT + p.groups) * (p.M / (96 * CG) + 1);      // at most
+  const long long tiles = ((long long)(p.rows + BT - 1) / BT + p.groups) * (p.M / (96 * CG) + 1) * (p.parts ? SPLIT_MAX : 1);   // at most
   if (tiles > 0x7fffffffll) return -JPB_ERR_BAD_ARGUMENT;
   static SmemLimit limit[2];
   if (w_mn) return launch(limit[1], ragged_rows_kernel<CG, BT, true>, CG, C::SMEM_BYTES, 192, tiles, stream, mw, mt, p);
@@ -756,6 +801,15 @@ static int launch_wgrad(const void* dy, const void* x, void* D, WgradParams& p, 
   return launch(limit, ragged_wgrad_kernel<CG, BN>, CG, C::smem_bytes(p.stages, p.groups), 224, tiles, stream, ma, mb, md, p);
 }
 
+// Parts that the reduction of blocks of up to 32 rows may have: none where the tiles may be more than half the SMs, or for
+// reductions of less than 2048, where their sum costs more than they save.  One token of two experts, us, whole / in parts: 4096 x
+// 14336 59 / 45, 4096 x 4096 21 / 16, 2048 x 8192 36 / 17, 1024 x 2048 13.1 / 10.4, 4096 x 2048 12.9 / 11.9, 4096 x 1024 9.4 / 10.9.
+static int most_parts(int rows, int groups, int M, int K) {
+  const long long tiles_m = (M + 127) / 128, blocks = rows / 32 + (rows < groups ? rows : groups), slots = sm_count_of_device();
+  if ((rows + groups - 1) / groups > 24 || K < 2048 || 2 * blocks * tiles_m > slots) return 1;
+  const long long most = slots / tiles_m;
+  return int(most < SPLIT_MAX ? most : SPLIT_MAX);
+}
 static bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 }  // namespace ragged
@@ -764,8 +818,9 @@ static bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) !=
 // y [rows, N] = x [rows, K] * w[e]^T (w [groups, N, K]; transposed = 0) or dx [rows, K] = dy [rows, N] * w[e] (transposed = 1),
 // row t in group e where offsets[e] <= t < offsets[e + 1] (int32 on the device); rows of no group give zeros.  bf16,
 // contiguous, on 16-byte boundaries, N and K multiples of 8.
+// scratch: as many fp32 elements as jpb_linear_ragged_scratch_elems says (none: null), on a 16-byte boundary.
 JPB_API int jpb_linear_ragged(const void* tokens, const void* w, const int* offsets, void* out, int rows, int groups, int N, int K,
-                              int transposed, void* stream) {
+                              int transposed, float* scratch, void* stream) {
   using namespace jpb;
   using namespace jpb::ragged;
   if (rows < 0 || groups < 1 || groups > MAX_GROUPS || N <= 0 || K <= 0 || (N & 7) || (K & 7) || bad(tokens) || bad(w) || bad(out))
@@ -783,11 +838,29 @@ JPB_API int jpb_linear_ragged(const void* tokens, const void* w, const int* offs
   //   8 x 2048 x 512      mean 250: - / 18 / 20      512 (8.6 GFLOP): - / 23 / 27      1024 (17 GFLOP): - / 35 / 33
   //   8 x 1024 x 4096     mean 128 (8.6 GFLOP): - / 33 / 35    192 (13 GFLOP): - / 33 / 37    250 (17 GFLOP): - / 49 / 39
   const int mean = (rows + groups - 1) / groups;
-  if (mean <= 24) return launch_rows<1, 32>(w, tokens, p, transposed, s);
+  if (mean <= 24) {
+    const int parts = most_parts(rows, groups, p.M, p.K);
+    if (parts > 1) {
+      if (!scratch || bad(scratch)) return -JPB_ERR_BAD_ARGUMENT;
+      p.head = reinterpret_cast<int*>(scratch);
+      p.parts = scratch + 4;
+    }
+    const int rc = launch_rows<1, 32>(w, tokens, p, transposed, s);
+    if (rc || parts < 2) return rc;
+    const long long pieces = (long long)rows * (p.M >> 3);
+    ragged_parts_kernel<<<int((pieces + 255) / 256), 256, 0, s>>>(p.head, p.parts, p.D, rows, p.M);
+    return launch_result(cudaSuccess);
+  }
   const long long pairs = ((long long)rows / 256 + groups) * ((p.M + 255) / 256);
   const bool small = pairs < sm_count_of_device() / 4 || 2.0 * rows * p.M * p.K < 14e9;
   if (mean <= 96 || small) return launch_rows<1, 128>(w, tokens, p, transposed, s);
   return launch_rows<2, 256>(w, tokens, p, transposed, s);
+}
+
+JPB_API long long jpb_linear_ragged_scratch_elems(int rows, int groups, int N, int K, int transposed) {
+  if (rows <= 0 || groups <= 0) return 0;
+  const int M = transposed ? K : N, parts = jpb::ragged::most_parts(rows, groups, M, transposed ? N : K);
+  return parts > 1 ? 4 + (long long)parts * rows * M : 0;
 }
 
 // dw [groups, N, K] (fp32 or bf16), written or (fp32 only) added to = sum over each group's rows of dy [rows, N]^T x [rows, K].

@@ -58,7 +58,9 @@ def load() -> ctypes.CDLL:
     lib.jpb_sum_squares_parts.restype = _c_ll
     lib.jpb_sum_squares_partial.argtypes = [_c_int, _c_int, _c_p, _c_p, _c_p, _c_p]
     lib.jpb_sum_partials.argtypes = [_c_p, _c_int, _c_p, _c_p]
-    lib.jpb_linear_ragged.argtypes = [_c_p] * 4 + [_c_int] * 5 + [_c_p]
+    lib.jpb_linear_ragged.argtypes = [_c_p] * 4 + [_c_int] * 5 + [_c_p, _c_p]
+    lib.jpb_linear_ragged_scratch_elems.argtypes = [_c_int] * 5
+    lib.jpb_linear_ragged_scratch_elems.restype = _c_ll
     lib.jpb_linear_ragged_wgrad.argtypes = [_c_p] * 4 + [_c_int] * 6 + [_c_p]
     lib.jpb_residual_norm_fwd.argtypes = [_c_int] + [_c_p] * 9 + [_c_ll, _c_int, _c_int, _c_f, _c_f, _c_p]
     lib.jpb_residual_norm_bwd.argtypes = [_c_int] + [_c_p] * 15 + [_c_ll, _c_int, _c_int, _c_f, _c_int, _c_p]
@@ -316,8 +318,11 @@ def _linear_ragged(what, rows, w, offsets, transposed):
     offsets, rows, w = _ragged_operands(what, offsets, rows, w)
     E, N, K = w.shape
     out = _new((rows.shape[0], K if transposed else N), torch.bfloat16, rows.device)
-    _check(load().jpb_linear_ragged(rows.data_ptr(), w.data_ptr(), offsets.data_ptr(), out.data_ptr(), rows.shape[0], E, N, K,
-                                    int(transposed), _stream()), what)
+    lib = load()
+    elems = lib.jpb_linear_ragged_scratch_elems(rows.shape[0], E, N, K, int(transposed))
+    scratch = _new((elems,), torch.float32, rows.device) if elems else None
+    _check(lib.jpb_linear_ragged(rows.data_ptr(), w.data_ptr(), offsets.data_ptr(), out.data_ptr(), rows.shape[0], E, N, K,
+                                 int(transposed), _p(scratch), _stream()), what, 2 if elems else 1)
     return out
 
 

@@ -63,7 +63,8 @@ CASES = [  # group sizes, rows in front, rows behind, N, K
     ([255, 256, 257], 0, 1, 512, 256), ([300, 0, 700, 24], 0, 0, 1032, 328), ([513, 40, 600, 2, 1000, 15, 0, 290], 7, 9, 768, 384),
     ([2000, 1], 0, 0, 2304, 192), ([0, 0], 4, 3, 40, 48), ([70] * 40, 0, 0, 128, 128), ([5] * 200, 0, 0, 72, 64), ([0] * 1000 + [3] * 24, 0, 0, 16, 16),
     ([1, 1], 0, 0, 2048, 4096), ([2600, 1500], 0, 100, 4096, 1024),
-    ([1, 0, 3], 0, 1, 19208, 72), ([20, 20, 1], 2, 0, 9608, 40),
+    ([1, 0, 3], 0, 1, 19208, 72), ([20, 20, 1], 2, 0, 9608, 40), ([0, 1, 2], 1, 2, 136, 4104), ([3, 0, 30, 1], 0, 0, 4352, 200),
+    ([0, 0, 0], 2, 1, 64, 4096),
 ]
 
 

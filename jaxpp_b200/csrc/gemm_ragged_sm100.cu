@@ -89,7 +89,7 @@ struct RowsParams {
   int w_blocked;         // MN-major weights through a 4-D map {64, K, M / 64, groups}: one copy per stage
   int tiles_m;
   __nv_bfloat16* D;      // [rows, M]
-  int* head;             // blocks of up to 32 rows, or null: number of parts of the reduction, first row of a group, end of the last
+  int* head;             // single CTAs, or null: number of parts of the reduction, first row of a group, end of the last
   float* parts;          // [parts][rows, M]
   int* status;
 };
@@ -180,13 +180,13 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   }
   // few tiles: their reductions in parts, which a second kernel adds up
   int splits = 1;
-  if constexpr (BT == 32)
+  if constexpr (CG == 1)
     if (p.parts) splits = max(1, min(min(SPLIT_MAX, k_blocks / SPLIT_MIN), tile_step / max(1, blocks * tiles_m)));
   const int num_items = blocks * tiles_m * splits;
-  auto k_from = [&](int item) { return BT == 32 ? k_blocks * (item % splits) / splits : 0; };
-  auto k_to = [&](int item) { return BT == 32 ? k_blocks * (item % splits + 1) / splits : k_blocks; };
-  auto tile_of = [&](int item) { return BT == 32 ? item / splits : item; };
-  if (BT == 32 && p.parts && blockIdx.x == 0 && threadIdx.x == 64) {
+  auto k_from = [&](int item) { return CG == 1 ? k_blocks * (item % splits) / splits : 0; };
+  auto k_to = [&](int item) { return CG == 1 ? k_blocks * (item % splits + 1) / splits : k_blocks; };
+  auto tile_of = [&](int item) { return CG == 1 ? item / splits : item; };
+  if (CG == 1 && p.parts && blockIdx.x == 0 && threadIdx.x == 64) {
     p.head[0] = splits;
     p.head[1] = off[0];
     p.head[2] = off[p.groups];
@@ -325,12 +325,12 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         uint32_t v[32];
         tmem_ld_32x32(t_acc + c, v);
         tc_wait_ld();
-        if (BT == 32 && splits > 1) {
+        if (CG == 1 && splits > 1) {
           const int own = at + odd;
-          float* to = p.parts + (size_t(item % splits) * p.rows + t.t0) * p.M + t.m_blk * height + own;
+          float* to = p.parts + (size_t(item % splits) * p.rows + t.t0 + c) * p.M + t.m_blk * height + own;
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (in && j < t.n) to[size_t(j) * p.M] = __uint_as_float(v[j]);
+            if (in && c + j < t.n) to[size_t(j) * p.M] = __uint_as_float(v[j]);
           continue;
         }
 #pragma unroll
@@ -801,12 +801,28 @@ static int launch_wgrad(const void* dy, const void* x, void* D, WgradParams& p, 
   return launch(limit, ragged_wgrad_kernel<CG, BN>, CG, C::smem_bytes(p.stages, p.groups), 224, tiles, stream, ma, mb, md, p);
 }
 
-// Parts that the reduction of blocks of up to 32 rows may have: none where the tiles may be more than half the SMs, or for
-// reductions of less than 2048, where their sum costs more than they save.  One token of two experts, us, whole / in parts: 4096 x
-// 14336 59 / 45, 4096 x 4096 21 / 16, 2048 x 8192 36 / 17, 1024 x 2048 13.1 / 10.4, 4096 x 2048 12.9 / 11.9, 4096 x 1024 9.4 / 10.9.
+// Which blocks of token rows (the host knows the mean of the groups' rows, not the rows).  Measured with ragged groups, us, as 1 x 32
+// rows / 1 x 128 / a pair's 256, L2 flushed:
+//   8 x 14336 x 4096    mean 1: 115 / 141 / 115    24: 170 / 180 / 182    32: 195 / 182 / 182    96: - / 186 / 186   128: - / 209 / 190
+//   64 x 1408 x 2048    mean 1: 55 / 55 / 61       24: 86 / 82 / 86       48: 100 / 82 / 88      96: - / 88 / 90     192: - / 115 / 94
+// Small products are short of tiles, or of steps in a tile to hide its start and its store behind:
+//   8 x 2048 x 512      mean 250: - / 18 / 20      512 (8.6 GFLOP): - / 23 / 27      1024 (17 GFLOP): - / 35 / 33
+//   8 x 1024 x 4096     mean 128 (8.6 GFLOP): - / 33 / 35    192 (13 GFLOP): - / 33 / 37    250 (17 GFLOP): - / 49 / 39
+static int block_rows(int rows, int groups, int M, int K) {
+  const int mean = (rows + groups - 1) / groups;
+  if (mean <= 24) return 32;
+  const long long pairs = ((long long)rows / 256 + groups) * ((M + 255) / 256);
+  const bool small = pairs < sm_count_of_device() / 4 || 2.0 * rows * M * K < 14e9;
+  return mean <= 96 || small ? 128 : 256;
+}
+// Parts that the reduction of a single CTA's tiles may have: none where the tiles may be more than half the SMs, or for reductions
+// of less than 2048, where their sum costs more than they save.  One token of two experts, us, whole / in parts: 4096 x 14336 59 / 45,
+// 4096 x 4096 21 / 16, 2048 x 8192 36 / 17, 1024 x 2048 13.1 / 10.4, 4096 x 2048 12.9 / 11.9, 4096 x 1024 9.4 / 10.9;
+// 300 rows of four, 256 x 4096, 22 / 14; 400 rows of eight, 512 x 4096, 21 / 14.5.
 static int most_parts(int rows, int groups, int M, int K) {
-  const long long tiles_m = (M + 127) / 128, blocks = rows / 32 + (rows < groups ? rows : groups), slots = sm_count_of_device();
-  if ((rows + groups - 1) / groups > 24 || K < 2048 || 2 * blocks * tiles_m > slots) return 1;
+  const int block = block_rows(rows, groups, M, K);
+  const long long tiles_m = (M + 127) / 128, blocks = rows / block + (rows < groups ? rows : groups), slots = sm_count_of_device();
+  if (block == 256 || K < 2048 || 2 * blocks * tiles_m > slots) return 1;
   const long long most = slots / tiles_m;
   return int(most < SPLIT_MAX ? most : SPLIT_MAX);
 }
@@ -830,31 +846,20 @@ JPB_API int jpb_linear_ragged(const void* tokens, const void* w, const int* offs
   p.offsets = offsets; p.groups = groups; p.rows = rows; p.M = transposed ? K : N; p.K = transposed ? N : K;
   p.w_blocked = transposed && p.M % 64 == 0; p.D = static_cast<__nv_bfloat16*>(out); p.status = jpb_status_device_ptr();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // Which blocks (the host knows the mean of the groups' rows, not the rows).  Measured with ragged groups, us, as 1 x 32 rows /
-  // 1 x 128 / a pair's 256, L2 flushed:
-  //   8 x 14336 x 4096    mean 1: 115 / 141 / 115    24: 170 / 180 / 182    32: 195 / 182 / 182    96: - / 186 / 186   128: - / 209 / 190
-  //   64 x 1408 x 2048    mean 1: 55 / 55 / 61       24: 86 / 82 / 86       48: 100 / 82 / 88      96: - / 88 / 90     192: - / 115 / 94
-  // Small products are short of tiles, or of steps in a tile to hide its start and its store behind:
-  //   8 x 2048 x 512      mean 250: - / 18 / 20      512 (8.6 GFLOP): - / 23 / 27      1024 (17 GFLOP): - / 35 / 33
-  //   8 x 1024 x 4096     mean 128 (8.6 GFLOP): - / 33 / 35    192 (13 GFLOP): - / 33 / 37    250 (17 GFLOP): - / 49 / 39
-  const int mean = (rows + groups - 1) / groups;
-  if (mean <= 24) {
-    const int parts = most_parts(rows, groups, p.M, p.K);
-    if (parts > 1) {
-      if (!scratch || bad(scratch)) return -JPB_ERR_BAD_ARGUMENT;
-      p.head = reinterpret_cast<int*>(scratch);
-      p.parts = scratch + 4;
-    }
-    const int rc = launch_rows<1, 32>(w, tokens, p, transposed, s);
-    if (rc || parts < 2) return rc;
-    const long long pieces = (long long)rows * (p.M >> 3);
-    ragged_parts_kernel<<<int((pieces + 255) / 256), 256, 0, s>>>(p.head, p.parts, p.D, rows, p.M);
-    return launch_result(cudaSuccess);
+  const int parts = most_parts(rows, groups, p.M, p.K);
+  if (parts > 1) {
+    if (!scratch || bad(scratch)) return -JPB_ERR_BAD_ARGUMENT;
+    p.head = reinterpret_cast<int*>(scratch);
+    p.parts = scratch + 4;
   }
-  const long long pairs = ((long long)rows / 256 + groups) * ((p.M + 255) / 256);
-  const bool small = pairs < sm_count_of_device() / 4 || 2.0 * rows * p.M * p.K < 14e9;
-  if (mean <= 96 || small) return launch_rows<1, 128>(w, tokens, p, transposed, s);
-  return launch_rows<2, 256>(w, tokens, p, transposed, s);
+  const int block = block_rows(rows, groups, p.M, p.K);
+  const int rc = block == 32    ? launch_rows<1, 32>(w, tokens, p, transposed, s)
+                 : block == 128 ? launch_rows<1, 128>(w, tokens, p, transposed, s)
+                                : launch_rows<2, 256>(w, tokens, p, transposed, s);
+  if (rc || parts < 2) return rc;
+  const long long pieces = (long long)rows * (p.M >> 3);
+  ragged_parts_kernel<<<int((pieces + 255) / 256), 256, 0, s>>>(p.head, p.parts, p.D, rows, p.M);
+  return launch_result(cudaSuccess);
 }
 
 JPB_API long long jpb_linear_ragged_scratch_elems(int rows, int groups, int N, int K, int transposed) {

@@ -64,7 +64,7 @@ CASES = [  # group sizes, rows in front, rows behind, N, K
     ([2000, 1], 0, 0, 2304, 192), ([0, 0], 4, 3, 40, 48), ([70] * 40, 0, 0, 128, 128), ([5] * 200, 0, 0, 72, 64), ([0] * 1000 + [3] * 24, 0, 0, 16, 16),
     ([1, 1], 0, 0, 2048, 4096), ([2600, 1500], 0, 100, 4096, 1024),
     ([1, 0, 3], 0, 1, 19208, 72), ([20, 20, 1], 2, 0, 9608, 40), ([0, 1, 2], 1, 2, 136, 4104), ([3, 0, 30, 1], 0, 0, 4352, 200),
-    ([0, 0, 0], 2, 1, 64, 4096),
+    ([0, 0, 0], 2, 1, 64, 4096), ([40, 0, 90], 1, 0, 136, 2056), ([130, 300, 0], 0, 2, 2056, 64),
 ]
 
 

@@ -882,10 +882,11 @@ JPB_API int jpb_linear_ragged_wgrad(const void* dy, const void* x, const int* of
   WgradParams p = {};
   p.offsets = offsets; p.groups = groups; p.rows = rows; p.N = N; p.K = K; p.dy_blocked = N % 64 == 0; p.x_blocked = K % 64 == 0;
   p.out_fp32 = out_fp32; p.accumulate = accumulate; p.status = jpb_status_device_ptr();
-  // Tiles of 128 x 128 where pairs' 256 x 256 would leave most SMs without one.  Measured, us, single / pairs: 8 x 512 x 512 (32
-  // pairs) 8.2 / 10.2 with 16 rows a group, 16.4 / 18.4 with 1024, 32.8 / 36.9 with 4096; 4 x 1024 x 1024 (64 pairs) 10.2 / 10.2,
-  // 20.5 / 18.4, 53.2 / 34.8.
+  // Tiles of 128 x 128 where pairs' 256 x 256 would leave most SMs without one, and for short groups, whose time is that of the
+  // stores.  Measured, us, single / pairs: 8 x 512 x 512 (32 pairs) 8.2 / 10.2 with 16 rows a group, 16.4 / 18.4 with 1024, 32.8 / 36.9
+  // with 4096; 4 x 1024 x 1024 (64 pairs) 20.5 / 18.4 with 1024, 53.2 / 34.8 with 4096; 64 x 2896 x 1864 194 / 304 with 4; 64 x 1408 x
+  // 2048 102 / 108 with 16, 103 / 115 with 128, 156 / 145 with 256.
   const long long pairs = (long long)groups * ((N + 255) / 256) * ((K + 255) / 256);
-  if (pairs < sm_count_of_device() / 3) return launch_wgrad<1, 128>(dy, x, dw, p, s);
+  if (pairs < sm_count_of_device() / 3 || (rows + groups - 1) / groups <= 128) return launch_wgrad<1, 128>(dy, x, dw, p, s);
   return launch_wgrad<2, 256>(dy, x, dw, p, s);
 }

@@ -165,3 +165,22 @@ def test_linear_ragged_refusals_gpu():
         ops.linear_ragged(x, rnd(3, 1025, 8, 16).cuda(), torch.zeros(1026, dtype=torch.int32, device="cuda"))
     with pytest.raises((ValueError, RuntimeError)):
         ops.linear_ragged(x, w, off.cpu())
+
+
+@pytest.mark.gpu
+def test_parts_replayed_with_other_offsets():
+    """A captured product whose reductions are cut decides how from the offsets of each replay."""
+    E, N, K = 8, 1096, 4096
+    w, x = rnd(1, E, N, K, scale=0.1).cuda(), rnd(2, 2, K).cuda()
+    offsets = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.linear_ragged(x, w, offsets)
+    for counts in ([1, 1], [2], [0] * 7 + [1], [0], [0, 0, 0, 1, 1]):
+        off = bounds(counts + [0] * (E - len(counts)), 0, 0)[0]
+        offsets.copy_(torch.tensor(off, dtype=torch.int32))
+        x.copy_(rnd(sum(off), 2, K))
+        graph.replay()
+        (y, sy), _, _ = oracle(x.cpu(), w.cpu(), torch.zeros(2, N), off)
+        near(got, y, sy, K, f"replayed with {counts}")

@@ -15,6 +15,8 @@
 #include "common.cuh"
 #include "launch.cuh"
 
+#include <type_traits>
+
 namespace jpb {
 namespace ragged {
 
@@ -116,7 +118,8 @@ __device__ __forceinline__ RowsTile rows_tile(int tiles_m, const int* off, const
   return {e, m_blk, off[e] + lo, min(hi, n) - lo};
 }
 
-template <int CG, int BT, bool W_MN>
+// SPLIT: tiles may be cut along the reduction (a kernel of its own: the tests for it cost 8 x 2048 x 512 with 2000 rows 1.8 us of 14).
+template <int CG, int BT, bool W_MN, bool SPLIT>
 __global__ void __launch_bounds__(192, 1)
 ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_t, const __grid_constant__ RowsParams p) {
   using C = RowsCfg<CG, BT>;
@@ -180,13 +183,12 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   }
   // few tiles: their reductions in parts, which a second kernel adds up
   int splits = 1;
-  if constexpr (CG == 1)
-    if (p.parts) splits = max(1, min(min(SPLIT_MAX, k_blocks / SPLIT_MIN), tile_step / max(1, blocks * tiles_m)));
+  if constexpr (SPLIT) splits = max(1, min(min(SPLIT_MAX, k_blocks / SPLIT_MIN), tile_step / max(1, blocks * tiles_m)));
   const int num_items = blocks * tiles_m * splits;
-  auto k_from = [&](int item) { return CG == 1 ? k_blocks * (item % splits) / splits : 0; };
-  auto k_to = [&](int item) { return CG == 1 ? k_blocks * (item % splits + 1) / splits : k_blocks; };
-  auto tile_of = [&](int item) { return CG == 1 ? item / splits : item; };
-  if (CG == 1 && p.parts && blockIdx.x == 0 && threadIdx.x == 64) {
+  auto k_from = [&](int item) { return SPLIT ? k_blocks * (item % splits) / splits : 0; };
+  auto k_to = [&](int item) { return SPLIT ? k_blocks * (item % splits + 1) / splits : k_blocks; };
+  auto tile_of = [&](int item) { return SPLIT ? item / splits : item; };
+  if (SPLIT && blockIdx.x == 0 && threadIdx.x == 64) {
     p.head[0] = splits;
     p.head[1] = off[0];
     p.head[2] = off[p.groups];
@@ -325,7 +327,7 @@ ragged_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         uint32_t v[32];
         tmem_ld_32x32(t_acc + c, v);
         tc_wait_ld();
-        if (CG == 1 && splits > 1) {
+        if (SPLIT && splits > 1) {
           const int own = at + odd;
           float* to = p.parts + (size_t(item % splits) * p.rows + t.t0 + c) * p.M + t.m_blk * height + own;
 #pragma unroll
@@ -765,9 +767,13 @@ static int launch_rows(const void* w, const void* tokens, RowsParams& p, int w_m
   p.tiles_m = (p.M + 128 * CG - 1) / (128 * CG);
   const long long tiles = ((long long)(p.rows + BT - 1) / BT + p.groups) * (p.M / (96 * CG) + 1) * (p.parts ? SPLIT_MAX : 1);   // at most
   if (tiles > 0x7fffffffll) return -JPB_ERR_BAD_ARGUMENT;
-  static SmemLimit limit[2];
-  if (w_mn) return launch(limit[1], ragged_rows_kernel<CG, BT, true>, CG, C::SMEM_BYTES, 192, tiles, stream, mw, mt, p);
-  return launch(limit[0], ragged_rows_kernel<CG, BT, false>, CG, C::SMEM_BYTES, 192, tiles, stream, mw, mt, p);
+  auto run = [&](auto mn, auto split) {
+    static SmemLimit limit;
+    return launch(limit, ragged_rows_kernel<CG, BT, decltype(mn)::value, decltype(split)::value>, CG, C::SMEM_BYTES, 192, tiles, stream, mw, mt, p);
+  };
+  if constexpr (CG == 1)
+    if (p.parts) return w_mn ? run(std::true_type(), std::true_type()) : run(std::false_type(), std::true_type());
+  return w_mn ? run(std::true_type(), std::false_type()) : run(std::false_type(), std::false_type());
 }
 
 static int columns_map(CUtensorMap* out, const void* t, uint64_t rows, uint64_t cols, uint32_t box_cols, int blocked) {

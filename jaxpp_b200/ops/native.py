@@ -319,7 +319,8 @@ def _linear_ragged(what, rows, w, offsets, transposed):
     E, N, K = w.shape
     out = _new((rows.shape[0], K if transposed else N), torch.bfloat16, rows.device)
     lib = load()
-    elems = lib.jpb_linear_ragged_scratch_elems(rows.shape[0], E, N, K, int(transposed))
+    # (shorter reductions are never cut: no need to ask)
+    elems = lib.jpb_linear_ragged_scratch_elems(rows.shape[0], E, N, K, int(transposed)) if (N if transposed else K) >= 2048 else 0
     scratch = _new((elems,), torch.float32, rows.device) if elems else None
     _check(lib.jpb_linear_ragged(rows.data_ptr(), w.data_ptr(), offsets.data_ptr(), out.data_ptr(), rows.shape[0], E, N, K,
                                  int(transposed), _p(scratch), _stream()), what, 2 if elems else 1)

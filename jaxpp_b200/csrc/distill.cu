@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       if (valid) {
         const float zj = logit_of(j == tid ? h.z : raw_logit(row, id));
         s_z[j] = zj;
-        top_max = fmaxf(top_max, top);
+        top_max = fmaxf(top_max, top == top ? top : INFINITY);      // (a NaN is an entry too)
         ref = fmaxf(ref, zj);
       }
       const long long e = id + lead;
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
         const float logq = s_q[j] - q_sub, qj = exp2_fast(logq * LOG2E) * q_inv;
         s_q[j] = qj;
         if (at < 0) continue;
-        if (qj > 0.f) cross += qj * (logq - (s_z[j] - ref) * it);
+        if (qj != 0.f) cross += qj * (logq - (s_z[j] - ref) * it);
         mass_in += qj;
       }
     }
@@ -432,7 +432,8 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       }
     }
     const float s_t = out_t + in_t, s_1 = MODE == 0 ? s_t : out_1 + in_1, p_o = out_t / s_t;
-    const float q_o = p.lse ? fmaxf(0.f, 1.f - mass_in) : 0.f;
+    // (comparisons that keep a NaN of the teacher's: fmaxf(0, NaN) would be 0)
+    const float q_o = p.lse == nullptr || mass_in >= 1.f ? 0.f : 1.f - mass_in;
     const bool rest = q_o > 0.f && p_o > 0.f;
     const float ratio = rest ? q_o / p_o : 0.f, mass = rest ? mass_in + q_o : mass_in;
     const bool hard = label >= 0 && label < V && p.alpha < 1.f;
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       float l = 0.f;
       if (some && p.alpha > 0.f) {
         float soft = cross + q_o * log_r;
-        if (mass_in > 0.f) soft += mass_in * (log_t + (M - ref) * it - log_q);
+        if (mass_in != 0.f) soft += mass_in * (log_t + (M - ref) * it - log_q);
         l = p.alpha * p.temperature * p.temperature * soft;
       }
       if (hard) l += (1.f - p.alpha) * (log_1 - (z_label - M));

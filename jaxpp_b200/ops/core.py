@@ -971,6 +971,7 @@ _autograd("cross_entropy", _ce_autograd, _ce_setup)
 #                      (unless p leaves less than 2^-126 there, the smallest normal number: then it has no such class)
 # An id that a row lists twice has the sum of both probabilities as far as p is concerned: each entry is a term of its own.
 # Rows without an entry have no first term, rows with a label outside of 0 .. V-1 no second one (labels None: no row has it).
+# A NaN among a row's teacher_logits or in its teacher_lse makes that row's loss and gradient NaN.
 # ``distill_loss_grad`` gives the losses together with the gradient of the logits for row weights ``dloss`` that are known
 # beforehand: the logits are read once.  The gradient of ``distill_loss`` is that op too.
 # ======================================================================================
@@ -1008,7 +1009,7 @@ def _distill_ref(dloss, logits, ids, top, lse, labels, temperature, alpha):
     else:
         logq = top - lse.reshape(-1, 1)
     q = torch.where(valid, logq.exp(), torch.zeros_like(top))
-    soft = torch.where(q > 0, q * (logq - logp.gather(-1, ids)), torch.zeros_like(q)).sum(-1)
+    soft = torch.where(q != 0, q * (logq - logp.gather(-1, ids)), torch.zeros_like(q)).sum(-1)     # (a NaN stays one)
     p = logp.exp()
     mass = q.sum(-1)
     if lse is not None:

@@ -1,0 +1,61 @@
+"""Distillation loss where the plain cases of ``test_step_operators`` do not reach: broken teachers, students that leave next to
+nothing outside of the entries, and CTAs and clusters that have several rows each."""
+import math
+
+import pytest
+import torch
+
+import jaxpp_b200 as jp  # noqa: F401  (registers the ops)
+from jaxpp_b200.ops import core as ops
+
+from tests.test_step_operators import check_distill, distill_inputs, rnd
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.fixture(autouse=True)
+def status():
+    yield
+    if torch.cuda.is_available():
+        from jaxpp_b200.ops import native
+
+        if native.is_available():
+            torch.cuda.synchronize()
+            assert native.read_status() == 0, "a kernel reported a time-out or a bad argument"
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("tail", [True, False])
+@pytest.mark.parametrize("V,K", [(90, 6), (300, 200), (70000, 5)])     # a CTA a row, several entries a thread, a cluster a row
+def test_a_broken_teacher_shows(device, tail, V, K):
+    """A NaN among a row's teacher values is a NaN loss and gradient of that row, and of no other one."""
+    args = distill_inputs(7, V, K, device, torch.float32, tail, True, 2.0, torch.int64)
+    dloss = 1 + rnd(4, 7, device=device).abs()
+    dloss[5] = 0.0
+    want = ops.distill_loss_grad(dloss, *args, 2.0, 0.5)
+    logits, ids, top, lse, labels = args
+    top = top.clone()
+    top[0] = math.nan                    # nothing but NaN
+    top[2, K - 1] = math.nan             # one entry
+    top[5, 0] = math.nan                 # in a row of weight zero: no gradient all the same
+    broken = [0, 2, 5]
+    if tail:
+        lse = lse.clone()
+        lse[3] = math.nan
+        broken.append(3)
+    ids = ids.clone()
+    top[6, 1], ids[6, 1] = math.nan, -1  # no entry: what it holds does not count
+    want[0][6], want[1][6] = (t[0] for t in ops.distill_loss_grad(
+        dloss[6:], logits[6:], ids[6:], torch.where(ids[6:] < 0, 0.0, top[6:]), None if lse is None else lse[6:], labels[6:], 2.0, 0.5))
+    loss, dz = ops.distill_loss_grad(dloss, logits, ids, top, lse, labels, 2.0, 0.5)
+    again = ops.distill_loss(logits, ids, top, lse, labels, 2.0, 0.5)
+    for r in range(7):
+        if r in broken:
+            assert torch.isnan(loss[r]) and torch.isnan(again[r]), r
+            assert torch.isnan(dz[r]).all() if r != 5 else not dz[r].any(), r
+        else:
+            assert torch.isfinite(loss[r]) and torch.isfinite(again[r]), r
+            if r != 6:
+                assert torch.equal(loss[r], want[0][r]) and torch.equal(dz[r], want[1][r]), r
+    torch.testing.assert_close(loss[6], want[0][6], rtol=1e-5, atol=1e-5)     # (another number of rows may sum in another order)
+    torch.testing.assert_close(dz[6], want[1][6], rtol=1e-5, atol=1e-5)

@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
           if (twice)
             for (int k = j + 1; k < K; ++k)
               if (s_id[k] == e) qj += s_q[k];
-          float d = grad(s_z[j], ct_in) - gs * qj;
+          float d = grad(s_z[j], ct_in) - (gs != 0.f ? gs * qj : 0.f);
           if (e == label_at) d -= gh;
           dz[e - lead] = from_f<T>(d);
         }

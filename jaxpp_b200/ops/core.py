@@ -970,7 +970,8 @@ _autograd("cross_entropy", _ce_autograd, _ce_setup)
 #                      teacher_lse), and what q leaves is held against what p leaves outside of the entries, as one more class
 #                      (unless p leaves less than 2^-126 there, the smallest normal number: then it has no such class)
 # An id that a row lists twice has the sum of both probabilities as far as p is concerned: each entry is a term of its own.
-# Rows without an entry have no first term, rows with a label outside of 0 .. V-1 no second one (labels None: no row has it).
+# Rows without an entry have no first term, rows with a label outside of 0 .. V-1 no second one (labels None: no row has it);
+# a term whose factor alpha or 1 - alpha is 0 is left out, whatever its tensors hold.
 # A NaN among a row's teacher_logits or in its teacher_lse makes that row's loss and gradient NaN.
 # ``distill_loss_grad`` gives the losses together with the gradient of the logits for row weights ``dloss`` that are known
 # beforehand: the logits are read once.  The gradient of ``distill_loss`` is that op too.
@@ -1001,7 +1002,7 @@ def _distill_ref(dloss, logits, ids, top, lse, labels, temperature, alpha):
     ids, top = ids.reshape(z.shape[0], ids.shape[-1]).long(), _f32(top).reshape(z.shape[0], top.shape[-1]) / t
     ninf = torch.full((), float("-inf"), device=z.device)
     valid = (ids >= 0) & (ids < V) & (top != ninf)
-    some = valid.any(-1, keepdim=True)
+    some = valid.any(-1, keepdim=True) & (alpha > 0)
     ids, top = ids.masked_fill(~valid, 0), torch.where(valid, top, ninf)
     logp = torch.log_softmax(z / t, -1)
     if lse is None:

@@ -59,3 +59,24 @@ def test_a_broken_teacher_shows(device, tail, V, K):
                 assert torch.equal(loss[r], want[0][r]) and torch.equal(dz[r], want[1][r]), r
     torch.testing.assert_close(loss[6], want[0][6], rtol=1e-5, atol=1e-5)     # (another number of rows may sum in another order)
     torch.testing.assert_close(dz[6], want[1][6], rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_terms_without_weight_are_left_out(device):
+    """alpha 0 is the cross entropy alone and alpha 1 the divergence alone, whatever the other one's tensors hold."""
+    logits, ids, top, lse, labels = distill_inputs(4, 60, 5, device)
+    ones = torch.ones(4, device=device)
+    logits[1, ids[1, 0]] = -math.inf                 # the divergence of this row is infinite
+    labels[1], labels[2] = ids[1, 1], -1
+    want = ops.distill_loss_grad(ones, logits, ids, top, lse, labels, 1.0, 0.0)
+    got = ops.distill_loss_grad(ones, logits, ids, torch.full_like(top, math.nan), lse, labels, 2.0, 0.0)
+    for p, q in zip(got, want):
+        assert torch.isfinite(q).all()
+        torch.testing.assert_close(p, q, rtol=1e-6, atol=1e-6)
+    plain, _ = ops.cross_entropy(logits, labels.clamp(min=0))
+    torch.testing.assert_close(got[0], torch.where(labels < 0, 0.0, plain), rtol=1e-6, atol=1e-6)
+    logits[1] = logits[0]
+    logits[3, labels[3]] = -math.inf                 # an infinite cross entropy
+    ids[3] = (labels[3] + 1 + torch.arange(5, device=device)) % 60
+    loss, dz = ops.distill_loss_grad(ones, logits, ids, top, None, labels, 1.0, 1.0)
+    assert torch.isfinite(loss).all() and torch.isfinite(dz).all()

@@ -146,12 +146,15 @@ struct PartSums {
 
 // MODE: exponentials of a gradient and a loss in which 0 only one temperature counts, 1 / 2 both and t = 2 / 4, 3 both, any t
 template <int MODE>
-__device__ __forceinline__ float plain_exp(float e, float f, float m1) {   // exp(f - m) from e = exp((f - m) / t)
+__device__ __forceinline__ float plain_exp(float e, float f, float k1, float m1) {   // exp(f - m) from e = exp((f - m) / t)
   if (MODE == 0) return e;
   if (MODE == 1) return e * e;
   if (MODE == 2) { const float s = e * e; return s * s; }
-  return exp2_fast(fmaf(f, LOG2E, -m1));
+  return exp2_fast(fmaf(f, k1, -m1));
 }
+// The factor k (log2(e) / t or log2(e)) of exponents relative to m, or 1 where m * k could leave fp32's range (a part of a row that is
+// masked with the type's lowest value has no other maximum): logits of that size are equal or so far apart that any factor does.
+__device__ __forceinline__ float factor(float m, float k) { return fabsf(m) > 1.2676506e30f ? 1.f : k; }    // 2^100
 __device__ __forceinline__ F2 exp2_pair(F2 x) { return f2(exp2_fast(x.lo()), exp2_fast(x.hi())); }
 template <typename T, bool GRAD, int MODE, int THREADS>
 __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const __grid_constant__ DistillParams p) {
@@ -248,8 +251,9 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
   }
   // The exponentials relative to m are 2^(z * it2 - fl(m * it2)): all of them too large by 2^off, off being what the rounding of
   // m * it2 leaves (and likewise for the plain ones).  Ratios do not see it; the logarithm of a sum takes it off.
-  auto off_t = [&](float m) { return fmaf(m, it2, -(m * it2)); };
-  auto off_1 = [&](float m) { return MODE == 1 ? 2.f * off_t(m) : MODE == 2 ? 4.f * off_t(m) : MODE == 3 ? fmaf(m, LOG2E, -(m * LOG2E)) : off_t(m); };
+  auto off_by = [&](float m, float k) { return fmaf(m, factor(m, k), -(m * factor(m, k))); };
+  auto off_t = [&](float m) { return off_by(m, it2); };
+  auto off_1 = [&](float m) { return MODE == 1 ? 2.f * off_t(m) : MODE == 2 ? 4.f * off_t(m) : MODE == 3 ? off_by(m, LOG2E) : off_t(m); };
   Ahead next;
   if (row0 < p.rows) {
     next = ahead_ids(row0, begin);
@@ -361,9 +365,9 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
     const Vec<T>* piece = reinterpret_cast<const Vec<T>*>(buf);
     float m = ref;
     for (int attempt = 0;; ++attempt) {
-      const float mt = m * it2, m1 = m * LOG2E;
+      const float km = factor(m, it2), k1m = factor(m, LOG2E), mt = m * km, m1 = m * k1m;
       F2 sum_t = f2(0.f), sum_1 = f2(0.f);
-      const F2 k = f2(it2), k1 = f2(LOG2E), at = f2(-mt), at1 = f2(-m1);
+      const F2 k = f2(km), k1 = f2(k1m), at = f2(-mt), at1 = f2(-m1);
 #pragma unroll 2
       for (int i = tid; i < q.pieces; i += THREADS) {
         F2 f[VN / 2];
@@ -380,9 +384,9 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       in_t = in_1 = 0.f;
       for (int j = tid, i = 0; j < K; j += THREADS, ++i)
         if (owner >> i & 1) {
-          const float e = exp2_fast(fmaf(s_z[j], it2, -mt));
+          const float e = exp2_fast(fmaf(s_z[j], km, -mt));
           in_t += e;
-          if (MODE != 0) in_1 += plain_exp<MODE>(e, s_z[j], m1);
+          if (MODE != 0) in_1 += plain_exp<MODE>(e, s_z[j], k1m, m1);
         }
       float acc[8] = {sum_t.lo() + sum_t.hi(), sum_1.lo() + sum_1.hi(), in_t, in_1, attempt ? 0.f : cross, attempt ? 0.f : mass_in, 0.f, 0.f};
       if (!GRAD) fence_proxy_async();   // elements of the row were written here, the next row comes by the bulk-copy unit
@@ -444,10 +448,10 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
     const bool zero = now.g == 0.f || (gs == 0.f && gh == 0.f);
     float ct = gs != 0.f ? gs * (mass - ratio) / s_t : 0.f, ct_in = gs != 0.f ? gs * mass / s_t : 0.f, c1 = gh != 0.f ? gh / s_1 : 0.f;
     if (MODE == 0) { ct += c1; ct_in += c1; c1 = 0.f; }
-    const float Mt = M * it2, M1 = M * LOG2E;
+    const float kM = factor(M, it2), k1M = factor(M, LOG2E), Mt = M * kM, M1 = M * k1M;
     auto grad = [&](float f, float c) {
-      const float e = exp2_fast(fmaf(f, it2, -Mt));
-      return MODE == 0 ? c * e : fmaf(c, e, c1 * plain_exp<MODE>(e, f, M1));
+      const float e = exp2_fast(fmaf(f, kM, -Mt));
+      return MODE == 0 ? c * e : fmaf(c, e, c1 * plain_exp<MODE>(e, f, k1M, M1));
     };
     if constexpr (GRAD) {
       uint8_t* out = static_cast<uint8_t*>(p.dlogits) + q.lo * 16;
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       if (zero) {
         for (int i = a + tid; i < b; i += THREADS) *reinterpret_cast<uint4*>(out + size_t(i) * 16) = make_uint4(0, 0, 0, 0);
       } else {
-        const F2 k = f2(it2), k1 = f2(LOG2E), at = f2(-Mt), at1 = f2(-M1), wt = f2(ct), w1 = f2(c1);
+        const F2 k = f2(kM), k1 = f2(k1M), at = f2(-Mt), at1 = f2(-M1), wt = f2(ct), w1 = f2(c1);
 #pragma unroll 2
         for (int i = a + tid; i < b; i += THREADS) {
           F2 f[VN / 2];

@@ -80,3 +80,29 @@ def test_terms_without_weight_are_left_out(device):
     ids[3] = (labels[3] + 1 + torch.arange(5, device=device)) % 60
     loss, dz = ops.distill_loss_grad(ones, logits, ids, top, None, labels, 1.0, 1.0)
     assert torch.isfinite(loss).all() and torch.isfinite(dz).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [900, 70000])
+@pytest.mark.parametrize("t,alpha", [(1.0, 0.5), (2.0, 0.5), (4.0, 1.0), (1.5, 0.75), (0.5, 0.5)])
+def test_masks_of_the_lowest_value(device, dtype, V, t, alpha):
+    """A vocabulary masked with the type's lowest value, whole parts of a row's cluster with nothing else among them, counts as
+    one masked with -inf; a row of nothing else is a row of equal logits."""
+    logits, ids, top, lse, labels = distill_inputs(5, V, 6, device, dtype, True, alpha < 1, t, torch.int64)
+    ids[:] = torch.arange(6, device=device) + 11
+    if labels is not None:
+        labels[:] = torch.arange(9, 14, device=device)
+    lowest = torch.finfo(dtype).min if t >= 1 else torch.finfo(dtype).min * t      # (no overflow by the temperature)
+    logits[1, V // 2:] = lowest
+    logits[2, 17:] = lowest
+    logits[3, :] = lowest
+    logits[4, :9], logits[4, V // 3:] = lowest, -math.inf
+    loss, dz = check_distill(device, logits, ids, top, lse, labels, t, alpha)
+    assert not dz[1, V // 2:].any() and not dz[2, 17:].any() and not dz[4, V // 3:].any()
+    other = torch.where(logits == lowest, -math.inf, logits.float()).to(dtype)
+    keep = [0, 1, 2, 4]
+    for tail in (lse, None):
+        got = ops.distill_loss_grad(torch.ones(5, device=device), logits, ids, top, tail, labels, t, alpha)
+        want = ops.distill_loss_grad(torch.ones(5, device=device), other, ids, top, tail, labels, t, alpha)
+        assert torch.equal(got[0][keep], want[0][keep]) and torch.equal(got[1][keep], want[1][keep])

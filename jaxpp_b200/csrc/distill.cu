@@ -139,10 +139,14 @@ __device__ __forceinline__ float piece_max(const Vec<__nv_bfloat16>& v) {
   return fmaxf(f.x, f.y);
 }
 
-// What a CTA tells the others about its part of a row; the sums of exponentials are relative to m.
+// What a CTA tells the others about its part of a row; the sums of exponentials are relative to m, out_t to m_out.
 struct PartSums {
-  float m, out_t, out_1, in_t, in_1, cross, mass, label;
+  float m, m_out, out_t, in_t, s_1, cross, mass, label;
 };
+// Below this share of the largest exponential the sum over the elements outside of S is taken relative to its own maximum: it then
+// keeps its digits down to the smallest p_o that counts, and 1 / p_o stays out of the gradient's coefficients (below it, a weight of
+// 1e22 still fits).  One pass more over such a row.
+constexpr float THIN = 9.094947017729282e-13f;       // 2^-40
 
 // MODE: exponentials of a gradient and a loss in which 0 only one temperature counts, 1 / 2 both and t = 2 / 4, 3 both, any t
 template <int MODE>
@@ -404,38 +408,69 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       if (mx == -INFINITY) break;       // nothing here but -inf: sums of zero, relative to anything
       m = mx;
     }
+    float m_out = m;
+    if (p.lse != nullptr && out_t < THIN) {
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int i = tid; i < q.pieces; i += THREADS) mx = fmaxf(mx, piece_max(piece[i]));
+      mx = reduce.template one<true>(mx);
+      if (mx != -INFINITY) {            // (else there is nothing outside)
+        const float km = factor(mx, it2), mt = mx * km;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int i = tid; i < q.pieces; i += THREADS) {
+          F2 f[VN / 2];
+          to_pairs(piece[i], f);
+#pragma unroll
+          for (int j = 0; j < VN / 2; ++j) sum += exp2_fast(fmaf(f[j].lo(), km, -mt)) + exp2_fast(fmaf(f[j].hi(), km, -mt));
+        }
+        out_t = reduce.template one<false>(sum);
+        m_out = mx;
+      }
+    }
     if (!GRAD && tid == THREADS - 32 && more) fetch(begin + step_bytes);   // (all have read it)
     // ---- together with the other parts ----
-    float M = m;
+    float M = m, M_out = m_out, s_1 = out_1 + in_1;
     if (C > 1) {
       PartSums* mine = &parts[turn];
-      if (tid == 0) *mine = {m, out_t, out_1, in_t, in_1, cross, mass_in, label_here ? z_own : -INFINITY};
+      if (tid == 0) *mine = {m, m_out, out_t, in_t, s_1, cross, mass_in, label_here ? z_own : -INFINITY};
       __syncwarp();
       cluster_sync();
       // lane c reads part c (lanes go round), and the parts are added up across lanes: one trip to the other SMs
       uint32_t at;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(tid & (C - 1)));
       PartSums o;
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.m), "=f"(o.out_t), "=f"(o.out_1), "=f"(o.in_t) : "r"(at) : "memory");
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.in_1), "=f"(o.cross), "=f"(o.mass), "=f"(o.label) : "r"(at + 16) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.m), "=f"(o.m_out), "=f"(o.out_t), "=f"(o.in_t) : "r"(at) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.s_1), "=f"(o.cross), "=f"(o.mass), "=f"(o.label) : "r"(at + 16) : "memory");
       M = o.m;
-      for (int x = 1; x < C; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+      M_out = o.out_t > 0.f ? o.m_out : -INFINITY;     // (a part with nothing outside has no say)
+      for (int x = 1; x < C; x <<= 1) {
+        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+        M_out = fmaxf(M_out, __shfl_xor_sync(0xffffffffu, M_out, x));
+      }
+      if (M_out == -INFINITY) M_out = M;
       const float et = exp2_fast((o.m - M) * it2 + (off_t(M) - off_t(o.m))), e1 = exp2_fast((o.m - M) * LOG2E + (off_1(M) - off_1(o.m)));
-      out_t = o.out_t * et; out_1 = o.out_1 * e1; in_t = o.in_t * et; in_1 = o.in_1 * e1;
+      const float eo = o.m_out == o.m && M_out == M ? et : exp2_fast((o.m_out - M_out) * it2 + (off_t(M_out) - off_t(o.m_out)));
+      out_t = o.out_t == 0.f ? 0.f : o.out_t * eo; in_t = o.in_t * et; s_1 = o.s_1 * e1;
       cross = o.cross; mass_in = o.mass; z_label = o.label;
       for (int x = 1; x < C; x <<= 1) {
         out_t += __shfl_xor_sync(0xffffffffu, out_t, x);
         in_t += __shfl_xor_sync(0xffffffffu, in_t, x);
-        if (MODE != 0) {
-          out_1 += __shfl_xor_sync(0xffffffffu, out_1, x);
-          in_1 += __shfl_xor_sync(0xffffffffu, in_1, x);
-        }
+        if (MODE != 0) s_1 += __shfl_xor_sync(0xffffffffu, s_1, x);
         cross += __shfl_xor_sync(0xffffffffu, cross, x);
         mass_in += __shfl_xor_sync(0xffffffffu, mass_in, x);
         z_label = fmaxf(z_label, __shfl_xor_sync(0xffffffffu, z_label, x));
       }
     }
-    const float s_t = out_t + in_t, s_1 = MODE == 0 ? s_t : out_1 + in_1, p_o = out_t / s_t;
+    const bool thin = M_out != M;                      // out_t has a reference of its own
+    float s_t = out_t + in_t, p_o = out_t / s_t, shift = 0.f;
+    if (thin) {
+      shift = (M_out - M) * it2 + (off_t(M) - off_t(M_out));
+      s_t = fmaf(out_t, exp2_fast(shift), in_t);
+      const float l = shift + __log2f(out_t) - __log2f(s_t);
+      p_o = l >= -126.f ? exp2_fast(l) : l == l ? 0.f : l;
+    }
+    if (MODE == 0) s_1 = s_t;
     // (comparisons that keep a NaN of the teacher's: fmaxf(0, NaN) would be 0)
     const float q_o = p.lse == nullptr || mass_in >= 1.f ? 0.f : 1.f - mass_in;
     const bool rest = q_o > 0.f && p_o > 0.f;
@@ -447,19 +482,29 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
     // gradient = ct * exp((z - M) / t) + c1 * exp(z - M); a row of weight zero has none, whatever it holds
     const bool zero = now.g == 0.f || (gs == 0.f && gh == 0.f);
     float ct = gs != 0.f ? gs * (mass - ratio) / s_t : 0.f, ct_in = gs != 0.f ? gs * mass / s_t : 0.f, c1 = gh != 0.f ? gh / s_1 : 0.f;
-    if (MODE == 0) { ct += c1; ct_in += c1; c1 = 0.f; }
+    if (MODE == 0) { ct += c1; ct_in += c1; }
+    // Outside of S: relative to M_out, where the plain exponential is a power of the softened one too.
+    float c1_out = MODE == 0 ? 0.f : c1;
+    if (thin) {
+      ct = gs != 0.f ? gs * ((mass * p_o - (rest ? q_o : 0.f)) / out_t) : 0.f;
+      if (MODE == 0) ct = fmaf(c1, exp2_fast(shift), ct);
+      if (MODE == 1) c1_out *= exp2_fast(2.f * shift);
+      if (MODE == 2) c1_out *= exp2_fast(4.f * shift);
+    }
     const float kM = factor(M, it2), k1M = factor(M, LOG2E), Mt = M * kM, M1 = M * k1M;
-    auto grad = [&](float f, float c) {
-      const float e = exp2_fast(fmaf(f, kM, -Mt));
+    const float kM_out = factor(M_out, it2), Mt_out = M_out * kM_out;
+    auto grad_of = [&](float f, float c, float c1, float k, float Mt) {
+      const float e = exp2_fast(fmaf(f, k, -Mt));
       return MODE == 0 ? c * e : fmaf(c, e, c1 * plain_exp<MODE>(e, f, k1M, M1));
     };
+    auto grad_out = [&](float f) { return grad_of(f, ct, c1_out, kM_out, Mt_out); };
     if constexpr (GRAD) {
       uint8_t* out = static_cast<uint8_t*>(p.dlogits) + q.lo * 16;
       const int a = first_whole(q), b = last_whole(q);
       if (zero) {
         for (int i = a + tid; i < b; i += THREADS) *reinterpret_cast<uint4*>(out + size_t(i) * 16) = make_uint4(0, 0, 0, 0);
       } else {
-        const F2 k = f2(kM), k1 = f2(k1M), at = f2(-Mt), at1 = f2(-M1), wt = f2(ct), w1 = f2(c1);
+        const F2 k = f2(kM_out), k1 = f2(k1M), at = f2(-Mt_out), at1 = f2(-M1), wt = f2(ct), w1 = f2(c1_out);
 #pragma unroll 2
         for (int i = a + tid; i < b; i += THREADS) {
           F2 f[VN / 2];
@@ -480,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
       const int ae = a * VN, be = max(ae, b * VN);
       for (int i = tid; i < ae + n - be; i += THREADS) {
         const int v = i < ae ? i : be + i - ae;
-        if (v >= v_lo && v < v_hi) dz[v - lead] = from_f<T>(zero ? 0.f : grad(to_f(elem[v]), ct));
+        if (v >= v_lo && v < v_hi) dz[v - lead] = from_f<T>(zero ? 0.f : grad_out(to_f(elem[v])));
       }
       fence_proxy_async();
       __syncthreads();            // the row is done with; the elements of S and the label's are written again
@@ -493,14 +538,14 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) distill_kernel(const _
           if (twice)
             for (int k = j + 1; k < K; ++k)
               if (s_id[k] == e) qj += s_q[k];
-          float d = grad(s_z[j], ct_in) - (gs != 0.f ? gs * qj : 0.f);
+          float d = grad_of(s_z[j], ct_in, c1, kM, Mt) - (gs != 0.f ? gs * qj : 0.f);
           if (e == label_at) d -= gh;
           dz[e - lead] = from_f<T>(d);
         }
         if (tid == THREADS - 1 && label_here && gh != 0.f) {
           bool listed = false;
           for (int k = 0; k < K; ++k) listed |= s_id[k] == label_at;
-          if (!listed) dz[label_at - lead] = from_f<T>(grad(z_own, ct) - gh);
+          if (!listed) dz[label_at - lead] = from_f<T>(grad_out(z_own) - gh);
         }
       }
     }

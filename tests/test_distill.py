@@ -8,7 +8,7 @@ import torch
 import jaxpp_b200 as jp  # noqa: F401  (registers the ops)
 from jaxpp_b200.ops import core as ops
 
-from tests.test_step_operators import check_distill, distill_inputs, rnd
+from tests.test_step_operators import U, check, check_distill, distill_exact, distill_inputs, distill_slack, rnd
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -106,3 +106,44 @@ def test_masks_of_the_lowest_value(device, dtype, V, t, alpha):
         got = ops.distill_loss_grad(torch.ones(5, device=device), logits, ids, top, tail, labels, t, alpha)
         want = ops.distill_loss_grad(torch.ones(5, device=device), other, ids, top, tail, labels, t, alpha)
         assert torch.equal(got[0][keep], want[0][keep]) and torch.equal(got[1][keep], want[1][keep])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,t,alpha", [(900, 4.0, 1.0), (900, 1.0, 0.5), (900, 2.0, 0.5), (900, 1.5, 0.75), (70000, 4.0, 0.5), (70000, 1.0, 1.0)])
+def test_students_that_leave_next_to_nothing(device, dtype, V, t, alpha):
+    """The teacher keeps mass outside of the entries and the student almost none, with weights as a scaled loss has them: what is
+    outside has a gradient of the size of the teacher's rest, however small the student's is.  Tolerances as in ``check_distill``;
+    what is flushed to zero on the way is below the smallest normal number, times the weight."""
+    gaps = [20.0, 26.0, 27.0, 28.0, 29.0, 45.0, 60.0, 78.0, 83.0, 91.0, 120.0]     # 2^-40 is 27.7 nats, 2^-126 is 87.3
+    rows, K = len(gaps), 5
+    logits, ids, top, lse, labels = distill_inputs(rows, V, K, device, torch.float32, True, alpha < 1, t, torch.int64)
+    first = V // 2 - 2
+    ids[:] = torch.arange(first, first + K, device=device)
+    outside = torch.ones(V, dtype=torch.bool, device=device)
+    outside[first:first + K] = False
+    logits[:, first:first + K] = rnd(1, rows, K, device=device)
+    tail = rnd(2, rows, V, device=device) * 0.5
+    for r, gap in enumerate(gaps):
+        # the outside as a whole lies `gap` below: its elements by the logarithm of their number more, but for the 120 (nothing
+        # is left) and the 91, whose sum of elements below 2^-126 is above it
+        down = gap if gap in (91.0, 120.0) else gap + math.log(V - K)
+        if gap == 91.0 and V < 1000:
+            down = 88.5
+        logits[r, outside] = t * (tail[r, outside] * 0.5 - down)
+    logits[5, 3:first // 2] = -800.0 * t
+    logits = logits.to(dtype)
+    lse = torch.logsumexp(top.float() / t, -1) + torch.linspace(0.01, 2.0, rows, device=device)      # q leaves 1 % to 86 %
+    dloss = torch.tensor([1.0, -1024.0, 3.0e4, 1.0e6] * 3, device=device)[:rows]
+    dloss[7:9] = 4096.0
+    if labels is not None:
+        labels[0], labels[5], labels[6], labels[8] = first, first + 1, 7, V - 1
+    z = logits.double().cpu() / t
+    left = torch.logsumexp(z[:, outside.cpu()], -1) - torch.logsumexp(z, -1)
+    assert (left + 126 * math.log(2)).abs().min() > 0.2           # (on the border either answer would be right)
+    el, eg, size = distill_exact(dloss, logits, ids, top, lse, labels, t, alpha)
+    rel = distill_slack(logits, t)
+    loss, dz = ops.distill_loss_grad(dloss, logits, ids, top, lse, labels, t, alpha)
+    check(loss, el, rel * 2 * max(1.0, t * t) * (1 + el.abs()) + 200 * U)
+    check(ops.distill_loss(logits, ids, top, lse, labels, t, alpha), el, rel * 2 * max(1.0, t * t) * (1 + el.abs()) + 200 * U)
+    check(dz, eg, 2 * rel * size + 2.0 ** -126 * (1 + t * dloss.abs().double().cpu()[:, None]))

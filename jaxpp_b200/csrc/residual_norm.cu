@@ -472,7 +472,8 @@ __global__ void __launch_bounds__(RN_THREADS, 1) residual_norm_bwd_kernel(const 
     const uint32_t sy = operand(s, 0), sx = operand(s, 1), sdh = operand(s, 2), sdr = operand(s, at_dr);
     // dR = A - k1 * r = dr + rstd2 * u - k1 * rstd1 * c - k1 * scale * x;   dy = rstd1 * gate * w_post * dR - k2 * y
     const float k1 = t.rstd2 * t.rstd2 * sums[0] * inv_d;
-    const float k2 = post ? t.rstd1 * t.rstd1 * t.rstd1 * (sums[1] - k1 * sums[2]) * inv_d : 0.f;
+    // (the sums are of the size of y: one factor at a time keeps the products within fp32 wherever the mean of y^2 is)
+    const float k2 = post ? t.rstd1 * (t.rstd1 * (t.rstd1 * ((sums[1] - k1 * sums[2]) * inv_d))) : 0.f;
     const F2 r1 = f2(t.rstd1), r2 = f2(t.rstd2), mc = f2(-k1 * t.rstd1), mx = f2(-k1 * p.scale), my = f2(-k2);
     T* const dx = static_cast<T*>(p.dx) + size_t(row) * p.d + size_t(tid) * VN;
     T* const dy = static_cast<T*>(p.dy) + size_t(row) * p.d + size_t(tid) * VN;

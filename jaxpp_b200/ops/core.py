@@ -59,7 +59,7 @@ def _define(schema: str, ref_impl, fake_impl, native_name: str | None = None, ch
     if native_name is None:
         impl = ref_impl
     else:
-        def impl(*args, __ref=ref_impl, __nn=native_name, __check=check):
+        def impl(*args, __ref=ref_impl, __fake=fake_impl, __nn=native_name, __check=check):
             if __check is not None:
                 __check(*args)
             for first in args:
@@ -67,7 +67,7 @@ def _define(schema: str, ref_impl, fake_impl, native_name: str | None = None, ch
                     break
             if _use_native(first):
                 return getattr(_native(), __nn)(*args)
-            return __ref(*args)
+            return (__fake if first.is_meta else __ref)(*args)      # (a direct call has not been sorted by device)
 
     _lib.impl(name, impl, "CompositeExplicitAutograd")
     if check is None:
@@ -84,8 +84,8 @@ def _define(schema: str, ref_impl, fake_impl, native_name: str | None = None, ch
 
 class _Direct:
     """An op whose eager calls go straight to its implementation where there is nothing for the dispatcher to do: plain tensors,
-    no gradient to record, no trace or transform under way.  The dispatcher's way to an op implemented in Python takes 15 us and
-    more, as long as many of these kernels run; everything else goes through it."""
+    no gradient to record, no compilation, trace, transform, mode or profile under way.  The dispatcher's way to an
+    op implemented in Python takes 15 us and more, as long as many of these kernels run; everything else goes through it."""
 
     def __init__(self, packet):
         self.packet, self.default = packet, packet.default
@@ -93,7 +93,10 @@ class _Direct:
         self.__name__ = str(packet)
 
     def __call__(self, *args, **kwargs):
-        if kwargs or _dispatch_modes() or _functorch_stack() is not None or _forward_ad._current_level >= 0:
+        # (compilation first: its tracer does not take the other questions; the arguments' own __torch_function__, as a symbolic
+        # trace's proxies have it, and the modes of that kind are one question)
+        if _compiling() or kwargs or _takes_over(args) or _dispatch_modes() or _functorch_stack() is not None \
+                or _forward_ad._current_level >= 0 or _profiling():
             return self.packet(*args, **kwargs)
         grad = torch.is_grad_enabled()
         for a in args:
@@ -106,7 +109,9 @@ class _Direct:
         return self._impl(*args)
 
 
+_compiling, _takes_over = torch.compiler.is_dynamo_compiling, torch.overrides.has_torch_function
 _dispatch_modes, _functorch_stack = torch._C._len_torch_dispatch_stack, torch._C._functorch.peek_interpreter_stack
+_profiling = torch._C._autograd._profiler_enabled
 
 
 def _autograd(name: str, backward, setup_context):

@@ -403,7 +403,7 @@ def _check_expert_order(top_i: Tensor, n_experts: int):
 def _expert_order_impl(top_i: Tensor, n_experts: int):
     _check_expert_order(top_i, n_experts)
     if not ops._use_native(top_i):
-        return _expert_order_ref(top_i, n_experts)
+        return (_expert_order_fake if top_i.is_meta else _expert_order_ref)(top_i, n_experts)
     lib, native = _native()
     native._here("expert_order", top_i)
     flat = top_i.contiguous()

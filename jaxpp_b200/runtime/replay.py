@@ -37,7 +37,8 @@ EAGER_CALLS = 2                  # calls that run op by op first: allocator, ker
 _pool_lock = threading.Lock()
 _pool_bytes = [0]
 _FLAGS = [v for v in vars(config).values() if isinstance(v, config.OverwriteableVar)]
-_MOE_OPS = {"router", "route_tokens", "route_tokens_bwd", "slots", "dispatch_rows", "combine_rows", "combine_rows_bwd"}
+_MOE_OPS = {"router", "route_tokens", "route_tokens_bwd", "slots", "expert_order", "dispatch_rows", "combine_rows",
+            "combine_rows_bwd"}
 # ATen ops that synchronise or allocate by value for some arguments although their schemas do not say so
 _ATEN_REFUSED = {"index", "index_put", "index_put_", "_index_put_impl_", "masked_select", "nonzero", "repeat_interleave", "item",
                  "_local_scalar_dense", "bincount", "lift_fresh", "lift_fresh_copy", "pin_memory", "is_pinned"}

@@ -75,3 +75,13 @@ def test_what_a_recording_covers():
     assert rec.covers(overlapping)              # nothing is updated in place
     rec.written = [0]
     assert rec.covers(ok) and not rec.covers(overlapping)
+
+
+def test_ops_of_dropless_layers_can_be_recorded():
+    """They synchronise nothing: the groups' sizes stay on the device."""
+    from jaxpp_b200.parallel import moe  # noqa: F401  (registers the ops)
+
+    b, m = torch.ops.b200, torch.ops.b200moe
+    for op in (m.route_tokens, m.expert_order, m.dispatch_rows, b.linear_ragged, b.linear_ragged_dgrad, b.linear_ragged_wgrad, m.combine_rows,
+               m.combine_rows_bwd, m.route_tokens_bwd, b.residual_norm, b.residual_norm_bwd, b.distill_loss, b.distill_loss_grad):
+        assert replay._capturable(op.default), op

@@ -230,3 +230,26 @@ def test_the_flag_holds_for_each_call():
     for _ in range(3):
         late(x, w)
     assert _replay(late).recording is not None
+
+
+def test_dropless_experts_and_a_teacher():
+    """The step of a student with sandwich norms and dropless experts, trained against a teacher's top logits, is recorded too."""
+    cfg = tf.ModelConfig("mixtral", vocab=1000, d_model=256, n_layers=2, n_heads=4, n_kv_heads=2, ffn=320, seq=65, n_experts=8, top_k=2,
+                         dropless=True, sandwich_norm=True, residual_scale=0.9, residual_gate=0.7)
+    schedule, device = jp.Std1F1B(1), torch.device("cuda", 0)
+    make = lambda: jp.mpmd_jit_with_loop(lt.make_train_step(cfg, schedule, lt.Hyper(distill_alpha=0.7, distill_temperature=2.0)), _mesh())
+    graph, eager = make(), make()
+    a, b = lt.init_state(cfg, schedule, device, seed=3), lt.init_state(cfg, schedule, device, seed=3)
+    g = torch.Generator().manual_seed(0)
+    for i in range(5):
+        # distinct tokens, as above; other picks, and so other groups, in every step
+        tok = torch.stack([torch.randperm(cfg.vocab, generator=g)[:2 * 66].view(2, 66) for _ in range(2)])
+        logits = torch.randn(2, 2, 65, cfg.vocab, generator=g) * 2
+        top, ids = logits.topk(12, -1)
+        batch = [t.contiguous().to(device) for t in (tok[:, :, :-1], tok[:, :, 1:], ids, top.bfloat16(), torch.logsumexp(logits / 2.0, -1))]
+        a, la = graph(a, *batch)
+        with config.step_graphs.set(False):
+            b, lb = eager(b, *batch)
+        for x, y in zip(_tensors((a, la)), _tensors((b, lb))):
+            assert torch.equal(x, y)
+    assert _replay(graph).recording is not None and _replay(eager).recording is None

@@ -147,3 +147,105 @@ def test_students_that_leave_next_to_nothing(device, dtype, V, t, alpha):
     check(loss, el, rel * 2 * max(1.0, t * t) * (1 + el.abs()) + 200 * U)
     check(ops.distill_loss(logits, ids, top, lse, labels, t, alpha), el, rel * 2 * max(1.0, t * t) * (1 + el.abs()) + 200 * U)
     check(dz, eg, 2 * rel * size + 2.0 ** -126 * (1 + t * dloss.abs().double().cpu()[:, None]))
+
+
+# ---- several rows to a CTA or a cluster ------------------------------------------------------------------------------------------
+def exact_rows(dloss, logits, ids, top, lse, labels, t, alpha):
+    """``distill_exact`` for all rows at once, where the tensors are."""
+    z, V = logits.double(), logits.shape[-1]
+    valid = (ids >= 0) & (ids < V) & (top != -math.inf)
+    at = ids.long().masked_fill(~valid, 0)
+    teacher = (top.double() / t).masked_fill(~valid, -math.inf)
+    some = valid.any(-1)
+    logp, logp1 = torch.log_softmax(z / t, -1), torch.log_softmax(z, -1)
+    logq = teacher - (torch.logsumexp(teacher, -1) if lse is None else lse.double())[:, None]
+    q = torch.where(valid, logq.exp(), 0.0)
+    soft = torch.where(q > 0, q * (logq - logp.gather(-1, at)), 0.0).sum(-1)
+    listed = torch.zeros_like(z).scatter_add(-1, at, valid.double()) > 0
+    mass, ratio = q.sum(-1), torch.zeros_like(soft)
+    if lse is not None:
+        q_o, p_o = (1 - mass).clamp(min=0), logp.exp().masked_fill(listed, 0.0).sum(-1)
+        rest = (q_o > 0) & (p_o >= 2.0 ** -126)
+        ratio = torch.where(rest, q_o / p_o, 0.0)
+        soft = soft + torch.where(rest, q_o * torch.where(rest, ratio, 1.0).log(), 0.0)
+        mass = mass + torch.where(rest, q_o, 0.0)
+    q_at = torch.zeros_like(z).scatter_add(-1, at, q)
+    on = some[:, None].double() * alpha * t
+    grad = on * (logp.exp() * (mass[:, None] - torch.where(listed, 0.0, ratio[:, None])) - q_at)
+    size = on * (logp.exp() * (mass + ratio)[:, None] + q_at)
+    loss = torch.where(some, alpha * t * t * soft, 0.0)
+    if labels is not None:
+        known = (labels >= 0) & (labels < V)
+        y = labels.masked_fill(~known, 0)[:, None]
+        loss = loss + torch.where(known, (alpha - 1) * logp1.gather(-1, y)[:, 0], 0.0)
+        hit = torch.zeros_like(z).scatter(-1, y, 1.0)
+        on = known[:, None].double() * (1 - alpha)
+        grad, size = grad + on * (logp1.exp() - hit), size + on * ((logp1.exp() - hit).abs() + 2 * hit)
+    w = dloss.double()[:, None]
+    return loss, grad * w, size * w.abs()
+
+
+def near(got, want, slack):
+    """``check`` of test_step_operators, where the tensors are."""
+    half = torch.finfo(got.dtype).eps / 2
+    assert got.shape == want.shape and not torch.isnan(got).any()
+    off = (got.double() - want).abs() - (half * want.abs() * (1 + 2 ** -7) + slack)
+    assert float(off.max()) <= 0, f"off by {float(off.max()):.3g} more than allowed at {int(off.argmax())}"
+
+
+def uneven(rows, V, K, device, dtype, tail, labels, t, ids_dtype):
+    """Inputs whose rows differ in kind, so that what one leaves behind would show in the next: without entries, with repeated ones,
+    without a label or one that is listed, weightless, with logits far apart."""
+    logits, ids, top, lse, lab = distill_inputs(rows, V, K, device, dtype, tail, labels, t, ids_dtype)
+    dloss = rnd(9, rows, device=device)
+    kind = torch.arange(rows, device=device)
+    ids[kind % 7 == 3] = -1
+    if K > 2:
+        ids[kind % 5 == 1, 2] = ids[kind % 5 == 1, 0]           # an id twice (where there are entries)
+        ids[kind % 10 == 6, 1:] = ids[kind % 10 == 6, :1]       # and one K times
+    if lab is not None:
+        lab[kind % 4 == 2] = -1
+        lab[kind % 6 == 5] = ids[kind % 6 == 5, 0].long()
+    if lse is not None:
+        lse += 0.3
+    dloss[kind % 11 == 4] = 0.0
+    logits[kind % 13 == 12, V // 2:] += 120.0                   # far above the entries, where these lie below
+    return dloss, logits, ids, top, lse, lab
+
+
+SEVERAL = [  # rows, V, K, tail, labels, temperature, alpha
+    (2000, 130, 5, True, True, 1.0, 0.5), (3000, 257, 200, True, True, 2.0, 0.5), (2000, 4097, 100, False, True, 4.0, 0.5),
+    (900, 24000, 16, True, True, 1.5, 0.9), (1400, 12000, 300, True, False, 2.0, 1.0), (700, 50257, 100, False, False, 1.0, 1.0),
+    (500, 50257, 600, True, True, 2.0, 0.5),     # one CTA of 256 threads to an SM
+    (300, 70000, 64, True, True, 2.0, 0.5), (160, 70000, 64, True, True, 1.0, 0.5), (120, 128256, 300, True, True, 4.0, 0.5),
+    (90, 200000, 40, False, True, 1.5, 0.5), (60, 420000, 20, True, True, 2.0, 0.5),
+]
+
+
+def check_several(device, dtype, rows, V, K, tail, labels, t, alpha):
+    dloss, *args = uneven(rows, V, K, device, dtype, tail, labels, t, torch.int64 if K % 2 else torch.int32)
+    el, eg, size = exact_rows(dloss, *args, t, alpha)
+    rel = distill_slack(args[0], t)
+    slack = rel * 2 * max(1.0, t * t) * (1 + el.abs()) + 40 * U
+    near(ops.distill_loss(*args, t, alpha), el, slack)
+    loss, dz = ops.distill_loss_grad(dloss, *args, t, alpha)
+    near(loss, el, slack)
+    near(dz, eg, 2 * rel * size + 2.0 ** -126)
+    again = ops.distill_loss_grad(dloss, *args, t, alpha)
+    assert torch.equal(loss, again[0]) and torch.equal(dz, again[1])
+    return dloss, args, (el, eg, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V,K,tail,labels,t,alpha", SEVERAL)
+def test_several_rows_to_a_cta_or_cluster(dtype, rows, V, K, tail, labels, t, alpha):
+    check_several("cuda", dtype, rows, V, K, tail, labels, t, alpha)
+
+
+@pytest.mark.parametrize("tail,labels,t,alpha", [(True, True, 2.0, 0.5), (False, True, 1.0, 0.25), (True, False, 1.5, 1.0)])
+def test_rows_of_every_kind(tail, labels, t, alpha):
+    """The same rows on the CPU, and the two 64-bit forms against one another."""
+    dloss, args, got = check_several("cpu", torch.float32, 60, 90, 7, tail, labels, t, alpha)
+    for p, q in zip(got, distill_exact(dloss, *args, t, alpha)):
+        torch.testing.assert_close(p, q, rtol=1e-9, atol=1e-12)

@@ -814,23 +814,31 @@ static int launch_wgrad(const void* dy, const void* x, void* D, WgradParams& p, 
 // Small products are short of tiles, or of steps in a tile to hide its start and its store behind:
 //   8 x 2048 x 512      mean 250: - / 18 / 20      512 (8.6 GFLOP): - / 23 / 27      1024 (17 GFLOP): - / 35 / 33
 //   8 x 1024 x 4096     mean 128 (8.6 GFLOP): - / 33 / 35    192 (13 GFLOP): - / 33 / 37    250 (17 GFLOP): - / 49 / 39
-static int block_rows(int rows, int groups, int M, int K) {
+static int block_rows(int rows, int groups, int M, int K, int sms) {
   const int mean = (rows + groups - 1) / groups;
   if (mean <= 24) return 32;
   const long long pairs = ((long long)rows / 256 + groups) * ((M + 255) / 256);
-  const bool small = pairs < sm_count_of_device() / 4 || 2.0 * rows * M * K < 14e9;
+  const bool small = pairs < sms / 4 || 2.0 * rows * M * K < 14e9;
   return mean <= 96 || small ? 128 : 256;
 }
 // Parts that the reduction of a single CTA's tiles may have: none where the tiles may be more than half the SMs, or for reductions
 // of less than 2048, where their sum costs more than they save.  One token of two experts, us, whole / in parts: 4096 x 14336 59 / 45,
 // 4096 x 4096 21 / 16, 2048 x 8192 36 / 17, 1024 x 2048 13.1 / 10.4, 4096 x 2048 12.9 / 11.9, 4096 x 1024 9.4 / 10.9;
 // 300 rows of four, 256 x 4096, 22 / 14; 400 rows of eight, 512 x 4096, 21 / 14.5.
-static int most_parts(int rows, int groups, int M, int K) {
-  const int block = block_rows(rows, groups, M, K);
-  const long long tiles_m = (M + 127) / 128, blocks = rows / block + (rows < groups ? rows : groups), slots = sm_count_of_device();
+static int most_parts(int rows, int groups, int M, int K, int slots) {
+  const int block = block_rows(rows, groups, M, K, slots);
+  const long long tiles_m = (M + 127) / 128, blocks = rows / block + (rows < groups ? rows : groups);
   if (block == 256 || K < 2048 || 2 * blocks * tiles_m > slots) return 1;
   const long long most = slots / tiles_m;
   return int(most < SPLIT_MAX ? most : SPLIT_MAX);
+}
+// Tiles of 128 x 128 where pairs' 256 x 256 would leave most SMs without one, and for short groups, whose time is that of the
+// stores.  Measured, us, single / pairs: 8 x 512 x 512 (32 pairs) 8.2 / 10.2 with 16 rows a group, 16.4 / 18.4 with 1024, 32.8 / 36.9
+// with 4096; 4 x 1024 x 1024 (64 pairs) 20.5 / 18.4 with 1024, 53.2 / 34.8 with 4096; 64 x 2896 x 1864 194 / 304 with 4; 64 x 1408 x
+// 2048 102 / 108 with 16, 103 / 115 with 128, 156 / 145 with 256.
+static int wgrad_tile(int rows, int groups, int N, int K, int sms) {
+  const long long pairs = (long long)groups * ((N + 255) / 256) * ((K + 255) / 256);
+  return pairs < sms / 3 || (rows + groups - 1) / groups <= 128 ? 128 : 256;
 }
 static bool bad(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
@@ -852,13 +860,13 @@ JPB_API int jpb_linear_ragged(const void* tokens, const void* w, const int* offs
   p.offsets = offsets; p.groups = groups; p.rows = rows; p.M = transposed ? K : N; p.K = transposed ? N : K;
   p.w_blocked = transposed && p.M % 64 == 0; p.D = static_cast<__nv_bfloat16*>(out); p.status = jpb_status_device_ptr();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int parts = most_parts(rows, groups, p.M, p.K);
+  const int sms = sm_count_of_device(), parts = most_parts(rows, groups, p.M, p.K, sms);
   if (parts > 1) {
     if (!scratch || bad(scratch)) return -JPB_ERR_BAD_ARGUMENT;
     p.head = reinterpret_cast<int*>(scratch);
     p.parts = scratch + 4;
   }
-  const int block = block_rows(rows, groups, p.M, p.K);
+  const int block = block_rows(rows, groups, p.M, p.K, sms);
   const int rc = block == 32    ? launch_rows<1, 32>(w, tokens, p, transposed, s)
                  : block == 128 ? launch_rows<1, 128>(w, tokens, p, transposed, s)
                                 : launch_rows<2, 256>(w, tokens, p, transposed, s);
@@ -870,7 +878,7 @@ JPB_API int jpb_linear_ragged(const void* tokens, const void* w, const int* offs
 
 JPB_API long long jpb_linear_ragged_scratch_elems(int rows, int groups, int N, int K, int transposed) {
   if (rows <= 0 || groups <= 0) return 0;
-  const int M = transposed ? K : N, parts = jpb::ragged::most_parts(rows, groups, M, transposed ? N : K);
+  const int M = transposed ? K : N, parts = jpb::ragged::most_parts(rows, groups, M, transposed ? N : K, jpb::sm_count_of_device());
   return parts > 1 ? 4 + (long long)parts * rows * M : 0;
 }
 
@@ -888,11 +896,16 @@ JPB_API int jpb_linear_ragged_wgrad(const void* dy, const void* x, const int* of
   WgradParams p = {};
   p.offsets = offsets; p.groups = groups; p.rows = rows; p.N = N; p.K = K; p.dy_blocked = N % 64 == 0; p.x_blocked = K % 64 == 0;
   p.out_fp32 = out_fp32; p.accumulate = accumulate; p.status = jpb_status_device_ptr();
-  // Tiles of 128 x 128 where pairs' 256 x 256 would leave most SMs without one, and for short groups, whose time is that of the
-  // stores.  Measured, us, single / pairs: 8 x 512 x 512 (32 pairs) 8.2 / 10.2 with 16 rows a group, 16.4 / 18.4 with 1024, 32.8 / 36.9
-  // with 4096; 4 x 1024 x 1024 (64 pairs) 20.5 / 18.4 with 1024, 53.2 / 34.8 with 4096; 64 x 2896 x 1864 194 / 304 with 4; 64 x 1408 x
-  // 2048 102 / 108 with 16, 103 / 115 with 128, 156 / 145 with 256.
-  const long long pairs = (long long)groups * ((N + 255) / 256) * ((K + 255) / 256);
-  if (pairs < sm_count_of_device() / 3 || (rows + groups - 1) / groups <= 128) return launch_wgrad<1, 128>(dy, x, dw, p, s);
+  if (wgrad_tile(rows, groups, N, K, sm_count_of_device()) == 128) return launch_wgrad<1, 128>(dy, x, dw, p, s);
   return launch_wgrad<2, 256>(dy, x, dw, p, s);
 }
+
+// What a product of these sizes runs as on a device of `sms` SMs (for tests; rows and groups above zero): rows of the token operand in
+// a block (32 and 128 of single CTAs, 256 of a pair), plus 1024 times the most parts that a reduction may have; and the edge of the
+// weight gradient's tiles (128 single CTAs, 256 pairs).
+JPB_API int jpb_linear_ragged_form(int rows, int groups, int N, int K, int transposed, int sms) {
+  using namespace jpb::ragged;
+  const int M = transposed ? K : N, R = transposed ? N : K;
+  return block_rows(rows, groups, M, R, sms) + 1024 * most_parts(rows, groups, M, R, sms);
+}
+JPB_API int jpb_linear_ragged_wgrad_form(int rows, int groups, int N, int K, int sms) { return jpb::ragged::wgrad_tile(rows, groups, N, K, sms); }

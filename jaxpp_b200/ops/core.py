@@ -995,8 +995,9 @@ def _check_distill(dloss, logits, ids, top, lse, labels, temperature=1.0, alpha=
         raise ValueError(f"distill_loss: labels are {tuple(rows)} int64, got {tuple(labels.shape)} {labels.dtype}")
     if dloss is not None and dloss.shape != rows:
         raise ValueError(f"distill_loss_grad: dloss is {tuple(rows)}, got {tuple(dloss.shape)}")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"distill_loss: temperature has to be positive, got {temperature}")
+    # (logits over the temperature, and its square times a divergence, have to stay numbers that fp32 tells apart)
+    if not 2.0 ** -14 <= temperature <= 2.0 ** 14:
+        raise ValueError(f"distill_loss: temperature has to lie between 2^-14 and 2^14, got {temperature}")
     if not 0 <= alpha <= 1:
         raise ValueError(f"distill_loss: alpha has to lie between 0 and 1, got {alpha}")
 

@@ -249,3 +249,19 @@ def test_rows_of_every_kind(tail, labels, t, alpha):
     dloss, args, got = check_several("cpu", torch.float32, 60, 90, 7, tail, labels, t, alpha)
     for p, q in zip(got, distill_exact(dloss, *args, t, alpha)):
         torch.testing.assert_close(p, q, rtol=1e-9, atol=1e-12)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_temperatures(device):
+    """Those at both ends of the range are right, those outside of it are refused: at 1e-10 an exponent has no digit left, at 1e25
+    the square of the temperature is no number."""
+    for t in (2.0 ** -14, 2.0 ** -7, 64.0, 2.0 ** 14):
+        logits, ids, top, lse, labels = distill_inputs(5, 300, 6, device, torch.float32, True, True, t, torch.int64)
+        lse += 0.5
+        check_distill(device, logits, ids, top, lse, labels, t, 0.5)
+        check_distill(device, logits, ids, top, None, labels, t, 0.5)
+    for t in (0.0, 1e-10, 2.0 ** -15, 1e25, 20000.0, math.nan):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.distill_loss(logits, ids, top, lse, labels, t, 0.5)
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.distill_loss_grad(torch.ones(5, device=device), logits, ids, top, lse, labels, t, 0.5)

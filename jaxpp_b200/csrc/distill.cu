@@ -14,10 +14,10 @@
 // are written last.
 // What bounds it: HBM (a row read, and one written), then the exponentials, of which an SM does 16 a cycle: one per element for
 // the sums and one for the gradient.  With both temperatures in play the plain exponential is a power of the softened one where
-// t is 2 or 4, else it is taken too.  4096 x 32000 bf16, 64 entries: the loss 61 us (4.3 TB/s), with the gradient 104 us (5.0 TB/s;
-// a copy would take 80): both exponentials alone keep an SM for 58 us, the rest are the barriers between a row's phases, which the
-// two or three other CTAs of the SM do not quite cover.  Many entries cost their scattered reads and writes: 512 of them 98 and
-// 198 us.
+// t is 2 or 4, else it is taken too.  4096 x 32000 bf16, 64 entries: the loss 60 us (4.4 TB/s; its bytes take 40, one exponential an
+// element 29), with the gradient 106 us (4.9 TB/s; a copy would take 80, both exponentials 58): the rest are the barriers between a
+// row's phases, which the two or three other CTAs of the SM do not quite cover.  Many entries cost their scattered reads and writes:
+// 512 of them 98 and 198 us.
 #include "launch.cuh"
 #include "vec.cuh"
 

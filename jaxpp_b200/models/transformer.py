@@ -79,7 +79,9 @@ class ModelConfig:
     dropless: bool = False
     # RMSNorm families: the output of each half of a block is normalised too, before it joins the residual stream:
     #   x <- residual_scale * x + gate * RMSNorm(half(RMSNorm(x)))
-    # ``residual_gate`` is the initial value of learned gates, one per channel and half (None: no gates)
+    # ``residual_gate`` is the initial value of learned gates, one per channel and half (None: no gates).  A whole block takes
+    # the norm in front of its feed-forward half of the unrounded stream, a stage that ends in half a block hands on the
+    # rounded one: in 16 bits such a boundary changes the values by that rounding
     sandwich_norm: bool = False
     residual_scale: float = 1.0
     residual_gate: float | None = None

@@ -629,7 +629,6 @@ template <typename T, bool GRAD>
 static int distill_mode(DistillParams p, cudaStream_t stream) {
   const int sms = sm_count_of_device();
   const DistillShape s = distill_shape(p.rows, p.V, p.K, sizeof(T), GRAD, sms);
-  if (s.smem > 220 * 1024) return -JPB_ERR_BAD_ARGUMENT;     // a row of more than 8 x (220 KB - 24 K)
   p.log_cluster = s.cluster == 8 ? 3 : s.cluster == 4 ? 2 : s.cluster == 2;
   p.buffer = s.buffer;
   p.status = jpb_status_device_ptr();
@@ -651,7 +650,8 @@ JPB_API int jpb_distill(int dt, const float* dloss, const void* logits, const vo
                         long long rows, int V, int K, void* stream) {
   using namespace jpb;
   if (rows <= 0) return 0;
-  if (V <= 0 || K < 0 || K > DISTILL_MAX_K || V > (8 * 220 * 1024) / (dt == 0 ? 4 : 2) || (dlogits && !dloss) ||
+  // (a part of the largest row and its entries take up to 163 bytes more than 220 KB, of the 227 that a CTA may have)
+  if (V <= 0 || K < 0 || K > DISTILL_MAX_K || (long long)V * (dt == 0 ? 4 : 2) > 8ll * (220 * 1024 - 24 * K) || (dlogits && !dloss) ||
       ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) & 15))
     return -JPB_ERR_BAD_ARGUMENT;
   DistillParams p = {logits, ids, top, lse, labels, dloss, loss, dlogits, rows, V, K, ids64, top_fp32, temperature, alpha, 0, 0, nullptr};

@@ -205,7 +205,8 @@ def uneven(rows, V, K, device, dtype, tail, labels, t, ids_dtype):
         ids[kind % 10 == 6, 1:] = ids[kind % 10 == 6, :1]       # and one K times
     if lab is not None:
         lab[kind % 4 == 2] = -1
-        lab[kind % 6 == 5] = ids[kind % 6 == 5, 0].long()
+        if K:
+            lab[kind % 6 == 5] = ids[kind % 6 == 5, 0].long()
     if lse is not None:
         lse += 0.3
     dloss[kind % 11 == 4] = 0.0
@@ -265,3 +266,17 @@ def test_temperatures(device):
             ops.distill_loss(logits, ids, top, lse, labels, t, 0.5)
         with pytest.raises((ValueError, RuntimeError)):
             ops.distill_loss_grad(torch.ones(5, device=device), logits, ids, top, lse, labels, t, 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [0, 1, 64, 1024])
+def test_the_largest_rows(dtype, K):
+    """Rows of 8 times (220 KB less 24 bytes an entry) are taken, with any start of a row on its 16 bytes; longer ones are refused."""
+    from jaxpp_b200.ops import native
+
+    most = 8 * (220 * 1024 - 24 * K) // dtype.itemsize
+    for V in (most, most - 1, most - 3):
+        check_several("cuda", dtype, 3, V, K, K % 2 == 0, True, 2.0, 0.5)
+    with pytest.raises(native.NativeError):
+        ops.distill_loss(*distill_inputs(2, most + 1, K, "cuda", dtype), 1.0, 0.5)

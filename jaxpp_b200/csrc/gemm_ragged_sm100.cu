@@ -25,6 +25,7 @@ constexpr int W_BYTES = 128 * BK * 2;          // 128 rows of the M operand per 
 constexpr int SMEM_MAX = 227 * 1024;
 constexpr int BAR_BYTES = 256;
 constexpr int MAX_GROUPS = 1024;
+constexpr int MAX_ROWS = 0x7fffffff - (1 << 16);      // a step past the last row, by a block at most, stays within 32 bits
 constexpr int TABLE_BYTES = 2 * (MAX_GROUPS + 1) * 4 + 8;
 constexpr int GROUP_BLOCKS = 2048;             // token rows that are walked together: they stay in L2 while W streams
 
@@ -853,7 +854,7 @@ JPB_API int jpb_linear_ragged(const void* tokens, const void* w, const int* offs
                               int transposed, float* scratch, void* stream) {
   using namespace jpb;
   using namespace jpb::ragged;
-  if (rows < 0 || groups < 1 || groups > MAX_GROUPS || N <= 0 || K <= 0 || (N & 7) || (K & 7) || bad(tokens) || bad(w) || bad(out))
+  if (rows < 0 || rows > MAX_ROWS || groups < 1 || groups > MAX_GROUPS || N <= 0 || K <= 0 || (N & 7) || (K & 7) || bad(tokens) || bad(w) || bad(out))
     return -JPB_ERR_BAD_ARGUMENT;
   if (rows == 0) return 0;
   RowsParams p = {};
@@ -888,7 +889,7 @@ JPB_API int jpb_linear_ragged_wgrad(const void* dy, const void* x, const int* of
                                     int out_fp32, int accumulate, void* stream) {
   using namespace jpb;
   using namespace jpb::ragged;
-  if (rows < 0 || groups < 1 || groups > MAX_GROUPS || N <= 0 || K <= 0 || (N & 7) || (K & 7) || bad(dy) || bad(x) || bad(dw) ||
+  if (rows < 0 || rows > MAX_ROWS || groups < 1 || groups > MAX_GROUPS || N <= 0 || K <= 0 || (N & 7) || (K & 7) || bad(dy) || bad(x) || bad(dw) ||
       (accumulate && !out_fp32))
     return -JPB_ERR_BAD_ARGUMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

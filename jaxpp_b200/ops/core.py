@@ -268,6 +268,9 @@ _autograd("linear_batched", _linear_batched_bwd, _linear_batched_setup)
 # that decrease or leave 0 .. T are taken as the nearest ones that do not.
 # ======================================================================================
 
+MAX_RAGGED_ROWS = 2 ** 31 - 2 ** 16     # the kernels step past a group's end, by a block at most, in 32 bits
+
+
 def _check_ragged(rows, w, offsets, width, what):
     if rows.dim() != 2 or w.dim() != 3 or rows.shape[1] != w.shape[width]:
         raise ValueError(f"{what}: rows {tuple(rows.shape)} and weights {tuple(w.shape)} do not go together "
@@ -278,8 +281,8 @@ def _check_ragged(rows, w, offsets, width, what):
 def _check_offsets(rows, offsets, groups, what):
     if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.shape[0] < 2 or (groups is not None and offsets.shape[0] != groups + 1):
         raise ValueError(f"{what}: offsets are [groups + 1] int32, got {tuple(offsets.shape)} {offsets.dtype}")
-    if rows.shape[0] >= 2 ** 31:
-        raise ValueError(f"{what}: fewer than 2^31 rows, got {rows.shape[0]}")
+    if rows.shape[0] >= MAX_RAGGED_ROWS:
+        raise ValueError(f"{what}: fewer than 2^31 - 2^16 rows, got {rows.shape[0]}")
     if offsets.device != rows.device:
         raise ValueError(f"{what}: offsets are on {offsets.device}, the rows on {rows.device}")
 

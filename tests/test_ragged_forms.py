@@ -128,3 +128,22 @@ def test_products_repeat_bit_for_bit():
         first = call()
         for _ in range(20):
             assert all(torch.equal(p, q) for p, q in zip(call(), first)), (sizes, N, K)
+
+
+def test_most_rows():
+    """Row numbers have room for a step past the last one in 32 bits: more rows are refused, here and at the C entry (without memory for
+    them: the entry looks at the sizes first)."""
+    most = ops.MAX_RAGGED_ROWS - 1
+    meta = lambda *shape: torch.empty(*shape, dtype=torch.bfloat16, device="meta")
+    w, offsets = meta(2, 16, 8), torch.empty(3, dtype=torch.int32, device="meta")
+    assert ops.linear_ragged(meta(most, 8), w, offsets).shape == (most, 16)
+    assert ops.linear_ragged_wgrad(meta(most, 16), meta(most, 8), offsets).shape == (2, 16, 8)
+    for call in (lambda n: ops.linear_ragged(meta(n, 8), w, offsets), lambda n: ops.linear_ragged_dgrad(meta(n, 16), w, offsets),
+                 lambda n: ops.linear_ragged_wgrad(meta(n, 16), meta(n, 8), offsets)):
+        for n in (most + 1, 2 ** 31 - 1, 2 ** 31):
+            with pytest.raises(ValueError):
+                call(n)
+    lib = native.load()
+    for n in (most + 1, 2 ** 31 - 1):
+        assert lib.jpb_linear_ragged(None, None, None, None, n, 2, 16, 8, 0, None, None) == -2
+        assert lib.jpb_linear_ragged_wgrad(None, None, None, None, n, 2, 16, 8, 0, 0, None) == -2
